@@ -354,8 +354,10 @@ PYBIND11_MODULE(_core, m) {
       "flash_attn_fwd",
       [](uintptr_t q, uintptr_t k, uintptr_t v, uintptr_t o, uintptr_t lse, long long qsb, long long qst,
          long long ksb, long long kst, long long vsb, long long vst, long long osb, long long ost, int B, int H, int T,
-         int D, float scale, bool causal, uintptr_t s) {
+         int D, float scale, bool causal, uintptr_t s, int window, int sinks) {
         AttnParams p{};
+        p.window = window;
+        p.sinks = sinks;
         p.q = P<const __nv_bfloat16>(q);
         p.k = P<const __nv_bfloat16>(k);
         p.v = P<const __nv_bfloat16>(v);
@@ -376,15 +378,21 @@ PYBIND11_MODULE(_core, m) {
         p.scale = scale;
         p.causal = causal ? 1 : 0;
         flash_attn_fwd(p, S(s));
-      });
+      },
+      py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("lse"), py::arg("qsb"), py::arg("qst"),
+      py::arg("ksb"), py::arg("kst"), py::arg("vsb"), py::arg("vst"), py::arg("osb"), py::arg("ost"),
+      py::arg("B"), py::arg("H"), py::arg("T"), py::arg("D"), py::arg("scale"), py::arg("causal"),
+      py::arg("stream"), py::arg("window") = 0, py::arg("sinks") = 0);
   m.def(
       "flash_attn_bwd",
       [](uintptr_t q, uintptr_t k, uintptr_t v, uintptr_t o, uintptr_t lse, uintptr_t dout, uintptr_t dq, uintptr_t dk,
          uintptr_t dv, uintptr_t delta, uintptr_t dq_accum, long long qsb, long long qst, long long ksb, long long kst,
          long long vsb, long long vst, long long osb, long long ost, long long dosb, long long dost, long long dqsb,
          long long dqst, long long dksb, long long dkst, long long dvsb, long long dvst, int B, int H, int T, int D,
-         float scale, bool causal, uintptr_t s) {
+         float scale, bool causal, uintptr_t s, int window, int sinks) {
         AttnBwdParams p{};
+        p.f.window = window;
+        p.f.sinks = sinks;
         p.f.q = P<const __nv_bfloat16>(q);
         p.f.k = P<const __nv_bfloat16>(k);
         p.f.v = P<const __nv_bfloat16>(v);
@@ -419,7 +427,13 @@ PYBIND11_MODULE(_core, m) {
         p.delta = P<float>(delta);
         p.dq_accum = P<float>(dq_accum);
         flash_attn_bwd(p, S(s));
-      });
+      },
+      py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("lse"), py::arg("dout"), py::arg("dq"),
+      py::arg("dk"), py::arg("dv"), py::arg("delta"), py::arg("dq_accum"), py::arg("qsb"), py::arg("qst"),
+      py::arg("ksb"), py::arg("kst"), py::arg("vsb"), py::arg("vst"), py::arg("osb"), py::arg("ost"),
+      py::arg("dosb"), py::arg("dost"), py::arg("dqsb"), py::arg("dqst"), py::arg("dksb"), py::arg("dkst"),
+      py::arg("dvsb"), py::arg("dvst"), py::arg("B"), py::arg("H"), py::arg("T"), py::arg("D"),
+      py::arg("scale"), py::arg("causal"), py::arg("stream"), py::arg("window") = 0, py::arg("sinks") = 0);
 
   m.def("set_attn_bwd_trace", [](uintptr_t buf) { set_attn_bwd_trace(P<unsigned long long>(buf)); });
   m.def("set_attn_fwd_trace", [](uintptr_t buf) { set_attn_fwd_trace(P<unsigned long long>(buf)); });

@@ -526,7 +526,8 @@ void bwd_impl(const AttnBwdParams& p, cudaStream_t s) {
     const char* e = getenv("UHFS_ATTN_BWD");
     return e != nullptr && std::string(e) == "mma_sync";
   }();
-  if (!legacy && flash_attn_bwd_tc_supported(p)) {
+  // a window runs on the tcgen05 kernel only (checked by flash_attn_bwd)
+  if (p.f.window > 0 || (!legacy && flash_attn_bwd_tc_supported(p))) {
     flash_attn_bwd_tc_main(p, s);
   } else {
     dim3 grid((p.f.T + 63) / 64, p.f.B * p.f.H);
@@ -540,10 +541,26 @@ void bwd_impl(const AttnBwdParams& p, cudaStream_t s) {
   note_launch();
 }
 
+void check_window(const AttnParams& p, bool supported) {
+  if (p.window < 0 || p.sinks < 0) throw std::runtime_error("flash attention: window and sinks must not be negative");
+  if (p.window == 0) return;
+  if (!p.causal) throw std::runtime_error("flash attention: a sliding window needs causal attention");
+  // the masks compare i - window and j + window in 32 bits
+  if (p.window > (1 << 30) || p.sinks > (1 << 30)) throw std::runtime_error("flash attention: window or sinks too large");
+  if (!supported)
+    throw std::runtime_error("flash attention: a sliding window needs head_dim 64 or 128 and the fused q | k | v "
+                             "layout with 16-byte aligned rows");
+}
+
 }  // namespace
 
 void flash_attn_fwd(const AttnParams& p, cudaStream_t s) {
   if (p.T <= 0 || p.B <= 0 || p.H <= 0) return;
+  check_window(p, flash_attn_fwd_tc_supported(p));
+  if (p.window > 0) {
+    flash_attn_fwd_tc(p, s);
+    return;
+  }
   static const bool legacy = [] {
     const char* e = getenv("UHFS_ATTN_FWD");
     return e != nullptr && std::string(e) == "mma_sync";
@@ -560,6 +577,7 @@ void flash_attn_fwd(const AttnParams& p, cudaStream_t s) {
 
 void flash_attn_bwd(const AttnBwdParams& p, cudaStream_t s) {
   if (p.f.T <= 0 || p.f.B <= 0 || p.f.H <= 0) return;
+  check_window(p.f, flash_attn_bwd_tc_supported(p));
   // the delta / dQ helper kernels move 8 elements per 16-byte access
   auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
   if (!al16(p.f.o) || !al16(p.dout) || !al16(p.dq) || !al16(p.dq_accum) || p.f.o_stride_t % 8 != 0 ||

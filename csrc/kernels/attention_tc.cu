@@ -27,6 +27,15 @@
 // Registers: 384 threads launch with 168 each; warpgroup 2 (producer, MMA,
 // two idle warps) gives back down to 96 and the softmax warpgroups take 200,
 // within the launch total (the host checks the launch count).
+// Sliding window with sinks (kWin): query i sees key j <= i when i - j < window
+// or j < sinks, so tile A needs the sink blocks [0, ceil(sinks / 128)) and the
+// blocks from (m0 - window + 1) / 128 to its diagonal; blocks between the two
+// are never loaded.  Both tiles walk tile A's list (tile B ends one block
+// later and skips the first window block where the window has left it), and
+// the masks cost compares only in blocks that hold a mask edge.  q / k / v are
+// read through a [B][T][3F] map whose rows past T are zeros, so a sequence of
+// ragged length never multiplies its zero probabilities with another
+// sequence's values.
 // Every mbarrier wait is bounded; waits that precede warp-collective TMEM
 // instructions return a warp-uniform result.
 // Reference: the single-head fp32 kernel cuda/kernels.cu:147-188 and the
@@ -45,6 +54,9 @@ namespace uhfs {
 
 CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
                               uint32_t box_inner, uint32_t box_outer);
+CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
+                              uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
+                              uint32_t box_rows);
 
 namespace {
 
@@ -99,6 +111,7 @@ struct FwdArgs {
   long long F;            // H * D (columns per q / k / v section)
   float sl2;              // softmax scale * log2(e)
   int causal;
+  int window, sinks;      // kWin only
   __nv_bfloat16* o;
   long long o_stride_t;   // elements between tokens of o (rows are [b*T + t])
   float* lse;             // [B, H, T] (log2 domain)
@@ -125,7 +138,7 @@ struct FwdArgs {
 // exp2_poly3_x2 (packed FMA-pipe polynomial) instead of ex2.approx (MUFU), so
 // the exponentials of a block split between the two pipes
 // (UHFS_ATTN_POLY=0|2|3|4 selects it; 0 = MUFU only).
-template <int D, int kPoly>
+template <int D, int kPoly, bool kWin>
 __global__ void __launch_bounds__(kThreads, 1)
     fa_fwd_tc_kernel(const __grid_constant__ CUtensorMap tm_qkv, const FwdArgs a) {
   using Cfg = FwdCfg<D>;
@@ -158,6 +171,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the longest (causal) query blocks come first in item order
   struct Item {
     int bh, b, h, m0, nA, nB, cta;
+    // kWin: list entry i is key block i for i < ns (sinks), lo + i - ns after;
+    // tile B has no work in entry skipB (-1: none)
+    int ns, lo, skipB;
   };
   auto decode = [&](int it) {
     Item w;
@@ -168,8 +184,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     w.m0 = mb * (2 * BQ);
     w.nA = a.causal ? min(kv_blocks, w.m0 / BKV + 1) : kv_blocks;
     w.nB = a.causal ? min(kv_blocks, w.m0 / BKV + 2) : kv_blocks;
+    if constexpr (kWin) {
+      w.lo = max(0, w.m0 - a.window + 1) / BKV;
+      w.ns = min(w.lo, (a.sinks + BKV - 1) / BKV);
+      w.nA += w.ns - w.lo;
+      w.nB += w.ns - w.lo;
+      // tile B's window starts at m0 + BQ - window + 1; its last entry is never skipped
+      const bool past = max(0, w.m0 + BQ - a.window + 1) / BKV > w.lo;
+      w.skipB = (past && w.lo * BKV >= a.sinks && w.nB - w.ns >= 2) ? w.ns : -1;
+    }
     w.cta = n_mblocks - 1 - mb;  // trace index (query blocks from the last)
     return w;
+  };
+
+  // key block of list entry i
+  [[maybe_unused]] auto block_of = [&](const Item& w, int i) {
+    if constexpr (kWin) return i < w.ns ? i : w.lo + i - w.ns;
+    return i;
   };
 
   constexpr int kProducerWarp = 8, kMmaWarp = 9;
@@ -219,12 +250,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Q of the previous item is no longer read by the tensor core
         if (!mbar_wait_bounded(q_empty, (k & 1u) ^ 1u, a.status, kErrWaitTimeoutEmpty, 203)) break;
         FWD_TRACE(w.cta, kTrStart, 0);
-        const int row0 = w.b * T;
+        [[maybe_unused]] const int row0 = w.b * T;
         mbar_arrive_expect_tx(q_full, 2 * Cfg::kTile);
         for (int t = 0; t < 2; ++t)
-          for (int kd = 0; kd < KD; ++kd)
-            tma_load_2d(sQ + t * Cfg::kTile + kd * (BQ * 128), &tm_qkv, q_full, (int)(w.h * D + kd * 64),
-                        row0 + w.m0 + t * BQ);
+          for (int kd = 0; kd < KD; ++kd) {
+            if constexpr (kWin)
+              tma_load_3d(sQ + t * Cfg::kTile + kd * (BQ * 128), &tm_qkv, q_full, (int)(w.h * D + kd * 64),
+                          w.m0 + t * BQ, w.b);
+            else
+              tma_load_2d(sQ + t * Cfg::kTile + kd * (BQ * 128), &tm_qkv, q_full, (int)(w.h * D + kd * 64),
+                          row0 + w.m0 + t * BQ);
+          }
         for (int i = 0; i < 2 * w.nB; ++i, ++L) {  // K_0, V_0, K_1, V_1, ...
           const uint32_t slot = L % NS, use = L / NS;
           if (!mbar_wait_bounded(&slot_empty[slot], (use & 1u) ^ 1u, a.status, kErrWaitTimeoutEmpty, 200)) {
@@ -234,9 +270,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint8_t* dst = sRing + slot * Cfg::kTile;
           mbar_arrive_expect_tx(&slot_full[slot], Cfg::kTile);
           const int col = (int)((i & 1) ? 2 * a.F : a.F) + w.h * D;
-          const int row = row0 + (i >> 1) * BKV;
-          for (int kd = 0; kd < KD; ++kd)
-            tma_load_2d(dst + kd * (BKV * 128), &tm_qkv, &slot_full[slot], col + kd * 64, row);
+          const int row = block_of(w, i >> 1) * BKV;
+          for (int kd = 0; kd < KD; ++kd) {
+            if constexpr (kWin)
+              tma_load_3d(dst + kd * (BKV * 128), &tm_qkv, &slot_full[slot], col + kd * 64, row, w.b);
+            else
+              tma_load_2d(dst + kd * (BKV * 128), &tm_qkv, &slot_full[slot], col + kd * 64, row0 + row);
+          }
         }
       }
       // drain: every issued copy lands before the CTA exits
@@ -265,6 +305,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Item w = decode(it);
         const bool tr_on = a.trace != nullptr && w.bh == a.trace_bh;
         (void)tr_on;
+        // list entries in which a tile has work, and its first one
+        auto active = [&](int t, int j) {
+          if constexpr (kWin) return t == 0 ? j < w.nA : j != w.skipB;
+          return t != 0 || j < w.nA;
+        };
+        auto first = [&](int t) {
+          if constexpr (kWin) return (t != 0 && w.skipB == 0) ? 1 : 0;
+          return 0;
+        };
         auto issue_s = [&](int t, int j) -> bool {
           if (s_cnt[t] > 0 &&
               !mbar_wait_bounded(&s_free[t], (s_cnt[t] - 1) & 1u, a.status, kErrWaitTimeoutAccum, 211))
@@ -287,14 +336,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                  kErrWaitTimeoutFull, 213))
             return false;
           // the previous item's O_t must have been read out before this item's first PV overwrites it
-          if (j == 0 && k > 0 && !mbar_wait_bounded(&o_free[t], (k - 1) & 1u, a.status, kErrWaitTimeoutAccum, 216))
+          if (j == first(t) && k > 0 && !mbar_wait_bounded(&o_free[t], (k - 1) & 1u, a.status, kErrWaitTimeoutAccum, 216))
             return false;
           tc_fence_after();
           const uint64_t ad = kmaj + p16 + t * (Cfg::kPBytes >> 4);
           const uint64_t bd = mnmaj + ring16 + slot_of(L + 2 * j + 1) * (Cfg::kTile >> 4);
 #pragma unroll
           for (int kk = 0; kk < BKV / 16; ++kk) {
-            const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
+            const uint32_t acc = (j > first(t) || kk > 0) ? 1u : 0u;
             if constexpr (Cfg::kPTmem) {
               // A = P_t from TMEM: keys [16 kk, 16 kk + 16) are columns [8 kk, 8 kk + 8)
               tc_mma_f16_ts(tmem + Cfg::kOCol + t * D, tmem + Cfg::kPCol + t * (BKV / 2) + (uint32_t)(kk * 8),
@@ -321,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           FWD_TRACE(w.cta, kTrKFull, j);
-          if ((j < w.nA && !issue_s(0, j)) || !issue_s(1, j)) {
+          if ((active(0, j) && !issue_s(0, j)) || (active(1, j) && !issue_s(1, j))) {
             ok = false;
             break;
           }
@@ -329,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j == w.nB - 1) tc_commit(q_empty);        // the item's last S products: Q is free
           FWD_TRACE(w.cta, kTrIssueS, j);
           if (j >= 1) {
-            if ((j - 1 < w.nA && !issue_pv(0, j - 1)) || !issue_pv(1, j - 1)) {
+            if ((active(0, j - 1) && !issue_pv(0, j - 1)) || (active(1, j - 1) && !issue_pv(1, j - 1))) {
               ok = false;
               break;
             }
@@ -338,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (ok && w.nB > 0) {
-          if ((w.nB - 1 < w.nA && !issue_pv(0, w.nB - 1)) || !issue_pv(1, w.nB - 1)) ok = false;
+          if ((active(0, w.nB - 1) && !issue_pv(0, w.nB - 1)) || !issue_pv(1, w.nB - 1)) ok = false;
           else tc_commit(&slot_empty[slot_of(L + 2 * (w.nB - 1) + 1)]);
         }
         L += 2 * w.nB;
@@ -369,7 +418,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nblk = t ? w.nB : w.nA;
       const int key_limit = a.causal ? min(q + 1, T) : T;  // keys [0, key_limit) are visible
       float m_run = -INFINITY, l_run = 0.f;
-      for (int j = 0; j < nblk && ok; ++j, ++blk) {
+      const int j_first = (kWin && t != 0 && w.skipB == 0) ? 1 : 0;
+      for (int j = j_first; j < nblk && ok; ++j, ++blk) {
+        if constexpr (kWin) {
+          if (t != 0 && j == w.skipB) ++j;  // never the last entry
+        }
         if (!mbar_wait_warp(&s_full[t], blk & 1u, a.status, kErrWaitTimeoutAccum, 220)) {
           ok = false;
           break;
@@ -383,8 +436,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&s_free[t]);  // S_t may be overwritten by the next block
         if (tracer && t == 0) FWD_TRACE(w.cta, kTrSRegsA, j);
-        const int lim = key_limit - j * BKV;  // visible columns of this block: [0, lim)
-        if (lim < BKV) {
+        const int key0 = block_of(w, j) * BKV;
+        const int lim = key_limit - key0;  // visible columns of this block: [0, lim)
+        if constexpr (kWin) {
+          // and of those the columns from `low` on (the window) or below `snk` (the sinks)
+          const int low = q - a.window + 1 - key0, snk = a.sinks - key0;
+          if (lim < BKV || (low > 0 && snk < BKV)) {
+#pragma unroll
+            for (int i = 0; i < BKV; ++i)
+              if (i >= lim || (i < low && i >= snk)) sr[i] = __float_as_uint(-INFINITY);
+          }
+        } else if (lim < BKV) {
 #pragma unroll
           for (int i = 0; i < BKV; ++i)
             if (i >= lim) sr[i] = __float_as_uint(-INFINITY);
@@ -428,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         m_run = m_new;
         if (tracer && t == 0) FWD_TRACE(w.cta, kTrExpA, j);
         // PV(j-1) finished: the P tile is free and O_t holds blocks < j
-        if (j > 0) {
+        if (j > j_first) {
           if (!mbar_wait_warp(&o_done[t], (blk - 1) & 1u, a.status, kErrWaitTimeoutAccum, 221)) {
             ok = false;
             break;
@@ -505,30 +567,35 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int D, int kPoly>
+template <int D, int kPoly, bool kWin = false>
 void launch_fwd(const AttnParams& p, cudaStream_t s) {
   using Cfg = FwdCfg<D>;
   static PerDeviceOnce once;
   once([] {
-    UHFS_CUDA_CHECK(cudaFuncSetAttribute(fa_fwd_tc_kernel<D, kPoly>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    UHFS_CUDA_CHECK(cudaFuncSetAttribute(fa_fwd_tc_kernel<D, kPoly, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          Cfg::kSmem));
     // setmaxnreg redistributes exactly the launch allocation; any other
     // launch count would make the increase wait for registers that never come
     cudaFuncAttributes fa{};
-    UHFS_CUDA_CHECK(cudaFuncGetAttributes(&fa, fa_fwd_tc_kernel<D, kPoly>));
+    UHFS_CUDA_CHECK(cudaFuncGetAttributes(&fa, fa_fwd_tc_kernel<D, kPoly, kWin>));
     if (fa.numRegs != kLaunchRegs)
       throw std::runtime_error("fa_fwd_tc_kernel: compiled with " + std::to_string(fa.numRegs) +
                                " registers per thread, the register split needs " + std::to_string(kLaunchRegs));
   });
   const long long F = (long long)p.H * D;
   // q, k, v are column blocks of one [B*T, 3F] matrix (the fused projection)
-  CUtensorMap tm = make_tmap_bf16_2d(p.q, (uint64_t)(3 * F), (uint64_t)p.B * p.T, (uint64_t)p.q_stride_t, 64, 128);
+  CUtensorMap tm =
+      kWin ? make_tmap_bf16_3d(p.q, (uint64_t)(3 * F), (uint64_t)p.T, (uint64_t)p.B, (uint64_t)p.q_stride_t,
+                               (uint64_t)p.q_stride_b, 64, 128)
+           : make_tmap_bf16_2d(p.q, (uint64_t)(3 * F), (uint64_t)p.B * p.T, (uint64_t)p.q_stride_t, 64, 128);
   FwdArgs a{};
   a.H = p.H;
   a.T = p.T;
   a.F = F;
   a.sl2 = p.scale * kLog2e;
   a.causal = p.causal;
+  a.window = p.window;
+  a.sinks = p.sinks;
   a.o = p.o;
   a.o_stride_t = p.o_stride_t;
   a.lse = p.lse;
@@ -550,7 +617,7 @@ void launch_fwd(const AttnParams& p, cudaStream_t s) {
   if (sms == 0) UHFS_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const int grid = (int)(items < sms ? items : sms);
   if (grid <= 0) return;
-  fa_fwd_tc_kernel<D, kPoly><<<grid, kThreads, Cfg::kSmem, s>>>(tm, a);
+  fa_fwd_tc_kernel<D, kPoly, kWin><<<grid, kThreads, Cfg::kSmem, s>>>(tm, a);
   note_launch();
   UHFS_CUDA_CHECK(cudaGetLastError());
 }
@@ -586,6 +653,7 @@ void flash_attn_fwd_tc(const AttnParams& p, cudaStream_t s) {
   }();
   auto go = [&](auto dtag) {
     constexpr int D = decltype(dtag)::value;
+    if (p.window > 0) return launch_fwd<D, kDefaultPolyPairs, true>(p, s);
     switch (poly) {
       case 2: return launch_fwd<D, 2>(p, s);
       case 3: return launch_fwd<D, 3>(p, s);

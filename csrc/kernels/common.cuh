@@ -181,6 +181,14 @@ __device__ __forceinline__ void tma_reduce_add_2d(const void* tmap, const void* 
       : "memory");
 }
 
+__device__ __forceinline__ void tma_reduce_add_3d(const void* tmap, const void* smem_src, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(tmap)),
+      "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
 // Shared tile -> global through the tensor map (TMA store); elements outside
 // the tensor are not written.  Same coordinate rules as the reduce above.
 __device__ __forceinline__ void tma_store_2d(const void* tmap, const void* smem_src, int coord0, int coord1) {

@@ -1420,6 +1420,42 @@ CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, 
   return m;
 }
 
+// [batch][rows][inner] maps: a box that runs past `rows` reads zeros and writes
+// nothing, so it never touches the next batch's rows.
+namespace {
+CUtensorMap make_tmap_3d(CUtensorMapDataType type, uint64_t elem, const void* base, uint64_t inner, uint64_t rows,
+                         uint64_t batch, uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
+                         uint32_t box_rows) {
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0) throw std::runtime_error("TMA base must be 16-byte aligned");
+  if ((row_stride_elems * elem) % 16 != 0 || (batch_stride_elems * elem) % 16 != 0)
+    throw std::runtime_error("TMA strides must be multiples of 16 bytes");
+  CUtensorMap m;
+  cuuint64_t dims[3] = {inner, rows, batch};
+  cuuint64_t strides[2] = {row_stride_elems * elem, batch_stride_elems * elem};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode_fn()(&m, type, 3, const_cast<void*>(base), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return m;
+}
+}  // namespace
+
+CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
+                              uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
+                              uint32_t box_rows) {
+  return make_tmap_3d(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, inner, rows, batch, row_stride_elems,
+                      batch_stride_elems, box_inner, box_rows);
+}
+
+CUtensorMap make_tmap_f32_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
+                             uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
+                             uint32_t box_rows) {
+  return make_tmap_3d(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, inner, rows, batch, row_stride_elems,
+                      batch_stride_elems, box_inner, box_rows);
+}
+
 CUtensorMap make_tmap_f32_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
                              uint32_t box_inner, uint32_t box_outer) {
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0) throw std::runtime_error("TMA base must be 16-byte aligned");

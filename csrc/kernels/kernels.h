@@ -92,6 +92,10 @@ struct AttnParams {
   int B, H, T, D;
   float scale;
   int causal;
+  // sliding window (causal only): query i sees key j <= i when i - j < window
+  // or j < sinks; window = 0 means no window
+  int window;
+  int sinks;
 };
 struct AttnBwdParams {
   AttnParams f;

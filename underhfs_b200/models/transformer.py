@@ -48,6 +48,10 @@ class LMSpec:
     tied: bool = False
     eps: float = 1e-8
     bias: bool = True
+    # sliding-window attention: token i sees the last `window` tokens up to
+    # itself and the first `sinks` tokens (None: the whole context)
+    window: int | None = None
+    sinks: int = 0
 
     @property
     def head_dim(self) -> int:
@@ -73,10 +77,17 @@ class LMSpec:
         return int(tokens * (self.layers * per_block + 2 * self.vocab_size + transient))
 
     def train_flops_per_token(self, seq_len: int) -> float:
-        """6N for the dense weights + causal attention (fwd 2 matmuls, bwd 4)."""
+        """6N for the dense weights + causal attention (fwd 2 matmuls, bwd 4)
+        over the keys that a token sees on average."""
         dense = 6.0 * (self.num_params() - self.vocab_size * self.features - self.max_seq_len * self.features)
         dense += 6.0 * self.vocab_size * self.features  # head (tied or not)
-        attn = self.layers * 3 * 2 * 2 * seq_len * self.features / 2  # causal half
+        keys = seq_len / 2  # causal half
+        if self.window is not None and self.window < seq_len:
+            # token i sees min(i, window) keys and the sinks that the window has left
+            far = seq_len - self.window
+            keys = self.window - self.window * self.window / (2 * seq_len)
+            keys += far * min(self.sinks, far) / seq_len - min(self.sinks, far) ** 2 / (2 * seq_len)
+        attn = self.layers * 3 * 2 * 2 * keys * self.features
         return dense + attn
 
 
@@ -281,7 +292,7 @@ class LMEngine:
             if self.context_attention is not None:
                 o, lse = self.context_attention.forward(qkv, B, T, H, D)
             else:
-                o, lse = K.flash_attn_qkv(qkv, B, T, H, D, self.causal)
+                o, lse = K.flash_attn_qkv(qkv, B, T, H, D, self.causal, window=s.window, sinks=s.sinks)
             x1 = K.linear_fwd_resid(o, blk["Wo"], blk["bo"], x)
             h2, r2 = K.rmsnorm(x1, blk["ln2"], s.eps)
             u, g = K.linear_fwd_gelu(h2, blk["W1"], blk["b1"])
@@ -405,7 +416,8 @@ class LMEngine:
             if self.context_attention is not None:
                 dqkv = self.context_attention.backward(qkv, o, lse, do, B, T, H, D)
             else:
-                dqkv = K.flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, self.causal)
+                dqkv = K.flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, self.causal, window=s.window,
+                                                 sinks=s.sinks)
             del do
             colsum_async(dqkv, blk["gbqkv"])
             dh1 = K.linear_dgrad(dqkv, blk["Wqkv"])

@@ -303,14 +303,24 @@ class MLP(Module):
 
 
 class SelfAttention(Module):
-    """Multi-head self-attention (heads=1 is the reference's layer, nn.py:229-249)."""
+    """Multi-head self-attention (heads=1 is the reference's layer, nn.py:229-249).
+
+    ``window`` / ``sinks`` (causal layers only): token i sees the last
+    ``window`` tokens up to itself and the first ``sinks`` tokens."""
 
     causal = False
 
-    def __init__(self, features: int, bias: bool = True, heads: int = 1) -> None:
+    def __init__(self, features: int, bias: bool = True, heads: int = 1, window: int | None = None,
+                 sinks: int = 0) -> None:
         super().__init__()
         if features % heads:
             raise ValueError("features must be divisible by heads")
+        if window is not None or sinks:
+            from underhfs_b200.ops.kernels import window_args
+
+            window_args(1, self.causal, window, sinks)  # raises for what the attention would refuse
+        self.window = window
+        self.sinks = sinks
         self.features = features
         self.heads = heads
         self.q_proj = Linear(features, features, bias=bias)
@@ -340,6 +350,9 @@ class SelfAttention(Module):
             s = (qh @ kh.transpose(-1, -2)) * scale
             if self.causal:
                 mask = torch.triu(torch.ones(T, T, dtype=torch.bool, device=t.device), 1)
+                if self.window is not None:
+                    pos = torch.arange(T, device=t.device)
+                    mask = mask | ((pos[:, None] - pos >= self.window) & (pos >= self.sinks))
                 s = s.masked_fill(mask, -1.0e9)
             o = (torch.softmax(s, -1) @ vh).transpose(1, 2).reshape(B, T, Fd)
             backend = "native_cuda" if t.is_cuda else "python"
@@ -360,9 +373,9 @@ class SelfAttention(Module):
             if self.q_proj.bias is not None:
                 b = torch.cat([self.q_proj.bias._data, self.k_proj.bias._data, self.v_proj.bias._data], 0)
             qkv = OF.linear(t.reshape(B * T, -1), w, b)
-            o = OF.flash_attention(qkv, B, T, H, D, self.causal)
+            o = OF.flash_attention(qkv, B, T, H, D, self.causal, window=self.window, sinks=self.sinks)
             return o.view(B, T, H * D), "native_cuda_attention"
-        if t.dtype == torch.float32 and H == 1 and B == 1:
+        if t.dtype == torch.float32 and H == 1 and B == 1 and self.window is None:
             q = OF.linear(t[0], self.q_proj.weight._data, _b(self.q_proj))
             k = OF.linear(t[0], self.k_proj.weight._data, _b(self.k_proj))
             v = OF.linear(t[0], self.v_proj.weight._data, _b(self.v_proj))
@@ -380,10 +393,12 @@ class CausalSelfAttention(SelfAttention):
 
 
 class TransformerBlock(Module):
-    def __init__(self, features: int, hidden_features: int, *, causal: bool = False, heads: int = 1) -> None:
+    def __init__(self, features: int, hidden_features: int, *, causal: bool = False, heads: int = 1,
+                 window: int | None = None, sinks: int = 0) -> None:
         super().__init__()
         self.attn_norm = RMSNorm(features)
-        self.attn = CausalSelfAttention(features, heads=heads) if causal else SelfAttention(features, heads=heads)
+        attention = CausalSelfAttention if causal else SelfAttention
+        self.attn = attention(features, heads=heads, window=window, sinks=sinks)
         self.mlp_norm = RMSNorm(features)
         self.mlp = MLP(features, hidden_features, features)
 
@@ -430,7 +445,8 @@ class TransformerLM(Module):
     ``forward(ids)`` returns logits ([T, V] for 1-D ids like the reference,
     [B, T, V] for 2-D); ``forward(ids, targets)`` returns the mean
     cross-entropy directly, which on the CUDA engine fuses the loss gradient
-    into the forward pass.
+    into the forward pass.  ``window`` / ``sinks`` limit every layer's attention
+    to the last ``window`` tokens and the first ``sinks`` ones.
     """
 
     def __init__(
@@ -446,6 +462,8 @@ class TransformerLM(Module):
         init: str = "reference",
         seed: int = 0,
         eps: float = 1e-8,
+        window: int | None = None,
+        sinks: int = 0,
     ) -> None:
         super().__init__()
         self.vocab_size = vocab_size
@@ -454,10 +472,13 @@ class TransformerLM(Module):
         self.hidden_features = hidden_features
         self.heads = heads
         self.tied = tied
+        self.window = window
+        self.sinks = sinks
         self.token_embedding = Embedding(vocab_size, features)
         self.position_embedding = Embedding(max_seq_len, features)
         self.blocks = ModuleList(
-            TransformerBlock(features, hidden_features, causal=True, heads=heads) for _ in range(layers)
+            TransformerBlock(features, hidden_features, causal=True, heads=heads, window=window, sinks=sinks)
+            for _ in range(layers)
         )
         self.norm = RMSNorm(features, eps=eps)
         for b in self.blocks:
@@ -477,7 +498,7 @@ class TransformerLM(Module):
         from underhfs_b200.models.transformer import LMSpec
 
         return LMSpec(self.vocab_size, self.max_seq_len, self.features, self.hidden_features, len(self.blocks),
-                      self.heads, self.tied, self.norm.eps, True)
+                      self.heads, self.tied, self.norm.eps, True, self.window, self.sinks)
 
     def _reinit(self, init: str, seed: int) -> None:
         from underhfs_b200.models.transformer import initial_value

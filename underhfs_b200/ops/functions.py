@@ -257,21 +257,33 @@ class _FlashAttention(torch.autograd.Function):
     """Causal/full multi-head attention over a fused qkv [B*T, 3*H*D] bf16 tensor."""
 
     @staticmethod
-    def forward(ctx, qkv, B, T, H, D, causal):
-        o, lse = K.flash_attn_qkv(qkv, B, T, H, D, causal)
+    def forward(ctx, qkv, B, T, H, D, causal, window, sinks):
+        o, lse = K.flash_attn_qkv(qkv, B, T, H, D, causal, window=window, sinks=sinks)
         ctx.save_for_backward(qkv, o, lse)
         ctx.dims = (B, T, H, D, causal)
+        ctx.window = (window, sinks)
         return o
 
     @staticmethod
     def backward(ctx, do):
         qkv, o, lse = ctx.saved_tensors
         B, T, H, D, causal = ctx.dims
-        return K.flash_attn_qkv_backward(qkv, o, lse, do.contiguous(), B, T, H, D, causal), None, None, None, None, None
+        window, sinks = ctx.window
+        dqkv = K.flash_attn_qkv_backward(qkv, o, lse, do.contiguous(), B, T, H, D, causal, window=window, sinks=sinks)
+        return dqkv, None, None, None, None, None, None, None
 
 
-def flash_attention(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: bool) -> torch.Tensor:
-    return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal)
+def flash_attention(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: bool, window: int | None = None,
+                    sinks: int = 0) -> torch.Tensor:
+    """Multi-head attention over a fused qkv [B*T, 3*H*D] bf16 tensor, D 64 or
+    128; returns [B*T, H*D].  ``window`` / ``sinks`` (causal only): query i sees
+    key j <= i when i - j < window or j < sinks."""
+    if window is not None or sinks:
+        if qkv.dtype != torch.bfloat16 or D not in (64, 128):
+            raise ValueError("windowed attention takes bf16 q/k/v with head_dim 64 or 128")
+        if tuple(qkv.shape) != (B * T, 3 * H * D):
+            raise ValueError(f"qkv must be [{B * T}, {3 * H * D}], got {list(qkv.shape)}")
+    return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal, window, sinks)
 
 
 class _AttentionF32(torch.autograd.Function):

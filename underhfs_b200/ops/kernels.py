@@ -300,8 +300,33 @@ def softmax_rows_backward(y: torch.Tensor, dy: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- attention
-def flash_attn_qkv(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: bool, scale: float | None = None):
-    """Attention over a fused [B*T, 3*H*D] projection; returns (o [B*T, H*D], lse [B,H,T])."""
+def window_args(T: int, causal: bool, window: int | None, sinks: int) -> tuple[int, int]:
+    """Checked (window, sinks) for the attention kernels: query i sees key
+    j <= i when i - j < window or j < sinks.  ``window=None`` (or one that
+    covers all T tokens) is plain attention, (0, 0)."""
+    sinks = int(sinks)
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a sliding window")
+        return 0, 0
+    window = int(window)
+    if window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if not causal:
+        raise ValueError("a sliding window needs causal attention")
+    return (0, 0) if window >= T else (window, min(sinks, T))
+
+
+def flash_attn_qkv(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: bool, scale: float | None = None,
+                   window: int | None = None, sinks: int = 0):
+    """Attention over a fused [B*T, 3*H*D] projection; returns (o [B*T, H*D], lse [B,H,T]).
+
+    With ``window`` (causal only) query i sees the last ``window`` keys up to
+    itself and the first ``sinks`` keys of its sequence; key blocks outside
+    are never loaded."""
+    window, sinks = window_args(T, causal, window, sinks)
     F = H * D
     scale = (1.0 / math.sqrt(D)) if scale is None else scale
     o = torch.empty((B * T, F), dtype=torch.bfloat16, device=qkv.device)
@@ -309,11 +334,12 @@ def flash_attn_qkv(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: bo
     base = qkv.data_ptr()
     st = qkv.stride(0)
     core().flash_attn_fwd(base, base + 2 * F, base + 4 * F, ptr(o), ptr(lse), T * st, st, T * st, st, T * st, st,
-                          T * F, F, B, H, T, D, float(scale), bool(causal), stream())
+                          T * F, F, B, H, T, D, float(scale), bool(causal), stream(), window, sinks)
     return o, lse
 
 
-def flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, causal, scale=None):
+def flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, causal, scale=None, window=None, sinks=0):
+    window, sinks = window_args(T, causal, window, sinks)
     F = H * D
     scale = (1.0 / math.sqrt(D)) if scale is None else scale
     dqkv = torch.empty((B * T, 3 * F), dtype=torch.bfloat16, device=qkv.device)
@@ -328,7 +354,7 @@ def flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, causal, scale=None):
         ptr(delta), ptr(dq_acc),
         T * st, st, T * st, st, T * st, st, T * F, F, T * F, F,
         T * 3 * F, 3 * F, T * 3 * F, 3 * F, T * 3 * F, 3 * F,
-        B, H, T, D, float(scale), bool(causal), stream(),
+        B, H, T, D, float(scale), bool(causal), stream(), window, sinks,
     )
     return dqkv
 

@@ -309,6 +309,8 @@ def enable_context_parallel(engine, seq_len: int, group=None) -> ContextParallel
     all-reduce, whose group then contains the context group)."""
     if not engine.causal:
         raise ValueError("context parallelism is implemented for causal attention")
+    if engine.spec.window is not None:
+        raise ValueError("context parallelism does not take sliding-window attention: its chunk pairs are whole")
     if seq_len > engine.spec.max_seq_len:
         raise ValueError(f"sequence length {seq_len} exceeds max_seq_len {engine.spec.max_seq_len}")
     cp = ContextParallelAttention(group)

@@ -48,6 +48,9 @@ class TrainConfig:
     context_parallel: bool = False
     # ZeRO-3 Adam moments: "auto" (the memory planner decides), "host", "device"
     offload: str = "auto"
+    # sliding-window attention (None: the whole context) and its sinks
+    window: int | None = None
+    sinks: int = 0
 
 
 def build_model(cfg: TrainConfig, device: str = "cuda"):
@@ -55,7 +58,8 @@ def build_model(cfg: TrainConfig, device: str = "cuda"):
 
     spec = PRESETS[cfg.model]
     model = TransformerLM(spec.vocab_size, spec.max_seq_len, spec.features, spec.hidden_features, spec.layers,
-                          heads=spec.heads, tied=spec.tied, init=cfg.init, seed=cfg.seed, eps=1e-6)
+                          heads=spec.heads, tied=spec.tied, init=cfg.init, seed=cfg.seed, eps=1e-6, window=cfg.window,
+                          sinks=cfg.sinks)
     if device.startswith("cuda"):
         model.to(device, dtype="bf16")
     return model
