@@ -435,6 +435,63 @@ PYBIND11_MODULE(_core, m) {
       py::arg("dvsb"), py::arg("dvst"), py::arg("B"), py::arg("H"), py::arg("T"), py::arg("D"),
       py::arg("scale"), py::arg("causal"), py::arg("stream"), py::arg("window") = 0, py::arg("sinks") = 0);
 
+  m.def("kv4_append", [](int dt, int D, uintptr_t k, std::array<long long, 3> ks, uintptr_t v,
+                         std::array<long long, 3> vs, uintptr_t pages, uintptr_t lengths, uintptr_t counts, int B,
+                         int T, int H, int pages_per_head, int capacity, uintptr_t s) {
+    Kv4Append p{};
+    p.k = P<const void>(k);
+    p.v = P<const void>(v);
+    p.k_stride_b = ks[0], p.k_stride_t = ks[1], p.k_stride_h = ks[2];
+    p.v_stride_b = vs[0], p.v_stride_t = vs[1], p.v_stride_h = vs[2];
+    p.pages = P<unsigned char>(pages);
+    p.lengths = P<const int>(lengths);
+    p.counts = P<const int>(counts);
+    p.B = B, p.T = T, p.H = H, p.pages_per_head = pages_per_head, p.capacity = capacity;
+    kv4_append(p, dt, D, S(s));
+  });
+  m.def("kv4_read", [](int dt, int D, uintptr_t pages, uintptr_t k, uintptr_t v, int B, int n, int H,
+                       int pages_per_head, int start, uintptr_t s) {
+    Kv4Read p{};
+    p.pages = P<const unsigned char>(pages);
+    p.k = P<void>(k);
+    p.v = P<void>(v);
+    p.B = B, p.n = n, p.H = H, p.pages_per_head = pages_per_head, p.start = start;
+    kv4_read(p, dt, D, S(s));
+  });
+  m.def("kv4_attend", [](int dt, int D, uintptr_t q, std::array<long long, 3> qs, uintptr_t pages, uintptr_t o,
+                         uintptr_t lengths, uintptr_t counts, int B, int Tq, int Hq, int Hkv, int pages_per_head,
+                         int capacity, float scale, int window, int sinks, uintptr_t s) {
+    Kv4Attend p{};
+    p.q = P<const void>(q);
+    p.q_stride_b = qs[0], p.q_stride_t = qs[1], p.q_stride_h = qs[2];
+    p.pages = P<const unsigned char>(pages);
+    p.o = P<void>(o);
+    p.lengths = P<const int>(lengths);
+    p.counts = P<const int>(counts);
+    p.B = B, p.Tq = Tq, p.Hq = Hq, p.Hkv = Hkv, p.pages_per_head = pages_per_head, p.capacity = capacity;
+    p.scale = scale, p.window = window, p.sinks = sinks;
+    kv4_attend(p, dt, D, S(s));
+  });
+
+  // temperature / top_k / top_p / min_p: one value, and a pointer that replaces it row by row unless 0
+  m.def("sample_tokens", [](int dt, uintptr_t logits, long long ld, int rows, int vocab, uintptr_t uniform,
+                            uintptr_t tokens, double temperature, uintptr_t temperature_rows, int top_k,
+                            uintptr_t top_k_rows, double top_p, uintptr_t top_p_rows, double min_p,
+                            uintptr_t min_p_rows, uintptr_t s) {
+    SampleArgs a{};
+    a.logits = P<const void>(logits);
+    a.ld = ld;
+    a.uniform = P<const float>(uniform);
+    a.tokens = P<int64_t>(tokens);
+    a.rows = rows, a.vocab = vocab;
+    a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
+    a.temperature_rows = P<const float>(temperature_rows);
+    a.top_k_rows = P<const int>(top_k_rows);
+    a.top_p_rows = P<const float>(top_p_rows);
+    a.min_p_rows = P<const float>(min_p_rows);
+    sample_tokens(a, dt, S(s));
+  });
+
   m.def("set_attn_bwd_trace", [](uintptr_t buf) { set_attn_bwd_trace(P<unsigned long long>(buf)); });
   m.def("set_attn_fwd_trace", [](uintptr_t buf) { set_attn_fwd_trace(P<unsigned long long>(buf)); });
   m.def("set_gemm_trace", [](uintptr_t buf) { set_gemm_trace(P<unsigned long long>(buf)); });

@@ -126,6 +126,57 @@ void flash_attn_bwd(const AttnBwdParams& p, cudaStream_t s);
 bool flash_attn_bwd_tc_supported(const AttnBwdParams& p);
 void flash_attn_bwd_tc_main(const AttnBwdParams& p, cudaStream_t s);
 
+// ---- key / value cache in 4 bits (kv4.cu): pages [B, Hkv, pages_per_head] of 32
+// tokens (D * 40 bytes each); `lengths` counts the tokens of each sequence
+// before the new ones, `counts` (or null: all) how many of the new ones are its own.
+struct DeviceStatus;
+struct Kv4Append {
+  const void *k, *v;  // [B, T, H, D] with element strides, D contiguous
+  long long k_stride_b, k_stride_t, k_stride_h, v_stride_b, v_stride_t, v_stride_h;
+  unsigned char* pages;
+  const int *lengths, *counts;
+  int B, T, H, pages_per_head;
+  int capacity;          // tokens; rows that would go past it are reported and left out
+  DeviceStatus* status;  // set by the launcher
+};
+struct Kv4Read {
+  const unsigned char* pages;
+  void *k, *v;  // [B, n, H, D], contiguous
+  int B, n, H, pages_per_head, start;
+};
+struct Kv4Attend {
+  const void* q;  // [B, Tq, Hq, D] with element strides, D contiguous
+  long long q_stride_b, q_stride_t, q_stride_h;
+  const unsigned char* pages;
+  void* o;  // [B, Tq, Hq, D], contiguous
+  const int *lengths, *counts;
+  int B, Tq, Hq, Hkv, pages_per_head, capacity;
+  float scale;
+  int window, sinks;     // window 0: none
+  int q_tiles, splits;   // set by the launcher
+  DeviceStatus* status;  // set by the launcher
+};
+void kv4_append(const Kv4Append& p, int dtype, int D, cudaStream_t s);
+void kv4_read(const Kv4Read& p, int dtype, int D, cudaStream_t s);
+void kv4_attend(const Kv4Attend& p, int dtype, int D, cudaStream_t s);
+
+// ---- next-token sampling (sample.cu): one token per row of logits [rows, vocab]
+struct SampleArgs {
+  const void* logits;
+  long long ld;            // elements between rows
+  const float* uniform;    // [rows], in [0, 1)
+  int64_t* tokens;         // [rows]; -1 where every logit is -inf or NaN
+  int rows, vocab;
+  // settings of all rows, or (where not null) of each
+  double temperature, top_p, min_p;
+  int top_k;
+  const float *temperature_rows, *top_p_rows, *min_p_rows;
+  const int* top_k_rows;
+  int splits, warp_len;    // set by the launcher, like vec
+  bool vec;
+};
+void sample_tokens(const SampleArgs& p, int dtype, cudaStream_t s);
+
 // ---- headless isometric voxel rasteriser (liveSee): quads [n][8] float, colors RGBA8
 void raster_iso(const float* quads, const unsigned int* colors, int nquads, unsigned int* order, unsigned int* rgba,
                 int width, int height, cudaStream_t s);

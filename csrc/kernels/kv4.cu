@@ -1,0 +1,692 @@
+// Key / value cache held in 4 bits: write, read back, and attention over it.
+//
+// Format.  The channels of one token and head are quantised in groups of 32:
+//   lo = fp16(min),  s = fp16((max - lo) * fp32(1 / 15)),  code = rhe((x - lo) / s) in 0..15
+// and a code stands for lo + s * code: 5 bits a value with its group's s and lo.
+// Values are held to the range +-61440 (so that every lo + s * code is a finite
+// fp16 number: a masked token then adds exactly 0, whatever was written), NaN
+// becomes the group's minimum.
+//
+// Layout.  A page holds 32 tokens of one head, contiguous (D * 40 bytes), so a
+// warp fetches it with one bulk copy:
+//   K codes [32 tokens][D / 2 bytes], K (s, lo) pairs [32][D / 32],
+//   V codes [32 tokens][D / 2 bytes], V s [D / 32][32], V lo [D / 32][32].
+// Word (8 codes) w of a K row holds channels 32 * (w % NG) + 8 * (w / NG) ..+7
+// (NG = D / 32): the quarter-warp lane that owns word w / NG reads its words of
+// all groups with one load.  A V row is in channel order.  The V s / lo planes
+// are permuted within 16 tokens (vslot) so that the two tokens of an MMA operand
+// register are neighbours.
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "vec.cuh"
+
+namespace uhfs {
+
+namespace {
+
+constexpr int kPage = 32;     // tokens per page
+constexpr int kGroup = 32;    // channels per (s, lo)
+constexpr float kRange = 61440.f;
+
+template <int D>
+struct Kv4 {
+  static constexpr int NG = D / kGroup;
+  static constexpr int kCodes = kPage * D / 2;    // bytes of K (or V) codes
+  static constexpr int kMeta = kPage * NG * 4;    // bytes of K (or V) s / lo
+  static constexpr int kKM = kCodes, kVC = kCodes + kMeta, kVM = 2 * kCodes + kMeta;
+  static constexpr int kBytes = 2 * (kCodes + kMeta);
+  static_assert(kBytes == D * 40 && kBytes % 16 == 0, "page size");
+};
+
+// position of a token's V s / lo within its plane: tokens t and t + 4 of 8 adjacent
+__device__ __forceinline__ int vslot(int tok) {
+  const int r = tok & 7;
+  return (tok & ~7) + (r < 4 ? 2 * r : 2 * r - 7);
+}
+
+// ------------------------------------------------------------ write / read
+// One thread per word (8 channels): 4 threads share a group, D / 8 a row.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
+  using F = Kv4<D>;
+  constexpr int LPR = D / 8;  // threads per row
+  const bool is_v = blockIdx.y != 0;
+  const T* src = static_cast<const T*>(is_v ? a.v : a.k);
+  const long long sb = is_v ? a.v_stride_b : a.k_stride_b, st = is_v ? a.v_stride_t : a.k_stride_t,
+                  sh = is_v ? a.v_stride_h : a.k_stride_h;
+  const long long rows = (long long)a.B * a.T * a.H;
+  const long long idx = blockIdx.x * 256ll + threadIdx.x;
+  const long long row = idx / LPR;
+  const int lw = (int)(idx % LPR);  // channels [8 lw, 8 lw + 8)
+  const int h = (int)(row % a.H), t = (int)(row / a.H % a.T), b = (int)(row / ((long long)a.H * a.T));
+  bool live = row < rows;
+  long long pos = 0;
+  if (live) {
+    if (a.counts != nullptr && t >= a.counts[b]) live = false;
+    pos = (long long)a.lengths[b] + t;
+    if (live && (pos < 0 || pos >= a.capacity)) {
+      if (lw == 0) report_error(a.status, kErrBounds, 60);
+      live = false;
+    }
+  }
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (live) load8<T>(src + b * sb + t * st + h * sh + lw * 8, x);
+  float mn = INFINITY, mx = -INFINITY;  // fminf / fmaxf pass over NaN
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    mn = fminf(mn, x[i]);
+    mx = fmaxf(mx, x[i]);
+  }
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  if (!live) return;
+  if (mn > mx) mn = mx = 0.f;  // nothing but NaN
+  mn = fminf(fmaxf(mn, -kRange), kRange);
+  mx = fminf(fmaxf(mx, -kRange), kRange);
+  const __half lo_h = __float2half_rn(mn);
+  const float lo = __half2float(lo_h);
+  const __half s_h = __float2half_rn(fmaxf((mx - lo) * (1.f / 15.f), 0.f));
+  const float s = __half2float(s_h), half_s = 0.5f * s;
+  const float inv = s > 0.f ? __fdividef(1.f, s) : 0.f;
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // d + e = x - lo without a rounding; k = rhe((d + e) / s): a guess by the
+    // reciprocal, put right by the remainder, which an FMA gives without a rounding
+    const float d = x[i] - lo, bb = d - x[i];
+    const float e = (x[i] - (d - bb)) + (-lo - bb);
+    int k = __float2int_rn(fminf(fmaxf(d * inv, 0.f), 15.f));
+    const float r = fmaf(-(float)k, s, d);
+    const float up = (r - half_s) + e, dn = (r + half_s) + e;
+    const int odd = k & 1;
+    if (up > 0.f || (up == 0.f && odd)) ++k;
+    if (dn < 0.f || (dn == 0.f && odd)) --k;
+    k = s > 0.f ? min(max(k, 0), 15) : 0;
+    word |= (uint32_t)k << (4 * i);
+  }
+  unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
+  const int tok = (int)(pos % kPage), gi = lw / 4;
+  if (!is_v) {
+    reinterpret_cast<uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi] = word;
+    if (lw % 4 == 0) reinterpret_cast<__half2*>(page + F::kKM)[tok * F::NG + gi] = __halves2half2(s_h, lo_h);
+  } else {
+    reinterpret_cast<uint32_t*>(page + F::kVC)[tok * LPR + lw] = word;
+    if (lw % 4 == 0) {
+      __half* m = reinterpret_cast<__half*>(page + F::kVM);
+      m[gi * kPage + vslot(tok)] = s_h;
+      m[(F::NG + gi) * kPage + vslot(tok)] = lo_h;
+    }
+  }
+}
+
+// out[b][t][h][:] = token start + t; one thread per word.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
+  using F = Kv4<D>;
+  constexpr int LPR = D / 8;
+  const bool is_v = blockIdx.y != 0;
+  const long long idx = blockIdx.x * 256ll + threadIdx.x;
+  const long long row = idx / LPR;
+  if (row >= (long long)a.B * a.n * a.H) return;
+  const int lw = (int)(idx % LPR), gi = lw / 4;
+  const int h = (int)(row % a.H), t = (int)(row / a.H % a.n), b = (int)(row / ((long long)a.H * a.n));
+  const int pos = a.start + t, tok = pos % kPage;
+  const unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
+  uint32_t w;
+  __half s, lo;
+  if (!is_v) {
+    w = reinterpret_cast<const uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi];
+    const __half2 m = reinterpret_cast<const __half2*>(page + F::kKM)[tok * F::NG + gi];
+    s = __low2half(m);
+    lo = __high2half(m);
+  } else {
+    w = reinterpret_cast<const uint32_t*>(page + F::kVC)[tok * LPR + lw];
+    const __half* m = reinterpret_cast<const __half*>(page + F::kVM);
+    s = m[gi * kPage + vslot(tok)];
+    lo = m[(F::NG + gi) * kPage + vslot(tok)];
+  }
+  const float sf = __half2float(s), lf = __half2float(lo);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = fmaf(sf, (float)((w >> (4 * i)) & 15u), lf);
+  store8<T>(static_cast<T*>(is_v ? a.v : a.k) + row * D + lw * 8, f);
+}
+
+// --------------------------------------------------------------- attention
+// The new tokens' queries of one key / value head (Tq tokens x group heads) are
+// taken eight at a time as the N = 8 side of m16n8k16 products (fp16 in, fp32
+// out); the 16 side is 16 tokens for S^T = K Q^T and 16 channels for O^T = V^T P^T,
+// so the codes, the operand that costs instructions, are read with no padding.
+//
+// The kernel is bound by HBM (0.625 bytes a value) as long as unpacking stays
+// under about 3 instructions a value:
+//   K  (w & 0x000f000f) | 0x64006400 is the fp16 pair 1024 + code, and with mask
+//      0x00f000f0 it is 1024 + 16 code: one LOP3 for two codes.  The 16 goes into
+//      q (q / 16 in those places), the 1024 into the accumulator's start value
+//      (-1024 sum q), and s and lo are applied in fp32 to the 16 x 8 product of
+//      each group: S = sum over groups of s * (q . code) + lo * sum(q).
+//   V  the tokens of a register pair have their own s and lo, so the code is
+//      freed of its 1024 (exact) and s * code + lo is one fp16 FMA (one rounding,
+//      2^-11 of the value at most; P is rounded to fp16 the same way).
+// q is scaled by softmax scale * log2(e) and, per query, by a power of two that
+// brings it to [1, 2), then rounded to fp16.
+//
+// Every warp works alone: it owns a ring of pages filled by bulk copies and takes
+// every kWarps-th page of the block's share, with its own running maximum (raised
+// only when a score exceeds it by 2^8) and sum.  The warps of a block are joined in
+// shared memory and the blocks of a cluster, which share one head's tokens, through
+// distributed shared memory: one launch, no workspace, no atomics, and a sum order
+// that depends on sizes only.
+constexpr int kWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescale = 8.0f;
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }  // 1024 + code
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return (w & 0x00f000f0u) | 0x64006400u; }  // 1024 + 16 code
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+
+__device__ __forceinline__ uint32_t dequant_lo(uint32_t w, __half2 s, __half2 lo) {
+  const __half2 c = __hsub2(as_half2(codes_lo(w)), __float2half2_rn(1024.f));
+  return as_u32(__hfma2(c, s, lo));
+}
+__device__ __forceinline__ uint32_t dequant_hi(uint32_t w, __half2 s, __half2 lo) {
+  const __half2 c = __hfma2(as_half2(codes_hi(w)), __float2half2_rn(0.0625f), __float2half2_rn(-64.f));
+  return as_u32(__hfma2(c, s, lo));
+}
+
+__device__ __forceinline__ float dsmem_load(const float* p, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(smem_cluster_addr(p, rank)) : "memory");
+  return v;
+}
+
+template <int D>
+struct Kv4Attn {
+  static constexpr int kStages = D == 128 ? 2 : 4;  // pages in flight per warp
+  static constexpr int kRing = kWarps * kStages * Kv4<D>::kBytes;
+  // after the pages: the warps' sums [kWarps][8][D], their m and l, and the block's result
+  static constexpr int kJoin = (kWarps * 8 * D + 2 * kWarps * 8 + 8 * D + 2 * 8) * 4;
+  static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kSmem = 128 + kBody + kWarps * kStages * 8;
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Attend a) {
+  using F = Kv4<D>;
+  using C = Kv4Attn<D>;
+  constexpr int NG = F::NG, NS = C::kStages, NT = D / 16;  // channel tiles of O^T
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBody);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int splits = a.splits;                  // blocks of a cluster
+  const int rank = blockIdx.x % splits;
+  long long unit = blockIdx.x / splits;         // (batch, head, query tile)
+  const int qt = (int)(unit % a.q_tiles);
+  unit /= a.q_tiles;
+  const int h = (int)(unit % a.Hkv), b = (int)(unit / a.Hkv);
+  const int G = a.Hq / a.Hkv;
+
+  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.Tq) : a.Tq;
+  const long long len = a.lengths[b];
+  const int row0 = qt * 8, rows = min(8, count * G - row0);  // live queries of this tile (may be <= 0)
+  if (threadIdx.x == 0 && rows > 0 && (len < 0 || len + count > a.capacity)) report_error(a.status, kErrBounds, 61);
+
+  // this tile's tokens: [0, hi) for its last query, from `first` on for its first, and the sinks
+  long long hi = 0, first = 0;
+  if (rows > 0) {
+    hi = min(max(len + (row0 + rows - 1) / G + 1, 0ll), (long long)a.capacity);
+    if (a.window > 0) first = max(0ll, len + row0 / G + 1 - a.window);
+  }
+  const int p_hi = (int)((hi + kPage - 1) / kPage), p_first = (int)min(first / kPage, (long long)p_hi);
+  const int p_sink = min((a.sinks + kPage - 1) / kPage, p_first);
+  const int n_pages = p_sink + p_hi - p_first;
+  const int share = (n_pages + splits - 1) / splits;
+  const int i_end = min(n_pages, (rank + 1) * share);
+  const int i_begin = rank * share + warp;  // this warp: i_begin, i_begin + kWarps, ...
+  auto page_of = [&](int i) { return i < p_sink ? i : p_first + i - p_sink; };
+
+  uint8_t* ring = smem + warp * (NS * F::kBytes);
+  uint64_t* full = bars + warp * NS;
+  const unsigned char* head = a.pages + ((long long)b * a.Hkv + h) * a.pages_per_head * F::kBytes;
+  auto issue = [&](int i, int slot) {
+    mbar_arrive_expect_tx(&full[slot], F::kBytes);
+    bulk_load(ring + slot * F::kBytes, head + (long long)page_of(i) * F::kBytes, F::kBytes, &full[slot]);
+  };
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(&full[s], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    for (int s = 0; s < NS; ++s)
+      if (i_begin + s * kWarps < i_end) issue(i_begin + s * kWarps, s);
+  }
+  __syncwarp();
+
+  // ---- queries: column g of the tile, channels 32 gi + 8 t .. + 7 of each group
+  uint32_t qf[NG][4];
+  float noffs[NG][2], qsum[NG][2], scale2[2];
+  {
+    const int m = row0 + g;
+    float q[NG][8];
+    float mx = 0.f;
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[gi][i] = 0.f;
+      if (g < rows) {
+        const T* src = static_cast<const T*>(a.q) + b * a.q_stride_b + (m / G) * a.q_stride_t +
+                       (h * G + m % G) * a.q_stride_h + gi * kGroup + t * 8;
+        load8<T>(src, q[gi]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[gi][i] *= a.scale * kLog2e;
+        mx = fmaxf(mx, fabsf(q[gi][i]));
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    // a power of two within (mx / 2, mx], of at most 2^100
+    const uint32_t eb = min(__float_as_uint(mx) & 0x7f800000u, 227u << 23);
+    const float up = mx > 1e-30f ? __uint_as_float(eb) : 1.f;
+    const float dn = mx > 1e-30f ? __uint_as_float((254u << 23) - eb) : 1.f;
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi) {
+      float off = 0.f, sum = 0.f;
+      __half hq[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool odd = i & 1;  // odd nibbles come as 16 code
+        hq[i] = __float2half_rn(q[gi][i] * (odd ? dn * 0.0625f : dn));
+        const float f = __half2float(hq[i]);
+        off += f;
+        sum += odd ? 16.f * f : f;
+      }
+      // register k of a word holds nibbles k and k + 4
+#pragma unroll
+      for (int k = 0; k < 4; ++k) qf[gi][k] = as_u32(__halves2half2(hq[k], hq[k + 4]));
+      off += __shfl_xor_sync(0xffffffffu, off, 1);
+      off += __shfl_xor_sync(0xffffffffu, off, 2);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // columns 2 t and 2 t + 1 of the products
+        noffs[gi][c] = -1024.f * __shfl_sync(0xffffffffu, off, (2 * t + c) * 4);
+        qsum[gi][c] = __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) scale2[c] = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4);
+  }
+  // tokens visible to columns 2 t, 2 t + 1: [low, lim) and [0, sinks)
+  int lim[2], low[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int col = 2 * t + c;
+    lim[c] = low[c] = 0;
+    if (col < rows) {
+      const long long end = len + (row0 + col) / G + 1;
+      lim[c] = (int)min(max(end, 0ll), (long long)a.capacity);
+      low[c] = a.window > 0 ? (int)max(0ll, min(end - a.window, (long long)a.capacity)) : 0;
+    }
+  }
+  const int lim_all = (int)max(0ll, min(len + row0 / G + 1, (long long)a.capacity));  // visible to every live query
+  const int low_all = rows > 0 && a.window > 0 ? (int)max(0ll, hi - a.window) : 0;
+
+  float o[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  const int prow = (g & 1) ? (g >> 1) + 4 : (g >> 1);  // token of product row g within 8
+
+  int n_done = 0;
+  for (int i = i_begin; i < i_end; i += kWarps, ++n_done) {
+    const int slot = n_done % NS;
+    if (!mbar_wait_warp(&full[slot], (uint32_t)(n_done / NS) & 1u, a.status, kErrWaitTimeoutFull, 62)) break;
+    const uint8_t* pg = ring + slot * F::kBytes;
+    const int key0 = page_of(i) * kPage;
+
+    // S^T: 2 x (16 tokens x 8 queries)
+    float s[2][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const int ra = mt * 16 + prow, rb = ra + 8;
+      uint32_t wa[NG], wb[NG], ma[NG], mb[NG];
+      if constexpr (NG == 4) {
+        *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(pg + ra * 64 + t * 16);
+        *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(pg + rb * 64 + t * 16);
+        *reinterpret_cast<uint4*>(ma) = *reinterpret_cast<const uint4*>(pg + F::kKM + ra * 16);
+        *reinterpret_cast<uint4*>(mb) = *reinterpret_cast<const uint4*>(pg + F::kKM + rb * 16);
+      } else {
+        *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(pg + ra * 32 + t * 8);
+        *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(pg + rb * 32 + t * 8);
+        *reinterpret_cast<uint2*>(ma) = *reinterpret_cast<const uint2*>(pg + F::kKM + ra * 8);
+        *reinterpret_cast<uint2*>(mb) = *reinterpret_cast<const uint2*>(pg + F::kKM + rb * 8);
+      }
+      s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        float c[4] = {noffs[gi][0], noffs[gi][1], noffs[gi][0], noffs[gi][1]};
+        mma_f16(c, codes_lo(wa[gi]), codes_lo(wb[gi]), codes_hi(wa[gi]), codes_hi(wb[gi]), qf[gi][0], qf[gi][1]);
+        mma_f16(c, codes_lo(wa[gi] >> 8), codes_lo(wb[gi] >> 8), codes_hi(wa[gi] >> 8), codes_hi(wb[gi] >> 8),
+                qf[gi][2], qf[gi][3]);
+        const float2 fa = __half22float2(as_half2(ma[gi])), fb = __half22float2(as_half2(mb[gi]));
+        s[mt][0] += fmaf(fa.x, c[0], fa.y * qsum[gi][0]);
+        s[mt][1] += fmaf(fa.x, c[1], fa.y * qsum[gi][1]);
+        s[mt][2] += fmaf(fb.x, c[2], fb.y * qsum[gi][0]);
+        s[mt][3] += fmaf(fb.x, c[3], fb.y * qsum[gi][1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[mt][e] *= scale2[e & 1];
+    }
+    if (key0 + kPage > lim_all || key0 < low_all) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + mt * 16 + (e >> 1) * 8 + prow;
+          if (key >= lim[e & 1] || (key < low[e & 1] && key >= a.sinks)) s[mt][e] = -INFINITY;
+        }
+    }
+    // running maximum per query: over this lane's tokens, then over the lanes of its columns
+    float mx[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      mx[c] = fmaxf(fmaxf(s[0][c], s[0][2 + c]), fmaxf(s[1][c], s[1][2 + c]));
+#pragma unroll
+      for (int w = 4; w <= 16; w <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], w));
+    }
+    if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kRescale || mx[1] > m_run[1] + kRescale)) {
+      float alpha[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float m_new = fmaxf(m_run[c], mx[c]);
+        alpha[c] = m_new == -INFINITY ? 1.f : ex2_approx(m_run[c] - m_new);
+        m_run[c] = m_new;
+        l_run[c] *= alpha[c];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][0] *= alpha[0];
+        o[n][1] *= alpha[1];
+        o[n][2] *= alpha[0];
+        o[n][3] *= alpha[1];
+      }
+    }
+    const float base[2] = {m_run[0] == -INFINITY ? 0.f : m_run[0], m_run[1] == -INFINITY ? 0.f : m_run[1]};
+    uint32_t pb[2][2];  // P as the products' second operand: [16 tokens][8 queries]
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[mt][e] = ex2_approx(s[mt][e] - base[e & 1]);
+        l_run[e & 1] += s[mt][e];
+      }
+      pb[mt][0] = transpose8x8(as_u32(__floats2half2_rn(s[mt][0], s[mt][1])));
+      pb[mt][1] = transpose8x8(as_u32(__floats2half2_rn(s[mt][2], s[mt][3])));
+    }
+    // O^T += V^T P^T: lane's tokens t, t + 4, t + 8, t + 12 of 16, channels D/8 g .. + D/8 - 1
+    constexpr int NW = D / 64;  // words per lane and token
+    const int vg = g * NW / 4;  // their group
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      uint32_t w[4][NW];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* src = pg + F::kVC + (mt * 16 + 4 * k + t) * (D / 2) + g * (4 * NW);
+        if constexpr (NW == 2) *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(src);
+        else w[k][0] = *reinterpret_cast<const uint32_t*>(src);
+      }
+      const uint8_t* meta = pg + F::kVM + (vg * kPage + mt * 16 + 2 * t) * 2;
+      const __half2 s0 = *reinterpret_cast<const __half2*>(meta), s1 = *reinterpret_cast<const __half2*>(meta + 16);
+      const __half2 l0 = *reinterpret_cast<const __half2*>(meta + NG * kPage * 2),
+                    l1 = *reinterpret_cast<const __half2*>(meta + NG * kPage * 2 + 16);
+#pragma unroll
+      for (int nw = 0; nw < NW; ++nw) {
+#pragma unroll
+        for (int q4 = 0; q4 < 2; ++q4) {  // nibbles 0..3, 4..7 of the word pair
+          const uint32_t x = __byte_perm(w[0][nw], w[1][nw], q4 ? 0x7632 : 0x5410);
+          const uint32_t y = __byte_perm(w[2][nw], w[3][nw], q4 ? 0x7632 : 0x5410);
+          float* acc = o[nw * 4 + q4 * 2];
+          mma_f16(acc, dequant_lo(x, s0, l0), dequant_hi(x, s0, l0), dequant_lo(y, s1, l1), dequant_hi(y, s1, l1),
+                  pb[mt][0], pb[mt][1]);
+          acc = o[nw * 4 + q4 * 2 + 1];
+          mma_f16(acc, dequant_lo(x >> 8, s0, l0), dequant_hi(x >> 8, s0, l0), dequant_lo(y >> 8, s1, l1),
+                  dequant_hi(y >> 8, s1, l1), pb[mt][0], pb[mt][1]);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the page
+    if (lane == 0 && i + NS * kWarps < i_end) issue(i + NS * kWarps, slot);
+  }
+  // copies still in flight (only after a wait that gave up): they land before the memory is used again
+  if (i_begin + n_done * kWarps < i_end) {
+    for (int s = 0; s < NS; ++s) {
+      const int k = n_done + s;
+      if (i_begin + k * kWarps < i_end)
+        mbar_wait_warp(&full[k % NS], (uint32_t)(k / NS) & 1u, a.status, kErrWaitTimeoutFull, 63);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int w = 4; w <= 16; w <<= 1) l_run[c] += __shfl_xor_sync(0xffffffffu, l_run[c], w);
+
+  // ---- join the block's warps
+  float* wo = reinterpret_cast<float*>(smem);   // [kWarps][8][D]
+  float* wm = wo + kWarps * 8 * D;              // [kWarps][8]
+  float* wl = wm + kWarps * 8;
+  float* bo = wl + kWarps * 8;                  // the block: [8][D], m, l
+  float* bm = bo + 8 * D;
+  float* bl = bm + 8;
+  __syncthreads();  // the pages are done with
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int col = 2 * t + c;
+    if (col >= rows) continue;
+    float* dst = wo + (warp * 8 + col) * D + g * (D / 8);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(dst + 2 * n) = make_float2(o[n][c], o[n][2 + c]);
+    if (g == 0) {
+      wm[warp * 8 + col] = m_run[c];
+      wl[warp * 8 + col] = l_run[c];
+    }
+  }
+  __syncthreads();
+  const int live = max(rows, 0) * D;
+  for (int e = threadIdx.x; e < live; e += kWarps * 32) {
+    const int col = e / D;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, wm[w * 8 + col]);
+    float l = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      // no maximum: nothing was visible (all sums are 0) or every score was NaN (so is the sum)
+      const float f = m == -INFINITY ? 1.f : ex2_approx(wm[w * 8 + col] - m);
+      l = fmaf(f, wl[w * 8 + col], l);
+      v = fmaf(f, wo[w * 8 * D + e], v);
+    }
+    bo[e] = v;
+    if (e % D == 0) {
+      bm[col] = m;
+      bl[col] = l;
+    }
+  }
+  // ---- join the cluster's blocks: each writes its share of the outputs
+  if (splits > 1) cluster_sync_all();
+  else __syncthreads();
+  T* out = static_cast<T*>(a.o);
+  for (int e = threadIdx.x + rank * (kWarps * 32); e < live; e += splits * (kWarps * 32)) {
+    const int col = e / D, mrow = row0 + col;
+    float m = -INFINITY, l = 0.f, v = 0.f;
+    if (splits == 1) {
+      l = bl[col];
+      v = bo[e];
+    } else {
+      for (int r = 0; r < splits; ++r) m = fmaxf(m, dsmem_load(bm + col, r));
+      for (int r = 0; r < splits; ++r) {
+        const float f = m == -INFINITY ? 1.f : ex2_approx(dsmem_load(bm + col, r) - m);
+        l = fmaf(f, dsmem_load(bl + col, r), l);
+        v = fmaf(f, dsmem_load(bo + e, r), v);
+      }
+    }
+    out[(((long long)b * a.Tq + mrow / G) * a.Hq + h * G + mrow % G) * D + e % D] =
+        from_float<T>(l > 0.f || l != l ? v / l : 0.f);
+  }
+  // queries past the sequence's own tokens: zeros
+  if (rank == 0) {
+    const int total = min(8, a.Tq * G - row0);
+    for (int e = live + threadIdx.x; e < total * D; e += kWarps * 32) {
+      const int mrow = row0 + e / D;
+      out[(((long long)b * a.Tq + mrow / G) * a.Hq + h * G + mrow % G) * D + e % D] = from_float<T>(0.f);
+    }
+  }
+  if (splits > 1) cluster_sync_all();  // no block leaves while another reads its sums
+}
+
+template <int D, typename T>
+void launch_attend(const Kv4Attend& a, cudaStream_t s) {
+  using C = Kv4Attn<D>;
+  static PerDeviceOnce once;
+  once([] {
+    UHFS_CUDA_CHECK(
+        cudaFuncSetAttribute(kv4_attend_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  });
+  const long long units = (long long)a.B * a.Hkv * a.q_tiles;
+  if (units * a.splits > 0x7fffffffll) throw std::runtime_error("kv4 attention: too many blocks");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(units * a.splits));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)a.splits;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.splits > 1 ? 1 : 0;
+  UHFS_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kv4_attend_kernel<D, T>, a));
+  note_launch();
+}
+
+void check_shape(int D, const void* pages, const char* what) {
+  if (D != 64 && D != 128) throw std::runtime_error(std::string(what) + ": head_dim must be 64 or 128");
+  if (reinterpret_cast<uintptr_t>(pages) % 16 != 0) throw std::runtime_error(std::string(what) + ": pages must be 16-byte aligned");
+}
+
+// rows of 8 channels are moved in 16-byte pieces
+void check_rows(const void* p, int elem, long long sb, long long st, long long sh, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % 16 != 0 || (sb * elem) % 16 != 0 || (st * elem) % 16 != 0 ||
+      (sh * elem) % 16 != 0)
+    throw std::runtime_error(std::string(what) + ": rows must be 16-byte aligned");
+}
+
+unsigned row_blocks(long long rows, int D, const char* what) {
+  const long long blocks = (rows * (D / 8) + 255) / 256;
+  if (blocks > 0x7fffffffll) throw std::runtime_error(std::string(what) + ": too many rows");
+  return (unsigned)blocks;
+}
+
+}  // namespace
+
+#define UHFS_KV4_TYPES(dtype, ...)                                  \
+  switch (dtype) {                                                  \
+    case DT_F32: { using T = float; __VA_ARGS__; break; }           \
+    case DT_F16: { using T = __half; __VA_ARGS__; break; }          \
+    case DT_BF16: { using T = __nv_bfloat16; __VA_ARGS__; break; }  \
+    default: throw std::runtime_error("unsupported dtype");         \
+  }
+
+void kv4_append(const Kv4Append& p, int dtype, int D, cudaStream_t s) {
+  if (p.B <= 0 || p.T <= 0 || p.H <= 0) return;
+  check_shape(D, p.pages, "kv4 append");
+  const int elem = dtype == DT_F32 ? 4 : 2;
+  check_rows(p.k, elem, p.k_stride_b, p.k_stride_t, p.k_stride_h, "kv4 append");
+  check_rows(p.v, elem, p.v_stride_b, p.v_stride_t, p.v_stride_h, "kv4 append");
+  Kv4Append a = p;
+  a.status = device_status_ptr();
+  const dim3 grid(row_blocks((long long)p.B * p.T * p.H, D, "kv4 append"), 2);
+  UHFS_KV4_TYPES(dtype, if (D == 64) kv4_append_kernel<64, T><<<grid, 256, 0, s>>>(a);
+                 else kv4_append_kernel<128, T><<<grid, 256, 0, s>>>(a));
+  note_launch();
+  UHFS_CUDA_CHECK(cudaGetLastError());
+}
+
+void kv4_read(const Kv4Read& a, int dtype, int D, cudaStream_t s) {
+  if (a.B <= 0 || a.n <= 0 || a.H <= 0) return;
+  check_shape(D, a.pages, "kv4 read");
+  if (a.start < 0 || (long long)a.start + a.n > (long long)a.pages_per_head * kPage)
+    throw std::runtime_error("kv4 read: tokens outside the cache");
+  check_rows(a.k, 4, 0, 0, 0, "kv4 read");
+  check_rows(a.v, 4, 0, 0, 0, "kv4 read");
+  const dim3 grid(row_blocks((long long)a.B * a.n * a.H, D, "kv4 read"), 2);
+  UHFS_KV4_TYPES(dtype, if (D == 64) kv4_read_kernel<64, T><<<grid, 256, 0, s>>>(a);
+                 else kv4_read_kernel<128, T><<<grid, 256, 0, s>>>(a));
+  note_launch();
+  UHFS_CUDA_CHECK(cudaGetLastError());
+}
+
+void kv4_attend(const Kv4Attend& p, int dtype, int D, cudaStream_t s) {
+  if (p.B <= 0 || p.Tq <= 0 || p.Hq <= 0) return;
+  check_shape(D, p.pages, "kv4 attention");
+  if (dtype != DT_BF16 && dtype != DT_F16) throw std::runtime_error("kv4 attention: q must be bf16 or fp16");
+  if (p.Hkv <= 0 || p.Hq % p.Hkv != 0) throw std::runtime_error("kv4 attention: query heads must be a multiple of key / value heads");
+  if (p.window < 0 || p.sinks < 0 || p.window > (1 << 30) || p.sinks > (1 << 30))
+    throw std::runtime_error("kv4 attention: window or sinks out of range");
+  check_rows(p.q, 2, p.q_stride_b, p.q_stride_t, p.q_stride_h, "kv4 attention");
+  Kv4Attend a = p;
+  a.status = device_status_ptr();
+  const long long rows = (long long)p.Tq * (p.Hq / p.Hkv);
+  if (rows > (1 << 28)) throw std::runtime_error("kv4 attention: too many new tokens");
+  a.q_tiles = (int)((rows + 7) / 8);
+  // Blocks per head: enough for two blocks on each SM, as far as every warp of a
+  // block still has a page; 8 is the largest portable cluster.
+  const long long units = (long long)p.B * p.Hkv * a.q_tiles;
+  int seen = p.pages_per_head;
+  if (p.window > 0) {
+    const long long w = (long long)(p.window + p.Tq) / kPage + 2 + (p.sinks + kPage - 1) / kPage;
+    if (w < seen) seen = (int)w;
+  }
+  a.splits = 1;
+  while (a.splits < 8 && units * a.splits < 2 * 148 && a.splits * 2 * kWarps <= seen + kWarps - 1) a.splits *= 2;
+  if (dtype == DT_BF16) {
+    if (D == 64) launch_attend<64, __nv_bfloat16>(a, s);
+    else launch_attend<128, __nv_bfloat16>(a, s);
+  } else {
+    if (D == 64) launch_attend<64, __half>(a, s);
+    else launch_attend<128, __half>(a, s);
+  }
+}
+
+}  // namespace uhfs

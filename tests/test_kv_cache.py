@@ -1,0 +1,400 @@
+"""The 4-bit key / value cache: write, read back, attention over it; CPU and CUDA."""
+
+import math
+
+import pytest
+import torch
+
+from underhfs.kv_cache import RANGE, QuantizedKVCache, quantize_groups
+
+H16 = torch.finfo(torch.float16).eps / 2  # one rounding to fp16, relative
+
+
+def attention(q, k, v, pos, window, sinks, scale):
+    """q [T, H, D], k / v [n, H, D] in 64 bits, pos [T]: (o, sum p |v|, sum |q||k| of the largest score)."""
+    s = torch.einsum("thd,nhd->htn", q, k) * scale
+    size = torch.einsum("thd,nhd->htn", q.abs(), k.abs()) * scale
+    j = torch.arange(k.shape[0], device=q.device)
+    ok = j[None, :] <= pos[:, None]
+    if window:
+        ok &= (pos[:, None] - j[None, :] < window) | (j[None, :] < sinks)
+    s = s.masked_fill(~ok, float("-inf"))
+    p = torch.softmax(s, -1)
+    size = size.masked_fill(~ok, 0).amax(-1)
+    return (torch.einsum("htn,nhd->thd", p, v), torch.einsum("htn,nhd->thd", p, v.abs()), size.transpose(0, 1))
+
+
+# ------------------------------------------------------------------- CPU
+def test_quantised_values_are_within_half_a_step():
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(50, 96, generator=g) * torch.logspace(-3, 3, 50).unsqueeze(1) + 5
+    y = quantize_groups(x)
+    w = x.double().unflatten(-1, (-1, 32))
+    lo, hi = w.amin(-1, keepdim=True), w.amax(-1, keepdim=True)
+    # half a step, and what the fp16 roundings of the minimum and of 15 steps can leave uncovered
+    bound = (hi - lo) / 30 * (1 + 2 * H16) + H16 * lo.abs() + H16 * (hi - lo) + 2.0**-24
+    assert ((y.unflatten(-1, (-1, 32)) - w).abs() <= bound).all()
+    assert (y.unflatten(-1, (-1, 32)) - w).abs().max() > 0
+    for i in range(3):
+        assert len(torch.unique(y[0, i * 32 : i * 32 + 32])) <= 16
+
+
+def test_quantised_special_values():
+    nan, inf = float("nan"), float("inf")
+    x = torch.zeros(6, 32)
+    x[1] = 3.0
+    x[2, :3] = torch.tensor([inf, -inf, 1e30])
+    x[3, :2] = torch.tensor([nan, 7.0])
+    x[4] = nan
+    x[5] = 1e-9
+    y = quantize_groups(x)
+    assert torch.isfinite(y).all() and y.abs().max() <= RANGE * (1 + 2 * H16)
+    assert (y[0] == 0).all() and (y[1] == 3).all() and (y[4] == 0).all()
+    assert y[2, 0] == y[2, 2] == RANGE and y[2, 1] == -RANGE
+    assert y[3, 0] == 0 and abs(y[3, 1] - 7) < 15 * 7 * H16
+
+
+def test_cpu_cache_holds_and_attends():
+    torch.manual_seed(1)
+    cache = QuantizedKVCache(2, 2, 2, 32, 12, device="cpu")
+    k, v = torch.randn(2, 5, 2, 32), torch.randn(2, 5, 2, 32)
+    cache.append(1, k, v, counts=torch.tensor([5, 3]))
+    cache.advance(torch.tensor([4, 3]))
+    kk, vv = cache.read(1, 0, 6, dtype=torch.float64)
+    assert torch.equal(kk[0, :5], quantize_groups(k[0])) and torch.equal(vv[1, :3], quantize_groups(v[1, :3]))
+    assert (kk[1, 3:] == 0).all() and (cache.read(0)[0] == 0).all()
+    cache.append(1, k[:, :2] + 1, v[:, :2] + 1)  # sequence 0 writes over its token 4
+    assert torch.equal(cache.read(1, 4, 2, dtype=torch.float64)[0][0], quantize_groups(k[0, :2] + 1))
+    q = torch.randn(2, 2, 4, 32, dtype=torch.float64)
+    for window, sinks in ((None, 0), (2, 1)):
+        o = cache.attend(1, q, window=window, sinks=sinks)
+        kk, vv = (t.repeat_interleave(2, 2) for t in cache.read(1, dtype=torch.float64))
+        for b, start in ((0, 4), (1, 3)):
+            n = start + 2
+            want, _, _ = attention(q[b], kk[b, :n], vv[b, :n], torch.arange(start, n), window, sinks, 32**-0.5)
+            assert torch.allclose(o[b], want, rtol=0, atol=1e-12)
+    assert (cache.attend(1, q, counts=torch.tensor([2, 1]))[1, 1] == 0).all()
+
+
+def test_refusals_on_the_cpu():
+    with pytest.raises(ValueError, match="head_dim"):
+        QuantizedKVCache(1, 1, 1, 40, 8, device="cpu")
+    with pytest.raises(ValueError, match="max_len"):
+        QuantizedKVCache(1, 1, 1, 32, 0, device="cpu")
+    c = QuantizedKVCache(1, 2, 2, 32, 8, device="cpu")
+    x = torch.zeros(2, 3, 2, 32)
+    with pytest.raises(IndexError):
+        c.append(1, x, x)
+    with pytest.raises(ValueError, match="k must be"):
+        c.append(0, x[:1], x[:1])
+    with pytest.raises(ValueError, match="differ"):
+        c.append(0, x, x.double())
+    with pytest.raises(ValueError, match="counts"):
+        c.append(0, x, x, counts=torch.ones(3, dtype=torch.int32))
+    with pytest.raises(TypeError, match="counts"):
+        c.append(0, x, x, counts=torch.ones(2))
+    with pytest.raises(TypeError, match="floating"):
+        c.append(0, x.long(), x.long())
+    with pytest.raises(ValueError, match="multiple"):
+        c.attend(0, torch.zeros(2, 1, 3, 32))
+    for bad in (dict(window=0), dict(sinks=2), dict(window=4, sinks=-1)):
+        with pytest.raises(ValueError):
+            c.attend(0, torch.zeros(2, 1, 2, 32), **bad)
+    c.append(0, x, x)
+    c.advance(3)
+    c.append(0, x, x)
+    c.advance(3)
+    for call in (lambda: c.append(0, x, x), lambda: c.attend(0, x), lambda: c.advance(3),
+                 lambda: c.append(0, x, x, counts=torch.tensor([1, 3]))):
+        with pytest.raises(ValueError, match="do not fit"):
+            call()
+    with pytest.raises(ValueError, match="outside"):
+        c.read(0, 7, 2)
+    c.reset()
+    c.append(0, x, x)
+
+
+# ------------------------------------------------------------------- GPU
+@pytest.fixture
+def status():
+    from underhfs_b200.ops._lib import core
+
+    yield lambda: core().device_status(True)
+    st = core().device_status(True)
+    assert st["code"] == 0, st
+
+
+def randn(*shape, seed=0, dtype=torch.bfloat16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,H,D", [(1, 1, 64), (2, 3, 128), (3, 5, 64)])
+def test_written_and_read_back(B, H, D, dtype, status):
+    """Appends of many lengths, page borders crossed; the values are the format's, bit for bit."""
+    cache = QuantizedKVCache(2, B, H, D, 150)
+    want = torch.zeros(2, B, 150, H, D, dtype=torch.float64, device="cuda")
+    at = 0
+    for n, t in enumerate((1, 30, 1, 1, 33, 64, 2)):
+        k = 3 * randn(B, t, H, D, seed=n, dtype=dtype) + 1
+        v = randn(B, t, H, D, seed=100 + n, dtype=dtype)
+        cache.append(1, k, v)
+        cache.advance(t)
+        want[0, :, at : at + t], want[1, :, at : at + t] = quantize_groups(k), quantize_groups(v)
+        at += t
+    assert cache.lengths.tolist() == [at] * B
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        for got, x in zip(cache.read(1, dtype=out), want):
+            assert torch.equal(got, x.float().to(out))
+        for got, x in zip(cache.read(1, 29, 70, dtype=out), want):
+            assert torch.equal(got, x[:, 29:99].float().to(out))
+    assert all((t == 0).all() for t in cache.read(0))
+
+
+@pytest.mark.gpu
+def test_written_from_strided_rows_and_ragged_batches(status):
+    B, T, H, D = 3, 45, 2, 64
+    qkv = randn(B * T, 3 * H * D, seed=5)
+    _, k, v = qkv.view(B, T, 3, H, D).unbind(2)  # fused projection, as the engine has it
+    kt = randn(B, H, T, D, seed=6).transpose(1, 2)  # heads first
+    odd = randn(B * T * H * D + 1, seed=7)[1:].view(B, T, H, D)  # not 16-byte aligned
+    wide = randn(B, T, H, 2 * D, seed=8)[..., ::2]  # channels apart
+    counts = torch.tensor([45, 0, 17], dtype=torch.int32, device="cuda")
+    for a, b in ((k, v), (kt, odd), (wide, k)):
+        cache = QuantizedKVCache(1, B, H, D, 64)
+        old_k, old_v = randn(B, 64, H, D, seed=9), randn(B, 64, H, D, seed=10)
+        cache.append(0, old_k, old_v)
+        cache.advance(3)
+        cache.append(0, a, b, counts=counts)
+        for got, new, old in zip(cache.read(0, dtype=torch.float32), (a, b), (old_k, old_v)):
+            want = quantize_groups(old)
+            for s, n in enumerate(counts.tolist()):
+                want[s, 3 : 3 + n] = quantize_groups(new[s, :n])
+            assert torch.equal(got, want.float())  # and what was not written is as it was
+
+
+@pytest.mark.gpu
+def test_special_values_are_stored_finite(status):
+    nan, inf = float("nan"), float("inf")
+    x = torch.zeros(1, 8, 1, 64, device="cuda")
+    x[0, 1] = 3.0
+    x[0, 2, 0, :4] = torch.tensor([inf, -inf, 1e30, nan], device="cuda")
+    x[0, 3] = nan
+    x[0, 4] = 1e-9
+    x[0, 5] = torch.linspace(-1e-6, 1e-6, 64)
+    x[0, 6] = torch.linspace(61439, 61440, 64)
+    x[0, 7] = torch.arange(64) * 0.25  # quotients on halves
+    for dtype in (torch.float32, torch.bfloat16):
+        cache = QuantizedKVCache(1, 1, 1, 64, 8)
+        cache.append(0, x.to(dtype), x.to(dtype))
+        for got in cache.read(0, dtype=torch.float32):
+            assert torch.equal(got, quantize_groups(x.to(dtype)).float())
+
+
+def fill(B, keys, Hkv, D, lens, tq, dtype, seed=0):
+    """A cache whose sequence b holds lens[b] tokens, the last tq of them not yet advanced."""
+    cache = QuantizedKVCache(1, B, Hkv, D, keys)
+    k = randn(B, keys, Hkv, D, seed=seed, dtype=dtype) + randn(1, 1, Hkv, D, seed=seed + 1, dtype=dtype)
+    v = randn(B, keys, Hkv, D, seed=seed + 2, dtype=dtype)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cache.append(0, k, v, counts=n)
+    cache.advance(n - torch.tensor(tq, dtype=torch.int32, device="cuda"))
+    return cache
+
+
+def check_attend(cache, q, got, lens, tq, window, sinks, scale=None):
+    """Against 64 bits over the cached values.
+
+    The kernel rounds q to fp16 (a score moves by H16 sum|q||k| at most, and by a
+    few 2^-23 of 1024 s sum|q| per group in its fp32 sums, s < 1 here), P and the
+    dequantised v to fp16, and the result to q's type; a P below fp16's normal range
+    is off by 2^-25 of the largest.
+    """
+    D, G = q.shape[3], q.shape[2] // cache.kv_heads
+    scale = D**-0.5 if scale is None else scale
+    half = torch.finfo(q.dtype).eps / 2
+    kk, vv = (t.double().repeat_interleave(G, 2) for t in cache.read(0, dtype=torch.float32))
+    for b, (n, t) in enumerate(zip(lens, tq)):
+        assert (got[b, t:] == 0).all()
+        if t == 0:
+            continue
+        pos = torch.arange(n - t, n, device="cuda")
+        qb = q[b, :t].double()
+        o, size, score = attention(qb, kk[b, :n], vv[b, :n], pos, window, sinks, scale)
+        move = H16 * score + 1024 * 2.0**-21 * scale * qb.abs().sum(-1)
+        err = (torch.expm1(2 * move) + 2 * H16).unsqueeze(-1) * size + half * o.abs()
+        err = err + n * 2.0**-24 * vv[b, :n].abs().max() + 1e-6
+        over = ((got[b, :t].double() - o).abs() - err).max().item()
+        assert over <= 0, (b, over)
+
+
+CASES = [  # B, tq, lens, Hq, Hkv, D, window, sinks
+    (1, [1], [1], 1, 1, 64, None, 0),
+    (2, [1, 1], [2, 31], 3, 3, 128, None, 0),
+    (4, [1, 1, 1, 1], [32, 33, 64, 65], 2, 2, 64, None, 0),
+    (1, [1], [1000], 12, 12, 64, None, 0),
+    (1, [1], [3001], 2, 1, 128, None, 0),
+    (3, [1, 0, 1], [700, 300, 1], 8, 1, 128, None, 0),
+    (2, [40, 13], [40, 13], 2, 2, 64, None, 0),
+    (2, [5, 5], [500, 77], 8, 1, 128, None, 0),
+    (2, [9, 4], [333, 96], 6, 2, 64, None, 0),
+    (2, [1, 1], [500, 20], 4, 2, 64, 33, 1),
+    (2, [1, 1], [640, 641], 4, 4, 128, 1, 0),
+    (1, [17], [900], 4, 2, 128, 100, 40),
+    (1, [60], [200], 1, 1, 64, 7, 3),
+    (2, [3, 3], [4000, 90], 5, 1, 64, 64, 200),
+    (1, [2], [2048], 24, 1, 128, 2047, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,tq,lens,Hq,Hkv,D,window,sinks", CASES)
+def test_attention(B, tq, lens, Hq, Hkv, D, window, sinks, dtype, status):
+    cache = fill(B, max(lens) + 3, Hkv, D, lens, tq, dtype)
+    q = randn(B, max(tq), Hq, D, seed=50, dtype=dtype)
+    counts = torch.tensor(tq, dtype=torch.int32, device="cuda") if len(set(tq)) > 1 else None
+    got = cache.attend(0, q, window=window, sinks=sinks, counts=counts)
+    check_attend(cache, q, got, lens, tq, window, sinks)
+
+
+@pytest.mark.gpu
+def test_attention_strides_scale_and_large_queries(status):
+    lens, tq = [300, 41], [2, 2]
+    cache = fill(2, 320, 2, 64, lens, tq, torch.bfloat16)
+    qkv = randn(2 * 2, 3 * 4 * 64, seed=51).view(2, 2, 3, 4, 64)
+    odd = randn(2 * 2 * 4 * 64 + 3, seed=52)[3:].view(2, 2, 4, 64)
+    for q in (qkv[:, :, 1], odd, randn(2, 4, 2, 64, seed=53).transpose(1, 2)):
+        check_attend(cache, q, cache.attend(0, q, scale=0.3), lens, tq, None, 0, 0.3)
+    # the power of two that brings q to fp16's range: results as for q of ordinary size
+    big = randn(2, 2, 4, 64, seed=54)
+    a = cache.attend(0, big, scale=0.125)
+    assert torch.equal(a, cache.attend(0, big * 2.0**60, scale=0.125 * 2.0**-60))
+    assert torch.equal(a, cache.attend(0, big * 2.0**-40, scale=0.125 * 2.0**40))
+    assert (cache.attend(0, torch.zeros_like(big)).isfinite()).all()
+    big[0, 0, 1, 5] = float("nan")
+    got = cache.attend(0, big, scale=0.125)
+    assert got[0, 0, 1].isnan().all()
+    got[0, 0, 1], a[0, 0, 1] = 0, 0
+    assert torch.equal(got, a)
+
+
+@pytest.mark.gpu
+def test_masked_tokens_may_hold_anything(status):
+    """NaN and infinities behind the window, behind the sequence and in another sequence change nothing."""
+    lens, tq = [200, 90], [1, 1]
+    cache = fill(2, 256, 1, 64, lens, tq, torch.float16)
+    q = randn(2, 1, 2, 64, seed=55, dtype=torch.float16)
+    want = cache.attend(0, q, window=40, sinks=3)
+    bad = torch.full((2, 120, 1, 64), float("nan"), device="cuda", dtype=torch.float16)
+    bad[:, ::2] = float("inf")
+    held = cache.lengths.clone()
+    cache.lengths.copy_(torch.tensor([10, 100], dtype=torch.int32))
+    cache.append(0, bad, -bad, counts=torch.tensor([120, 60], dtype=torch.int32, device="cuda"))
+    cache.lengths.copy_(held)
+    assert torch.equal(cache.attend(0, q, window=40, sinks=3), want)
+
+
+@pytest.mark.gpu
+def test_tokens_past_the_end_are_left_out_and_reported(status):
+    cache = QuantizedKVCache(1, 2, 1, 64, 40)
+    cache.append(0, randn(2, 40, 1, 64), randn(2, 40, 1, 64, seed=1))
+    before = cache.pages.clone()
+    cache.advance(torch.tensor([40, 39], dtype=torch.int32, device="cuda"))
+    k = randn(2, 2, 1, 64, seed=2)
+    cache.append(0, k, k)
+    st = status()
+    assert st["code"] == 5 and st["count"] >= 1  # bounds
+    got = cache.read(0, 39, 1, dtype=torch.float32)[0]
+    assert torch.equal(got[1, 0], quantize_groups(k[1, 0]).float())
+    assert torch.equal(cache.pages[:, 0], before[:, 0])
+    o = cache.attend(0, randn(2, 2, 1, 64, seed=3))
+    assert status()["code"] == 5 and o.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(status):
+    """A layer of 4.6 GB: the last head's last pages."""
+    n = 450_000
+    cache = QuantizedKVCache(1, 1, 64, 128, n)
+    assert cache.nbytes > 1 << 32
+    cache.advance(n - 70)
+    k, v = randn(1, 70, 64, 128, seed=1), randn(1, 70, 64, 128, seed=2)
+    cache.append(0, k, v)
+    for got, x in zip(cache.read(0, n - 70, 70, dtype=torch.float32), (k, v)):
+        assert torch.equal(got, quantize_groups(x).float())
+    cache.advance(69)
+    q = randn(1, 1, 64, 128, seed=3)
+    got = cache.attend(0, q, window=70)
+    kk, vv = (t.double()[0] for t in cache.read(0, n - 70, 70, dtype=torch.float32))
+    want, _, _ = attention(q[0].double(), kk, vv, torch.tensor([69], device="cuda"), None, 0, 128**-0.5)
+    assert (got[0].double() - want).abs().max() < 0.02
+
+
+@pytest.mark.gpu
+def test_captured_decoding_and_two_streams(status):
+    """A captured step (append, attend, advance) replays with the lengths it finds on the device;
+    two caches on two streams do not disturb each other."""
+    B, H, D, steps = 2, 2, 64, 70
+
+    def tokens(i):
+        return [randn(B, 1, H, D, seed=1000 + 3 * i + j) for j in range(3)]
+
+    eager = QuantizedKVCache(1, B, H, D, 96)
+    want = []
+    for i in range(steps):
+        q, k, v = tokens(i)
+        eager.append(0, k, v)
+        want.append(eager.attend(0, q, window=50, sinks=2))
+        eager.advance(1)
+
+    cache = QuantizedKVCache(1, B, H, D, 96)
+    q, k, v = tokens(0)
+
+    def step():
+        cache.append(0, k, v)
+        o = cache.attend(0, q, window=50, sinks=2)
+        cache.advance(1)
+        return o
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = step()
+    cache.reset()
+    other = QuantizedKVCache(1, B, H, D, 96)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(steps):
+        for dst, src in zip((q, k, v), tokens(i)):
+            dst.copy_(src)
+        with torch.cuda.stream(side):
+            a, b, c = tokens(i)
+            other.append(0, b, c)
+            p = other.attend(0, a, window=50, sinks=2)
+            other.advance(1)
+        graph.replay()
+        assert torch.equal(o, want[i]), i
+    side.synchronize()
+    assert torch.equal(p, want[-1])
+    assert cache.lengths.tolist() == [steps] * B
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    with pytest.raises(ValueError, match="head_dim 64 or 128"):
+        QuantizedKVCache(1, 1, 1, 96, 8)
+    c = QuantizedKVCache(1, 1, 1, 64, 8)
+    x = torch.zeros(1, 1, 1, 64, device="cuda")
+    with pytest.raises(TypeError, match="bf16 or fp16"):
+        c.attend(0, x)
+    with pytest.raises(RuntimeError, match="the cache on"):
+        c.append(0, x.cpu(), x.cpu())
+    with pytest.raises(RuntimeError, match="counts are on"):
+        c.append(0, x, x, counts=torch.ones(1, dtype=torch.int32))
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        c.append(0, x.double(), x.double())
+    with pytest.raises(TypeError, match="reads as"):
+        c.read(0, dtype=torch.float64)
+    assert c.attend(0, torch.zeros(1, 0, 1, 64, device="cuda", dtype=torch.bfloat16)).shape == (1, 0, 1, 64)

@@ -1,0 +1,241 @@
+"""Next-token sampling: CPU path, CUDA kernel and TransformerLM.generate."""
+
+import math
+
+import pytest
+import torch
+
+from underhfs import functional as F
+
+INF = math.inf
+
+
+def reference(x, u, t=1.0, k=0, p=1.0, m=0.0):
+    """One row in Python floats, token by token."""
+    order = sorted((i for i in range(len(x)) if x[i] > -INF), key=lambda i: (-x[i], i))
+    if not order:
+        return -1
+    if t <= 0:
+        return order[0]
+    w = {i: 1.0 if x[i] == x[order[0]] else math.exp((x[i] - x[order[0]]) / t) for i in order}
+    if k > 0:
+        order = order[:k]
+    if p < 1.0:
+        total, run, kept = math.fsum(w[i] for i in order), 0.0, []
+        for i in order:
+            if kept and run >= p * total:
+                break
+            kept.append(i)
+            run += w[i]
+        order = kept
+    order = sorted(i for i in order if w[i] >= min(m, 1.0))
+    goal, run, last = u * math.fsum(w[i] for i in order), 0.0, -1
+    for i in order:
+        if w[i] == 0.0:
+            continue
+        run, last = run + w[i], i
+        if run > goal:
+            return i
+    return last
+
+
+def rows(n, vocab, seed, dtype=torch.float32, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(n, vocab, generator=g)).to(dtype), torch.rand(n, generator=g)
+
+
+def check(x, u, device, t=1.0, k=0, p=1.0, m=0.0):
+    got = F.sample(x.to(device), u.to(device), temperature=t, top_k=k, top_p=p, min_p=m).torch()
+    assert got.dtype == torch.int64 and got.device.type == device
+    pick = lambda v, i: float(v[i]) if isinstance(v, torch.Tensor) else v  # noqa: E731
+    want = [reference([float(v) for v in x[i]], float(u[i]), pick(t, i), int(pick(k, i)), pick(p, i), pick(m, i))
+            for i in range(x.shape[0])]
+    assert got.tolist() == want
+
+
+SETTINGS = [dict(), dict(t=0.0), dict(t=0.7), dict(k=1), dict(k=5), dict(k=10**9), dict(p=0.9), dict(p=0.3),
+            dict(p=1e-9), dict(m=0.1), dict(m=1.0), dict(t=1.7, k=40, p=0.8, m=0.02), dict(t=1e-4), dict(t=50.0, p=0.99)]
+
+
+def special_rows():
+    """Rows where a sampler can go wrong: ties, nothing visible, infinities, the type's lowest value."""
+    low = torch.finfo(torch.float32).min
+    return torch.tensor([
+        [0.0] * 9,
+        [-INF] * 9,
+        [-INF, -INF, 3.0, -INF, -INF, -INF, -INF, -INF, -INF],
+        [low] * 9,
+        [low, 1.0, low, 1.0, low, 0.5, low, 0.5, low],
+        [1.0, INF, 1.0, INF, 0.0, 0.0, 0.0, 0.0, 0.0],
+        [-0.0, 0.0, -0.0, 0.0, -1.0, -1.0, -1.0, -1.0, -1.0],
+        [-1000.0, -1001.0, -1000.0, -1002.0, -1e30, -1000.5, -3e38, -1000.0, -1001.0],
+        [80.0, -80.0, 79.0, 79.0, 79.0, -INF, 78.0, 79.0, 10.0],
+    ])
+
+
+def run_special(device, **kw):
+    x = special_rows()
+    for u in (0.0, 0.2, 0.5, 0.75, 0.9999999):
+        check(x, torch.full((x.shape[0],), u), device, **kw)
+
+
+# ------------------------------------------------------------------- CPU
+@pytest.mark.parametrize("kw", SETTINGS)
+def test_cpu(kw):
+    x, u = rows(12, 57, 1)
+    check(x, u, "cpu", **kw)
+    check((x * 2).round() / 2, u, "cpu", **kw)  # many ties
+    run_special("cpu", **kw)
+
+
+def test_cpu_per_row_and_shapes():
+    x, u = rows(6, 31, 2)
+    kw = dict(t=torch.tensor([0.0, 0.5, 1.0, 1.0, 2.0, 0.9]), k=torch.tensor([0, 3, 0, 7, -1, 50], dtype=torch.int32),
+              p=torch.tensor([1.0, 0.9, 0.5, 1.0, 0.2, 2.0]), m=torch.tensor([0.0, 0.0, 0.2, 0.0, 0.5, 0.01]))
+    check(x, u, "cpu", **kw)
+    got = F.sample(x.view(2, 3, 31), u.view(2, 3), top_k=4).torch()
+    assert torch.equal(got.reshape(-1), F.sample(x, u, top_k=4).torch())
+    assert F.sample(x[0], u[0]).torch().shape == ()
+
+
+def test_nan_is_never_chosen():
+    x = torch.tensor([[float("nan"), 1.0, float("nan"), 2.0], [float("nan")] * 4])
+    for u in (0.0, 0.5, 0.999):
+        got = F.sample(x, torch.full((2,), u), temperature=5.0).torch()
+        assert got[0].item() in (1, 3) and got[1].item() == -1
+
+
+def test_distribution_follows_the_softmax():
+    x = torch.tensor([[0.0, 1.0, -1.0, 2.0]])
+    n = 4000
+    u = (torch.arange(n) + 0.5) / n  # evenly spread: each count is within one of n * probability
+    got = F.sample(x.expand(n, 4), u).torch().bincount(minlength=4)
+    assert (got - n * torch.softmax(x[0].double(), 0)).abs().max() <= 1
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(top_k=-1), "top_k"), (dict(top_p=1.5), "top_p"), (dict(top_p=-0.1), "top_p"),
+    (dict(min_p=float("nan")), "min_p"), (dict(min_p=1.1), "min_p"),
+    (dict(temperature=torch.ones(3)), "temperature needs one value"),
+])
+def test_refuses_settings(kw, match):
+    with pytest.raises(ValueError, match=match):
+        F.sample(torch.zeros(2, 5), torch.zeros(2), **kw)
+
+
+def test_refuses_shapes_and_types():
+    with pytest.raises(ValueError, match="uniform"):
+        F.sample(torch.zeros(2, 5), torch.zeros(3))
+    with pytest.raises(ValueError, match="vocab"):
+        F.sample(torch.zeros(2, 0), torch.zeros(2))
+    with pytest.raises(TypeError, match="floating"):
+        F.sample(torch.zeros(2, 5, dtype=torch.int64), torch.zeros(2))
+
+
+# ------------------------------------------------------------------- GPU
+@pytest.fixture
+def status_ok():
+    yield
+    from underhfs_b200.ops._lib import core
+
+    st = core().device_status(True)
+    assert st["code"] == 0, st
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", SETTINGS)
+def test_gpu_special_rows(kw, status_ok):
+    run_special("cuda", **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,vocab", [(1, 1), (3, 2), (5, 63), (2, 1001), (1, 5000), (300, 129), (2, 33001)])
+def test_gpu_sizes(n, vocab, dtype, status_ok):
+    x, u = rows(n, vocab, n + vocab, dtype)
+    for kw in (dict(), dict(t=0.8, p=0.9), dict(k=50, p=0.95, m=0.01), dict(t=0.0), dict(k=max(1, vocab // 2))):
+        check(x, u, "cuda", **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [4096, 40000])
+@pytest.mark.parametrize("kw", [dict(k=1500), dict(k=3000, p=0.7), dict(p=0.9), dict(p=0.999, m=0.5), dict(t=0.3, p=0.2)])
+def test_gpu_long_runs_of_equal_logits(vocab, kw, status_ok):
+    """More tokens at the border than the kernel compares at once: the key's bits decide, then the index."""
+    g = torch.Generator().manual_seed(5)
+    x = torch.randint(-1, 2, (2, vocab), generator=g).float()
+    x = torch.cat((x, torch.full((1, vocab), 2.5), torch.arange(vocab).float().unsqueeze(0) * 1e-6 + 7.0))
+    for u in (0.0, 0.31, 0.999):
+        check(x, torch.full((4,), u), "cuda", **kw)
+    check(x.bfloat16(), torch.full((4,), 0.6), "cuda", **kw)
+
+
+@pytest.mark.gpu
+def test_gpu_per_row_settings_strides_and_alignment(status_ok):
+    big, u = rows(8, 4100, 9)
+    kw = dict(t=torch.tensor([0.0, 0.5, 1.0, 1.0, 2.0, 0.9, 1.1, 0.7]),
+              k=torch.tensor([0, 3, 0, 700, -1, 5000, 1, 9], dtype=torch.int32),
+              p=torch.tensor([1.0, 0.9, 0.5, 1.0, 0.2, 2.0, 0.9, 0.0]),
+              m=torch.tensor([0.0, 0.0, 0.2, 0.0, 0.5, 0.01, 0.3, 0.0]))
+    dev = {n: v.cuda() for n, v in kw.items()}
+    x = big.cuda()
+    for view in (x, x[:, 1:], x[:, 3:2050], x.t().contiguous().t()):
+        cpu = view.cpu()
+        got = F.sample(view, u.cuda(), temperature=dev["t"], top_k=dev["k"], top_p=dev["p"], min_p=dev["m"]).torch()
+        want = [reference(cpu[i].tolist(), float(u[i]), float(kw["t"][i]), int(kw["k"][i]), float(kw["p"][i]),
+                          float(kw["m"][i])) for i in range(8)]
+        assert got.tolist() == want
+
+
+@pytest.mark.gpu
+def test_gpu_nan_and_odd_uniforms(status_ok):
+    x = torch.tensor([[float("nan"), 1.0, float("nan"), 2.0], [float("nan")] * 4, [0.0, 1.0, 2.0, -INF],
+                      [0.0, 1.0, 2.0, -INF], [0.0, 1.0, 2.0, -INF]], device="cuda")
+    u = torch.tensor([0.0, 0.5, 1.0, -3.0, float("nan")], device="cuda")
+    assert F.sample(x, u).torch().tolist() == [1, -1, 2, 0, 0]
+
+
+@pytest.mark.gpu
+def test_gpu_same_choice_however_the_row_is_split(status_ok):
+    """One row takes a cluster of blocks, 400 equal rows one block each."""
+    x, _ = rows(1, 30000, 11)
+    u = torch.rand(400, generator=torch.Generator().manual_seed(3))
+    many = F.sample(x.cuda().expand(400, -1).contiguous(), u.cuda(), temperature=1.3, top_p=0.97).torch()
+    one = [F.sample(x.cuda(), u[i : i + 1].cuda(), temperature=1.3, top_p=0.97).torch().item() for i in range(0, 400, 7)]
+    assert many.cpu()[::7].tolist() == one
+
+
+@pytest.mark.gpu
+def test_gpu_captured_and_replayed_and_other_stream(status_ok):
+    x, u = rows(4, 9000, 21)
+    xd, ud = x.cuda(), u.cuda()
+    F.sample(xd, ud, top_p=0.9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F.sample(xd, ud, top_p=0.9).torch()
+    for seed in (22, 23):
+        y, w = rows(4, 9000, seed)
+        xd.copy_(y)
+        ud.copy_(w)
+        graph.replay()
+        want = [reference(y[i].tolist(), float(w[i]), p=0.9) for i in range(4)]
+        assert out.tolist() == want
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = F.sample(xd, ud, top_p=0.9).torch()
+    side.synchronize()
+    assert got.tolist() == want
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    with pytest.raises(ValueError, match="vocabularies up to"):
+        F.sample(torch.zeros(1, 400000, device="cuda"), torch.zeros(1, device="cuda"))
+    with pytest.raises(RuntimeError, match="uniform is on"):
+        F.sample(torch.zeros(1, 40, device="cuda"), torch.zeros(1))
+    with pytest.raises(RuntimeError, match="top_p is on"):
+        F.sample(torch.zeros(1, 40, device="cuda"), torch.zeros(1, device="cuda"), top_p=torch.ones(1))
+    assert F.sample(torch.zeros(0, 40, device="cuda"), torch.zeros(0, device="cuda")).torch().shape == (0,)

@@ -17,7 +17,7 @@ from underhfs_b200 import __all__, __version__  # noqa: F401
 _SUBMODULES = (
     "tensor", "autograd", "functional", "nn", "optim", "data", "datasets", "text", "testing", "cuda", "runtime",
     "compile", "config", "serialization", "serve", "cli", "benchmarks", "diagnostics", "native", "distributed",
-    "train",
+    "train", "kv_cache",
 )
 
 _this = sys.modules[__name__]

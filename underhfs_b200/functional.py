@@ -7,6 +7,7 @@ matching the reference's Python-float semantics.
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -82,3 +83,99 @@ def gelu(input: Tensor) -> Tensor:
 
 def softmax(input: Tensor) -> Tensor:
     return input.softmax()
+
+
+def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dtype, low: float, high: float):
+    """A sampling setting: a checked number, or a tensor with one value per row."""
+    if isinstance(value, Tensor):
+        value = value._data
+    if isinstance(value, torch.Tensor):
+        if value.numel() != rows:
+            raise ValueError(f"{name} needs one value for each of {rows} rows, got {list(value.shape)}")
+        if value.device != device:
+            raise RuntimeError(f"{name} is on {value.device}, the logits on {device}")
+        return value.detach().reshape(-1).to(dtype).contiguous()
+    if not low <= value <= high:  # False for NaN
+        raise ValueError(f"{name} must lie in [{low:g}, {high:g}], got {value}")
+    return int(value) if dtype == torch.int32 else float(value)
+
+
+def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tensor:
+    """The next token of each row of logits [..., vocab], chosen by ``uniform``
+    [...] (numbers in [0, 1)); int64 [...].
+
+    In this order: ``top_k`` > 0 keeps the k largest logits; ``top_p`` < 1 keeps,
+    of those, the fewest largest whose probabilities reach top_p; ``min_p`` keeps
+    tokens of at least min_p times the largest probability.  Equal logits are
+    taken by lowest index.  Probabilities are softmax(logits / temperature); the
+    token is the first, by index, at which the running sum of the kept ones
+    passes uniform times their sum.  ``temperature`` 0 takes the largest logit
+    (lowest index).  Each setting is a number or a tensor with one value per
+    row (a temperature <= 0, a top_k <= 0 and a top_p >= 1 there are "off"; at
+    least the largest logit is always kept).
+
+    Logits of -inf and NaN are never chosen; a row without any other gives -1.
+    On CUDA (fp32, fp16, bf16, vocabularies up to 393216) this is one kernel
+    whose result does not depend on how the row is split; on the CPU it runs in
+    float64.  No gradient flows through the choice.
+    """
+    x = (logits._data if isinstance(logits, Tensor) else logits).detach()
+    u = (uniform._data if isinstance(uniform, Tensor) else uniform).detach()
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"sample expects logits [..., vocab], got {list(x.shape)}")
+    if not x.is_floating_point():
+        raise TypeError(f"logits must be floating-point, got {x.dtype}")
+    if u.shape != x.shape[:-1]:
+        raise ValueError(f"uniform must have shape {list(x.shape[:-1])}, got {list(u.shape)}")
+    if u.device != x.device:
+        raise RuntimeError(f"uniform is on {u.device}, the logits on {x.device}")
+    shape, vocab = x.shape[:-1], x.shape[-1]
+    x = x.reshape(-1, vocab)
+    rows = x.shape[0]
+    real = torch.float32 if x.is_cuda else torch.float64
+    u = u.reshape(-1).to(real).contiguous()
+    temperature = _setting(temperature, "temperature", rows, x.device, real, 0.0, 1e30)
+    top_k = _setting(top_k, "top_k", rows, x.device, torch.int32, 0, 2**31 - 1)
+    top_p = _setting(top_p, "top_p", rows, x.device, real, 0.0, 1.0)
+    min_p = _setting(min_p, "min_p", rows, x.device, real, 0.0, 1.0)
+    if x.is_cuda:
+        from underhfs_b200.ops import kernels as K
+
+        if vocab > 393216:
+            raise ValueError(f"the CUDA kernel takes vocabularies up to 393216, got {vocab}")
+        guard = contextlib.nullcontext()
+        if x.device.index != torch.cuda.current_device():
+            guard = torch.cuda.device(x.device)
+        with guard:
+            token = K.sample_tokens(x, u, temperature, top_k, top_p, min_p)
+    else:
+        token = _sample_cpu(x.double(), u, temperature, top_k, top_p, min_p)
+    return Tensor._wrap(token.reshape(shape))
+
+
+def _sample_cpu(x: torch.Tensor, u: torch.Tensor, temperature, top_k, top_p, min_p) -> torch.Tensor:
+    rows, vocab = x.shape
+
+    def column(v):
+        v = v.double() if isinstance(v, torch.Tensor) else torch.full((rows,), float(v), dtype=torch.float64)
+        return v.reshape(-1, 1)
+
+    temperature, top_k, top_p, min_p = (column(v) for v in (temperature, top_k, top_p, min_p))
+    x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
+    val, idx = torch.sort(x, dim=1, descending=True, stable=True)
+    top = val[:, :1]
+    t = torch.where(temperature > 0, temperature, torch.ones_like(temperature)).clamp(1e-30, 1e30)
+    # the largest logit's own weight is 1, infinite or not
+    w = torch.where(val == top, torch.ones_like(val), torch.exp((val - top) / t)) * (val > -math.inf)
+    rank = torch.arange(vocab).unsqueeze(0)
+    w = w * ((top_k <= 0) | (rank < top_k))
+    before = torch.cumsum(w, 1) - w
+    keep = ~(top_p < 1.0) | (before < top_p * w.sum(1, keepdim=True)) | (rank == 0)
+    w = w * keep * ((w >= min_p) | (val == top))
+    run = torch.cumsum(torch.zeros_like(w).scatter_(1, idx, w), 1)
+    total = run[:, -1:]
+    goal = torch.nan_to_num(u.reshape(-1, 1), nan=0.0).clamp(0.0, 1.0) * total
+    last = (run < total).sum(1)  # the last kept token, where a goal of the whole sum ends
+    token = torch.minimum((run <= goal).sum(1), last)
+    token = torch.where(temperature[:, 0] > 0, token, idx[:, 0])
+    return torch.where(top[:, 0] > -math.inf, token, torch.full_like(token, -1))

@@ -359,6 +359,68 @@ def flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, causal, scale=None, win
     return dqkv
 
 
+# ----------------------------------------------------------------- sampling
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_k, top_p, min_p) -> torch.Tensor:
+    """int64 [rows]: the token of each row of logits [rows, vocab] that uniform
+    [rows] (fp32) chooses after temperature, top-k, top-p and min-p, each a
+    number or a tensor [rows] (fp32; int32 for top_k).  One launch; -1 where
+    nothing can be chosen."""
+    rows, vocab = logits.shape
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    tokens = torch.empty((rows,), dtype=torch.int64, device=logits.device)
+
+    def setting(x, off):
+        return (off, ptr(x)) if isinstance(x, torch.Tensor) else (x, 0)
+
+    t, k, p, m = setting(temperature, 1.0), setting(top_k, 0), setting(top_p, 1.0), setting(min_p, 0.0)
+    core().sample_tokens(dt(logits), ptr(logits), logits.stride(0), rows, vocab, ptr(uniform), ptr(tokens),
+                         float(t[0]), t[1], int(k[0]), k[1], float(p[0]), p[1], float(m[0]), m[1], stream())
+    return tokens
+
+
+# ------------------------------------------------- 4-bit key / value cache
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """`t` [B, T, H, D] itself where the cache kernels can read its rows in
+    16-byte pieces (D contiguous, strides and start aligned), else a copy."""
+    per = 16 // t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in t.stride()[:3]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def kv4_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor,
+               counts: torch.Tensor | None, capacity: int) -> None:
+    """Quantise k / v [B, T, H, D] into `pages` [B, H, P, 40 D] behind each
+    sequence's `lengths` tokens (one launch); only the first counts[b] tokens
+    of sequence b are written."""
+    B, T, H, D = k.shape
+    k, v = _rows16(k), _rows16(v)
+    core().kv4_append(dt(k), D, ptr(k), list(k.stride()[:3]), ptr(v), list(v.stride()[:3]), ptr(pages), ptr(lengths),
+                      ptr(counts), B, T, H, pages.shape[2], capacity, stream())
+
+
+def kv4_read(pages: torch.Tensor, start: int, n: int, D: int, dtype: torch.dtype):
+    """(k, v) [B, n, H, D] in `dtype`: what tokens start..start+n-1 of `pages` stand for (one launch)."""
+    B, H, P, _ = pages.shape
+    k = torch.empty((B, n, H, D), dtype=dtype, device=pages.device)
+    v = torch.empty_like(k)
+    core().kv4_read(dt(k), D, ptr(pages), ptr(k), ptr(v), B, n, H, P, start, stream())
+    return k, v
+
+
+def kv4_attend(pages: torch.Tensor, q: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None,
+               capacity: int, scale: float, window: int, sinks: int) -> torch.Tensor:
+    """Attention of the new tokens' q [B, Tq, Hq, D] (bf16 or fp16) over `pages`
+    (one launch): token t of sequence b sees the cache up to lengths[b] + t."""
+    B, Tq, Hq, D = q.shape
+    q = _rows16(q)
+    o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
+    core().kv4_attend(dt(q), D, ptr(q), list(q.stride()[:3]), ptr(pages), ptr(o), ptr(lengths), ptr(counts), B, Tq,
+                      Hq, pages.shape[1], pages.shape[2], capacity, float(scale), window, sinks, stream())
+    return o
+
+
 def attention_f32(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, causal: bool) -> torch.Tensor:
     """Reference-contract single-head fp32 attention, q/k/v [T, F]."""
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
