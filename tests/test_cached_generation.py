@@ -1,0 +1,221 @@
+"""TransformerLM.decode / generate over the 4-bit cache with sampling: the operators as they are used together."""
+
+import json
+
+import pytest
+import torch
+
+from underhfs import functional as F
+from underhfs.cli import main
+from underhfs.nn import TransformerLM
+from underhfs.tensor import tensor
+
+KW = dict(vocab_size=64, max_seq_len=48, features=64, hidden_features=96, layers=2, heads=2, init="normal", seed=3)
+
+
+def lm(**kw):
+    return TransformerLM(**{**KW, **kw})
+
+
+# ------------------------------------------------------------------- CPU
+@pytest.mark.parametrize("window,sinks", [(None, 0), (6, 2)])
+def test_cpu_prompt_is_exact_and_steps_follow_closely(window, sinks):
+    m = lm(window=window, sinks=sinks)
+    ids = torch.randint(0, 64, (2, 12), generator=torch.Generator().manual_seed(0))
+    cache = m.new_cache(batch=2, max_len=20)
+    with torch.no_grad():
+        full = m(ids)._data
+    got = m.decode(ids[:, :9], cache)._data
+    assert torch.allclose(got, full[:, 8], rtol=0, atol=1e-12)
+    for t in range(9, 12):  # over the quantised cache: near, not equal
+        got = m.decode(ids[:, t : t + 1], cache)._data
+        assert 0 < (got - full[:, t]).norm() < 0.05 * full[:, t].norm()
+    assert cache.lengths.tolist() == [12, 12] and not cache.is_empty
+
+
+def test_cpu_ragged_prompts_match_single_ones():
+    m = lm()
+    ids = torch.randint(0, 64, (2, 10), generator=torch.Generator().manual_seed(1))
+    counts = torch.tensor([10, 4])
+    cache = m.new_cache(batch=2)
+    got = [m.decode(ids, cache, counts)._data, m.decode(ids[:, :2], cache)._data]
+    assert cache.lengths.tolist() == [12, 6]
+    for b, n in enumerate(counts.tolist()):
+        one = m.new_cache()
+        want = [m.decode(ids[b : b + 1, :n], one)._data, m.decode(ids[b : b + 1, :2], one)._data]
+        for g, w in zip(got, want):
+            assert torch.allclose(g[b], w[0], rtol=0, atol=1e-12)
+
+
+def test_generate_samples_and_defaults_to_greedy():
+    m = lm()
+    prompt = tensor([1, 2, 3])
+    greedy = m.generate(prompt, 6)._storage
+    assert greedy == m.generate(prompt, 6, temperature=0.0)._storage
+    assert greedy == m.generate(prompt, 6, temperature=2.0, top_k=1, seed=0)._storage
+    a, b = (m.generate(prompt, 30, temperature=2.0, seed=5)._storage for _ in range(2))
+    assert a == b and a != m.generate(prompt, 30, temperature=2.0, seed=6)._storage
+    u = torch.rand(4, generator=torch.Generator().manual_seed(2))
+    ids = [1, 2, 3]
+    for i in range(4):
+        with torch.no_grad():
+            logits = m(torch.tensor(ids))._data[-1]
+        ids.append(int(F.sample(logits, u[i].double(), temperature=1.5, top_p=0.9).torch()))
+    assert m.generate(prompt, 4, temperature=1.5, top_p=0.9, uniform=u)._storage == ids
+
+
+def test_generate_over_the_cache_on_the_cpu():
+    m = lm()
+    prompt = tensor([5, 6, 7, 8])
+    out = m.generate(prompt, 8, cache="int4")._storage
+    assert len(out) == 12 and out[:5] == m.generate(prompt, 1)._storage  # the first token comes from exact keys
+    cache = m.new_cache(max_len=40)
+    for _ in range(2):  # a cache is reset and used again
+        assert m.generate(prompt, 8, cache=cache)._storage == out
+    assert m.generate(prompt, 0, cache="int4")._storage == [5, 6, 7, 8]
+
+
+def test_refusals():
+    m = lm()
+    with pytest.raises(ValueError, match="do not fit"):
+        m.generate(tensor([1] * 40), 9, cache="int4")
+    with pytest.raises(ValueError, match="unknown cache"):
+        m.generate(tensor([1]), 2, cache="int8")
+    with pytest.raises(ValueError, match="prompt"):
+        m.generate(torch.zeros(0, dtype=torch.int64), 2, cache="int4")
+    with pytest.raises(ValueError, match="uniform needs"):
+        m.generate(tensor([1]), 3, temperature=1.0, uniform=torch.rand(2))
+    with pytest.raises(ValueError, match="temperature"):
+        m.generate(tensor([1]), 3, temperature=float("inf"))
+    with pytest.raises(ValueError, match="another model"):
+        m.decode(torch.zeros(1, 1, dtype=torch.int64), lm(layers=1).new_cache())
+    with pytest.raises(ValueError, match="token ids"):
+        m.decode(torch.zeros(2, 1, dtype=torch.int64), m.new_cache())
+    with pytest.raises(ValueError, match="positions"):
+        m.decode(torch.zeros(1, 1, dtype=torch.int64), lm(max_seq_len=99).new_cache())
+    with pytest.raises(ValueError, match="head_dim"):
+        lm(heads=8).new_cache()  # 8 channels a head: less than one group
+
+
+def test_cli_generates_with_a_cache_and_sampling(capsys):
+    args = ["generate", "--prompt", "hi", "--max-new-tokens", "5", "--features", "32", "--seq-len", "16",
+            "--cache", "int4", "--temperature", "0.9", "--top-k", "20", "--top-p", "0.95", "--min-p", "0.01", "--seed", "4",
+            "--window", "4", "--sinks", "1"]
+    outs = []
+    for _ in range(2):
+        assert main(args) == 0
+        outs.append(json.loads(capsys.readouterr().out)["tokens"])
+    assert outs[0] == outs[1] and len(outs[0]) == 7
+
+
+# ------------------------------------------------------------------- GPU
+@pytest.fixture
+def status_ok():
+    yield
+    from underhfs_b200.ops._lib import core
+
+    st = core().device_status(True)
+    assert st["code"] == 0, st
+
+
+def gpu_pair(**kw):
+    big = dict(vocab_size=512, max_seq_len=320, features=256, hidden_features=512, layers=3, heads=4, init="normal", seed=2)
+    cpu, gpu = TransformerLM(**{**big, **kw}), TransformerLM(**{**big, **kw}).to("cuda", dtype="bf16")
+    for (_, a), (_, b) in zip(cpu.named_parameters(), gpu.named_parameters()):
+        with torch.no_grad():
+            a._data.copy_(8 * b._data.double().cpu())  # larger weights: logits that differ
+            b._data.copy_(a._data)
+    return cpu, gpu
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [2, 4])  # head_dim 128, 64
+@pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3)])
+def test_engine_decodes_over_the_cache(heads, window, sinks, status_ok):
+    """Ragged prompts, a chunk and single tokens: the prompt's logits are the plain forward's,
+    and in every layer the step's keys, values and attention are what the formulas give for
+    that layer's own input.  (Logits of different roundings are not compared: with these
+    weights the plain bf16 forward alone is a quarter of their size from 64 bits.)"""
+    from tests.test_kv_cache import check_attend
+    from underhfs_b200.kv_cache import QuantizedKVCache, quantize_groups
+
+    seen = []
+
+    class Watched(QuantizedKVCache):
+        def append(self, layer, k, v, counts=None):
+            super().append(layer, k, v, counts=counts)
+            at, n = self.lengths.tolist(), [k.shape[1]] * self.batch if counts is None else counts.tolist()
+            for x, got in zip((k, v), self.read(layer, dtype=torch.float32)):
+                for b in range(self.batch):
+                    assert torch.equal(got[b, at[b] : at[b] + n[b]], quantize_groups(x[b, : n[b]]).float())
+
+        def attend(self, layer, q, **kw):
+            o = super().attend(layer, q, **kw)
+            one = QuantizedKVCache(1, self.batch, self.kv_heads, self.head_dim, self.max_len)
+            one.pages = self.pages[layer : layer + 1]
+            new = [q.shape[1]] * self.batch
+            check_attend(one, q, o, [a + n for a, n in zip(self.lengths.tolist(), new)], new, window, sinks)
+            seen.append(layer)
+            return o
+
+    _, gpu = gpu_pair(heads=heads, window=window, sinks=sinks)
+    ids = torch.randint(0, 512, (2, 200), generator=torch.Generator().manual_seed(4)).cuda()
+    counts = torch.tensor([150, 97], dtype=torch.int32, device="cuda")
+    cache = Watched(3, 2, heads, 256 // heads, 300)
+    got = gpu.decode(ids[:, :150], cache, counts)._data
+    with torch.no_grad():
+        full = gpu(ids[:, :150])._data
+    assert torch.equal(got, torch.stack((full[0, 149], full[1, 96])))
+    for x in (ids[:, 150:163], ids[:, 163:164], ids[:, 164:165]):
+        assert gpu.decode(x, cache)._data.isfinite().all()
+    assert seen == [0, 1, 2] * 3
+    assert cache.lengths.tolist() == [165, 112]
+
+
+@pytest.mark.gpu
+def test_engine_steps_stay_near_the_whole_context(status_ok):
+    """Weights of ordinary size: tokens run one by one over the cache against the whole context at once.
+
+    The cache moves a value by at most 1/30 of its group's range (about 0.13 of a
+    standard deviation; a third of that in the mean), a bf16 forward adds a few 2^-8:
+    logits off by well under a tenth, those of another context by about their size.
+    """
+    kw = dict(vocab_size=512, max_seq_len=320, features=256, hidden_features=512, layers=3, heads=4, init="normal", seed=2)
+    gpu = TransformerLM(**kw).to("cuda", dtype="bf16")
+    ids = torch.randint(0, 512, (1, 100), generator=torch.Generator().manual_seed(4)).cuda()
+    cache = gpu.new_cache()
+    gpu.decode(ids[:, :60], cache)
+    with torch.no_grad():
+        full = gpu(ids)._data[0].double()
+    for t in range(60, 100):
+        got = gpu.decode(ids[:, t : t + 1], cache)._data[0].double()
+        assert (got - full[t]).norm() < 0.1 * full[t].norm()
+        assert (got - full[t - 1]).norm() > 0.5 * full[t].norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.9, top_k=40, top_p=0.95, min_p=0.01)])
+def test_generate_graph_equals_eager_steps(kw, status_ok):
+    _, m = gpu_pair(window=64, sinks=4)
+    prompt = list(range(3, 70))
+    n = 60
+    u = torch.rand(n, generator=torch.Generator().manual_seed(8))
+    got = m.generate(tensor(prompt), n, cache="int4", uniform=u, **kw)._storage
+    cache = m.new_cache()
+    ids, out = torch.tensor([prompt], device="cuda"), []
+    settings = {"temperature": 0.0, **kw}
+    for i in range(n):
+        tok = F.sample(m.decode(ids, cache)._data, u[i : i + 1].cuda(), **settings).torch()
+        ids = tok.view(1, 1)
+        out.append(int(tok))
+    assert got == prompt + out
+    # a second run on the same cache, and the uncached path still runs
+    assert m.generate(tensor(prompt), n, cache=cache, uniform=u, **kw)._storage == got
+    assert m.generate(tensor(prompt), 3, uniform=u[:3], **kw)._storage[: len(prompt) + 1] == got[: len(prompt) + 1]
+
+
+@pytest.mark.gpu
+def test_cache_needs_the_engine_on_cuda():
+    m = lm(features=64, heads=1).to("cuda")
+    with pytest.raises(ValueError, match="bf16 engine"):
+        m.new_cache()

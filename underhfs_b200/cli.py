@@ -133,7 +133,8 @@ def _cmd_train(args) -> int:
 
     cfg = TrainConfig(model=args.model, batch=args.batch, seq_len=args.seq_len_train, lr=args.lr_train,
                       zero_stage=args.zero, cuda_graph=not args.no_graph, offload=args.offload,
-                      context_parallel=getattr(args, "context_parallel", False))
+                      context_parallel=getattr(args, "context_parallel", False), window=args.window,
+                      sinks=args.sinks)
     from underhfs_b200.distributed import policy_from_env
     from underhfs_b200.train import StepMeter
 
@@ -243,12 +244,14 @@ def _cmd_generate(args) -> int:
 
     tok = ByteTokenizer()
     model = TransformerLM(vocab_size=256, max_seq_len=args.seq_len, features=args.features,
-                          hidden_features=args.hidden_features, layers=args.layers)
+                          hidden_features=args.hidden_features, layers=args.layers, heads=args.heads,
+                          window=args.window, sinks=args.sinks)
     if args.checkpoint:
         model.load_state_dict(load_binary_state_tensors(args.checkpoint))
     if args.device.startswith("cuda"):
-        model.to(args.device)
-    out = model.generate(tok.encode(args.prompt), args.max_new_tokens)
+        model.to(args.device, dtype=args.dtype)
+    out = model.generate(tok.encode(args.prompt), args.max_new_tokens, temperature=args.temperature,
+                         top_k=args.top_k, top_p=args.top_p, min_p=args.min_p, seed=args.seed, cache=args.cache)
     print(json.dumps({"prompt": args.prompt, "response": tok.decode(out), "tokens": [int(v) for v in out._storage]},
                      indent=2))
     return 0
@@ -315,6 +318,8 @@ def main(argv: list[str] | None = None) -> int:
                    help="bf16 dense peak per GPU for the MFU column (default: B200 nominal 2250)")
     p.add_argument("--context-parallel", action="store_true",
                    help="shard every sequence over all ranks (zigzag) instead of giving each rank its own batch")
+    p.add_argument("--window", type=int, help="sliding-window attention (default: the whole context)")
+    p.add_argument("--sinks", type=int, default=0, help="first tokens that stay visible with --window")
     p.set_defaults(func=_cmd_train)
 
     p = sub.add_parser("checkpoint")
@@ -346,6 +351,16 @@ def main(argv: list[str] | None = None) -> int:
     p.add_argument("--features", type=int, default=4)
     p.add_argument("--hidden-features", type=int, default=8)
     p.add_argument("--layers", type=int, default=1)
+    p.add_argument("--heads", type=int, default=1)
+    p.add_argument("--window", type=int, help="attention window of the model (default: the whole context)")
+    p.add_argument("--sinks", type=int, default=0, help="first tokens that stay visible with --window")
+    p.add_argument("--dtype", choices=("fp32", "bf16"), help="parameter type on a CUDA device")
+    p.add_argument("--temperature", type=float, default=0.0, help="0 (default): greedy")
+    p.add_argument("--top-k", type=int, default=0)
+    p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=0.0)
+    p.add_argument("--seed", type=int, help="seed of the sampling's random numbers")
+    p.add_argument("--cache", choices=("int4",), help="keep keys and values in a 4-bit cache")
     p.set_defaults(func=_cmd_generate)
 
     p = sub.add_parser("export")

@@ -226,7 +226,80 @@ def _torch_mm_case(m: int, n: int, k: int):
     return case
 
 
+def _kept_keys(T: int, window: int, sinks: int) -> int:
+    """(query, key) pairs that a causal window with sinks leaves visible."""
+    return sum(min(i + 1, window + min(sinks, max(0, i + 1 - window))) for i in range(T))
+
+
+def _window_case(B: int, T: int, H: int, D: int, window: int, sinks: int, backward: bool):
+    def case():
+        qkv, do = _bf(B * T, 3 * H * D), _bf(B * T, H * D)
+        pairs = B * H * D * _kept_keys(T, window, sinks)
+        if not backward:
+            return lambda: K.flash_attn_qkv(qkv, B, T, H, D, True, window=window, sinks=sinks), 4.0 * pairs, 0
+        o, lse = K.flash_attn_qkv(qkv, B, T, H, D, True, window=window, sinks=sinks)
+        return (lambda: K.flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, True, window=window, sinks=sinks),
+                10.0 * pairs, 0)
+    return case
+
+
+def _kv4_cache(B: int, H: int, D: int, n: int, tokens: int):
+    """A 4-bit cache of n tokens a sequence, the last `tokens` of them new."""
+    from underhfs_b200.kv_cache import QuantizedKVCache
+
+    cache = QuantizedKVCache(1, B, H, D, n)
+    cache.append(0, _bf(B, n, H, D), _bf(B, n, H, D))
+    cache.advance(n - tokens)
+    return cache
+
+
+def _kv4_attend_case(B: int, n: int, Hq: int, H: int, D: int, tokens: int):
+    def case():
+        cache, q = _kv4_cache(B, H, D, n, tokens), _bf(B, tokens, Hq, D)
+        return lambda: cache.attend(0, q), 0, cache.nbytes + 4 * q.numel()
+    return case
+
+
+def _kv4_append_case(B: int, n: int, H: int, D: int):
+    def case():
+        cache = _kv4_cache(B, H, D, n, n)
+        k, v = _bf(B, n, H, D), _bf(B, n, H, D)
+        return lambda: cache.append(0, k, v), 0, cache.nbytes + 4 * k.numel()
+    return case
+
+
+def _kv4_read_case(B: int, n: int, H: int, D: int):
+    def case():
+        cache = _kv4_cache(B, H, D, n, n)
+        return lambda: cache.read(0), 0, cache.nbytes + 4 * B * n * H * D
+    return case
+
+
+def _sample_case(rows: int, vocab: int, dtype: torch.dtype, **settings):
+    def case():
+        from underhfs_b200 import functional as F
+
+        x, u = (3 * torch.randn(rows, vocab, device="cuda")).to(dtype), torch.rand(rows, device="cuda")
+        return lambda: F.sample(x, u, **settings), 0, x.numel() * x.element_size()
+    return case
+
+
 CASES: dict[str, Callable] = {
+    # sliding window and sinks; 4-bit cache; sampling
+    "window_fwd": _window_case(2, 4096, 16, 128, 1024, 4, False),
+    "window_bwd": _window_case(2, 4096, 16, 128, 1024, 4, True),
+    "window_fwd16": _window_case(16, 1024, 12, 64, 256, 4, False),
+    "window_bwd16": _window_case(16, 1024, 12, 64, 256, 4, True),
+    "kv4_attend": _kv4_attend_case(16, 4096, 32, 32, 128, 1),
+    "kv4_attend64": _kv4_attend_case(32, 4096, 32, 32, 64, 1),
+    "kv4_attend_one": _kv4_attend_case(1, 1000, 12, 12, 64, 1),
+    "kv4_attend_draft": _kv4_attend_case(4, 16384, 32, 8, 128, 5),
+    "kv4_append": _kv4_append_case(8, 2048, 16, 128),
+    "kv4_read": _kv4_read_case(8, 2048, 16, 128),
+    "sample_one": _sample_case(1, 32000, torch.bfloat16, temperature=0.8, top_p=0.95),
+    "sample_256": _sample_case(256, 32000, torch.bfloat16, top_k=50, top_p=0.9),
+    "sample_all": _sample_case(256, 32000, torch.bfloat16),
+    "sample_wide": _sample_case(64, 131072, torch.float32, top_p=0.98),
     "torch_mm_fwd_qkv": _torch_mm_case(TOKENS, 2304, 768),
     "torch_mm_fc1": _torch_mm_case(TOKENS, 3072, 768),
     "torch_mm_8192": _torch_mm_case(8192, 8192, 8192),

@@ -88,6 +88,11 @@ class QuantizedKVCache:
             return self.pages.numel()
         return self._k.element_size() * 2 * self._k.numel()
 
+    @property
+    def is_empty(self) -> bool:
+        """No token has been counted since the start or the last ``reset``."""
+        return self._host_length == 0
+
     # ------------------------------------------------------------- checks
     def _on_device(self):
         """Launch on the cache's device, whichever is current."""
@@ -234,6 +239,11 @@ class QuantizedKVCache:
         with self._on_device():
             self.lengths += counts
         self._host_length = None
+
+    def set_host_length(self, tokens: int | None) -> None:
+        """Tell the host side how many tokens every sequence holds (None: not known)
+        after a captured graph has advanced the lengths on the device."""
+        self._host_length = tokens
 
     def reset(self) -> None:
         """Forget every token (the memory is kept and written over)."""

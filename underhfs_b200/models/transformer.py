@@ -320,6 +320,43 @@ class LMEngine:
         }
         return loss, (None if dlogits_ready else logits)
 
+    # ------------------------------------------------------------- decode
+    def decode(self, ids: torch.Tensor, cache, counts: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits [B, V] after the last of each sequence's new tokens ids [B, T]
+        (of which sequence b brings counts[b]); `cache` (QuantizedKVCache)
+        receives their keys and values and counts them.
+
+        Into an empty cache the tokens attend to one another's own keys and
+        values (flash attention); later ones attend over the cache."""
+        if self.context_attention is not None:
+            raise RuntimeError("context parallelism does not decode over a cache")
+        s = self.spec
+        B, T = ids.shape
+        H, D = s.heads, s.head_dim
+        fresh = cache.is_empty
+        pos = cache.lengths if T == 1 else cache.lengths[:, None] + torch.arange(T, device=ids.device)
+        pos = pos.reshape(-1).clamp(max=s.max_seq_len - 1)  # padding may run past the last position
+        x = K.embedding(ids.reshape(-1).contiguous(), self.E, self.P.index_select(0, pos), B * T)
+        for i, blk in enumerate(self.blocks):
+            h, _ = K.rmsnorm(x, blk["ln1"], s.eps)
+            qkv = K.linear_fwd(h, blk["Wqkv"], blk["bqkv"])
+            q, k, v = qkv.view(B, T, 3, H, D).unbind(2)
+            cache.append(i, k, v, counts=counts)
+            if fresh:
+                o, _ = K.flash_attn_qkv(qkv, B, T, H, D, self.causal, window=s.window, sinks=s.sinks)
+            else:
+                o = cache.attend(i, q, window=s.window, sinks=s.sinks, counts=counts).view(B * T, H * D)
+            x = K.linear_fwd_resid(o, blk["Wo"], blk["bo"], x)
+            h, _ = K.rmsnorm(x, blk["ln2"], s.eps)
+            _, g = K.linear_fwd_gelu(h, blk["W1"], blk["b1"])
+            x = K.linear_fwd_resid(g, blk["W2"], blk["b2"], x)
+        if T > 1:
+            first = torch.arange(B, device=ids.device) * T
+            x = x.index_select(0, first + T - 1 if counts is None else first + (counts - 1).clamp(min=0))
+        cache.advance(T if counts is None else counts)
+        h, _ = K.rmsnorm(x, self.lnf, s.eps)
+        return K.linear_fwd(h, self.Wh, None)
+
     # ----------------------------------------------------------- backward
     def backward(self, dlogits: torch.Tensor | None = None, loss_grad: torch.Tensor | None = None) -> None:
         """Accumulate every parameter gradient into the flat fp32 buffer.

@@ -17,6 +17,7 @@ training on B200:
 
 from __future__ import annotations
 
+import contextlib
 import math
 from collections import OrderedDict
 from dataclasses import dataclass
@@ -362,6 +363,21 @@ class SelfAttention(Module):
         out = _wrap(y, x, "attention", (x,), backend=backend)
         return out
 
+    def decode(self, x: Tensor, cache, layer: int, counts: torch.Tensor | None = None) -> Tensor:
+        """forward for new tokens x [batch, tokens, features] of sequences whose
+        earlier keys and values are in ``cache`` (QuantizedKVCache); theirs are added."""
+        t = x._data
+        B, T, Fd = t.shape
+        fresh = cache.is_empty
+        q, k, v = (_linear_t(t, m.weight._data, _b(m)).view(B, T, self.heads, Fd // self.heads)
+                   for m in (self.q_proj, self.k_proj, self.v_proj))
+        cache.append(layer, k, v, counts=counts)
+        if fresh:
+            return self.forward(x)
+        o = cache.attend(layer, q, window=self.window, sinks=self.sinks, counts=counts)
+        y = _linear_t(o.reshape(B, T, Fd), self.out_proj.weight._data, _b(self.out_proj))
+        return _wrap(y, x, "attention", (x,))
+
     def _try_native(self, t: torch.Tensor, B: int, T: int, H: int, D: int, scale: float):
         if not t.is_cuda:
             return None
@@ -682,20 +698,139 @@ class TransformerLM(Module):
             logits = logits[0]
         return Tensor._wrap(logits, like=like, backend="native_cuda", op="transformer_lm", parents=(like,))
 
-    def generate(self, token_ids: Tensor, max_new_tokens: int) -> Tensor:
-        """Greedy decoding; the context is the last max_seq_len tokens."""
+    # ------------------------------------------------------ generation
+    def new_cache(self, batch: int = 1, max_len: int | None = None):
+        """An empty 4-bit key / value cache for this model (QuantizedKVCache) on its device."""
+        from underhfs_b200.kv_cache import QuantizedKVCache
+
+        w = self.token_embedding.weight._data
+        if self._zero3 is not None:
+            raise RuntimeError("a ZeRO-3 sharded model does not decode over a cache")
+        if w.is_cuda and self._engine is None:
+            raise ValueError("on CUDA the cache serves the bf16 engine: call .to('cuda', dtype='bf16') first")
+        return QuantizedKVCache(len(self.blocks), batch, self.heads, self.features // self.heads,
+                                self.max_seq_len if max_len is None else max_len, device=w.device)
+
+    def decode(self, token_ids: Tensor | torch.Tensor, cache, counts: torch.Tensor | None = None) -> Tensor:
+        """Logits [B, V] after the last new token of each of B sequences.
+
+        ``token_ids`` [B, T] follow the tokens that ``cache`` (from ``new_cache``)
+        holds, and are added to it; sequence b brings only its first counts[b]
+        tokens (int tensor on the model's device; at least 1).  No gradients."""
+        ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
+        if ids.dim() != 2 or ids.shape[0] != cache.batch or ids.shape[1] < 1:
+            raise ValueError(f"decode expects token ids [{cache.batch}, tokens], got {list(ids.shape)}")
+        if (cache.layers, cache.kv_heads, cache.head_dim) != (len(self.blocks), self.heads, self.features // self.heads):
+            raise ValueError("the cache was made for another model")
+        if cache.max_len > self.max_seq_len:
+            raise ValueError(f"the cache holds {cache.max_len} tokens, the model has {self.max_seq_len} positions")
+        if self._zero3 is not None:
+            raise RuntimeError("a ZeRO-3 sharded model does not decode over a cache")
+        like = self.token_embedding.weight
+        ids = ids.to(cache.device, torch.int64)
+        with torch.no_grad():
+            if self._engine is not None:
+                logits = self._engine.decode(ids, cache, counts)
+                return Tensor._wrap(logits, like=like, backend="native_cuda", op="transformer_lm", parents=(like,))
+            B, T = ids.shape
+            pos = (cache.lengths[:, None].long() + torch.arange(T)).clamp(max=self.max_seq_len - 1)
+            x = self.token_embedding(Tensor._wrap(ids)) + self.position_embedding(Tensor._wrap(pos))
+            for i, block in enumerate(self.blocks):
+                x = x + block.attn.decode(block.attn_norm(x), cache, i, counts)
+                x = x + block.mlp(block.mlp_norm(x))
+            last = torch.full((B,), T - 1) if counts is None else (counts.long() - 1).clamp(min=0)
+            cache.advance(T if counts is None else counts)
+            h = self.norm(Tensor._wrap(x._data[torch.arange(B), last], like=x))
+            head_w = like if self.tied else self.head.weight
+            return _wrap(_linear_t(h._data, head_w._data, None), h, "linear", (h, head_w))
+
+    def generate(self, token_ids: Tensor, max_new_tokens: int, *, temperature: float = 0.0, top_k: int = 0,
+                 top_p: float = 1.0, min_p: float = 0.0, uniform: torch.Tensor | None = None,
+                 seed: int | None = None, cache=None) -> Tensor:
+        """``max_new_tokens`` tokens after the 1-D ``token_ids``.
+
+        Greedy by default; with a ``temperature`` each token is drawn by
+        functional.sample with ``top_k`` / ``top_p`` / ``min_p`` from ``uniform``
+        [max_new_tokens] or, without it, from numbers seeded with ``seed``.
+
+        Without a ``cache`` every token runs the last max_seq_len tokens again.
+        ``cache="int4"`` (or a batch-1 cache of ``new_cache``, which is reset) keeps
+        their keys and values in 4 bits and runs new tokens only; prompt and new
+        tokens then have to fit the cache.  On CUDA the steps of such a run are
+        one captured graph."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
         if ids.dim() != 1:
             raise ValueError("TransformerLM.generate expects 1D token ids")
         generated = [int(v) for v in ids.tolist()]
+        if uniform is not None:
+            uniform = (uniform._data if isinstance(uniform, Tensor) else uniform).reshape(-1)
+            if uniform.numel() != max_new_tokens:
+                raise ValueError(f"uniform needs {max_new_tokens} numbers, got {uniform.numel()}")
+        elif temperature > 0:
+            gen = torch.Generator()
+            if seed is not None:
+                gen.manual_seed(seed)
+            else:
+                gen.seed()
+            uniform = torch.rand(max(0, max_new_tokens), generator=gen)
+        else:
+            uniform = torch.zeros(max(0, max_new_tokens))
+        dev = (self._engine_device() if self._engine is not None else self.token_embedding.weight._data.device)
+        uniform = uniform.to(dev)
+        kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        if cache is not None:
+            return tensor(generated + self._generate_cached(generated, max_new_tokens, uniform, kw, cache))
         with torch.no_grad():
-            for _ in range(max_new_tokens):
+            for i in range(max_new_tokens):
                 context = generated[-self.max_seq_len:]
-                dev = (self._engine_device() if self._engine is not None
-                       else self.token_embedding.weight._data.device)
                 logits = self(torch.tensor(context, dtype=torch.int64, device=dev))
-                generated.append(int(torch.argmax(logits._data[-1].float()).item()))
+                if temperature > 0:
+                    generated.append(int(F.sample(logits._data[-1], uniform[i], **kw).torch().item()))
+                else:
+                    generated.append(int(torch.argmax(logits._data[-1].float()).item()))
         return tensor(generated)
+
+    def _generate_cached(self, prompt: list[int], n: int, uniform: torch.Tensor, kw: dict, cache) -> list[int]:
+        if not prompt:
+            raise ValueError("generation over a cache needs a prompt")
+        if isinstance(cache, str):
+            if cache != "int4":
+                raise ValueError(f"unknown cache {cache!r} (int4)")
+            cache = self.new_cache(max_len=min(self.max_seq_len, max(len(prompt) + n, 1)))
+        else:
+            cache.reset()
+        if len(prompt) + n > cache.max_len:
+            raise ValueError(f"{len(prompt)} + {n} tokens do not fit the cache of {cache.max_len}")
+        if n < 1:
+            return []
+        dev = cache.device
+        out = torch.empty((n,), dtype=torch.int64, device=dev)
+        # static storage of the captured step: the last token and its uniform number
+        token = torch.empty((1, 1), dtype=torch.int64, device=dev)
+        u = torch.empty((1,), dtype=uniform.dtype, device=dev)
+
+        def choose(logits: Tensor) -> None:
+            token.copy_(F.sample(logits._data, u, **kw).torch().view(1, 1))
+
+        guard = torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext()
+        with torch.no_grad(), guard:
+            u.copy_(uniform[:1])
+            choose(self.decode(torch.tensor([prompt], dtype=torch.int64, device=dev), cache))
+            out[:1].copy_(token[0])
+            graph = None
+            for i in range(1, n):
+                u.copy_(uniform[i : i + 1])
+                if graph is not None:
+                    graph.replay()
+                else:
+                    choose(self.decode(token, cache))
+                    if dev.type == "cuda" and n - i > 4:  # the capture costs a few eager steps
+                        graph = torch.cuda.CUDAGraph()
+                        with torch.cuda.graph(graph):
+                            choose(self.decode(token, cache))
+                out[i : i + 1].copy_(token[0])
+            cache.set_host_length(len(prompt) + n - 1)  # replays advanced the device's lengths only
+            return [int(v) for v in out.tolist()]
 
 
 def _require_cuda(device: Device) -> None:
