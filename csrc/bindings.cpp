@@ -435,8 +435,8 @@ PYBIND11_MODULE(_core, m) {
       py::arg("dvsb"), py::arg("dvst"), py::arg("B"), py::arg("H"), py::arg("T"), py::arg("D"),
       py::arg("scale"), py::arg("causal"), py::arg("stream"), py::arg("window") = 0, py::arg("sinks") = 0);
 
-  m.def("kv4_append", [](int dt, int D, uintptr_t k, std::array<long long, 3> ks, uintptr_t v,
-                         std::array<long long, 3> vs, uintptr_t pages, uintptr_t lengths, uintptr_t counts, int B,
+  m.def("kv4_append", [](int dt, int D, uintptr_t k, const std::array<long long, 4>& ks, uintptr_t v,
+                         const std::array<long long, 4>& vs, uintptr_t pages, uintptr_t lengths, uintptr_t counts, int B,
                          int T, int H, int pages_per_head, int capacity, uintptr_t s) {
     Kv4Append p{};
     p.k = P<const void>(k);
@@ -458,7 +458,7 @@ PYBIND11_MODULE(_core, m) {
     p.B = B, p.n = n, p.H = H, p.pages_per_head = pages_per_head, p.start = start;
     kv4_read(p, dt, D, S(s));
   });
-  m.def("kv4_attend", [](int dt, int D, uintptr_t q, std::array<long long, 3> qs, uintptr_t pages, uintptr_t o,
+  m.def("kv4_attend", [](int dt, int D, uintptr_t q, const std::array<long long, 4>& qs, uintptr_t pages, uintptr_t o,
                          uintptr_t lengths, uintptr_t counts, int B, int Tq, int Hq, int Hkv, int pages_per_head,
                          int capacity, float scale, int window, int sinks, uintptr_t s) {
     Kv4Attend p{};

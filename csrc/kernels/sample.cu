@@ -6,9 +6,12 @@
 // as follows, and the choice walks the vocabulary in index order:
 //   1. the row goes to shared memory (one block, or a cluster whose blocks each hold
 //      a slice); maximum and minimum;
-//   2. top-k: a histogram of 1024 equal steps of the logit finds the step that holds
-//      the k-th token, whose few tokens are then compared with one another;
-//   3. top-p: the same with the sum of weights in place of the count;
+//   2. top-k of at most kShortK: the k-th largest of the threads' own maxima bounds
+//      the k-th logit from below, so one pass gathers little more than k tokens and
+//      the rest, top-p and the choice included, is done on that list;
+//   3. otherwise, for top-k: a histogram of 1024 equal steps of the logit finds the
+//      step that holds the k-th token, whose tokens are then compared with one
+//      another; for top-p: the same with the sum of weights in place of the count;
 //   4. sums of the kept weights per warp (a contiguous part of the row each); the warp
 //      that holds u * total walks its part again.
 // A step that holds more tokens than the list (equal logits in long runs) is cut by
@@ -16,12 +19,16 @@
 //
 // Weights 2^((l - max) log2(e) / T) are 64-bit integers in units of 2^-44: sums do
 // not depend on the order of atomics, blocks or warps, and a token on the border of
-// top-p or of u is decided alike however the row was split.  Within 2^16 of the
-// largest a weight is computed in 64 bits (relative error below 2^-36, from the
-// Taylor series of exp), below that in 32 bits, where its error is below 2^-35 of
-// the largest weight.
+// top-p or of u is decided alike however the row was split.  A weight is right to
+// 2^-29 of itself (fp32 pairs for the exponent, a table of 64 powers, a short series;
+// tests/test_sampling.py restates the steps), so that a sum over n tokens of like
+// weight is right to about 2^-29 / sqrt(n) and the choice is that of exact arithmetic
+// but for u in a few parts in 10^8.  In 64-bit floating point the same choice took
+// 1.5 to 2 times the kernel's time.  A histogram holds its sums as three 32-bit words
+// of 15 bits of the weights each (shared memory adds 32-bit words at full rate).
 //
-// Bound by latency for a few rows, by HBM for many (one read of the logits).
+// Bound by latency for a few rows (a cluster joins its blocks four or five times), by
+// the passes over shared memory for many.
 #include <stdexcept>
 #include <string>
 
@@ -37,26 +44,31 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;   // two per thread
 constexpr int kCap = 1024;    // tokens compared with one another at the border
-static_assert(kCap <= kBins, "the border tokens' weights reuse the histogram");
-constexpr float kFine = -16.f;  // log2 of the weight from which 64 bits are used
+constexpr int kShortK = 256;  // top-k up to which one gathered list does
 typedef unsigned long long u64;
+
+constexpr int kMaxSplits = 8;
+constexpr int kPowers = 64;   // entries of the table of 2^(i / 64)
 
 // shared memory in front of the row's slice
 struct alignas(16) Shared {
-  u64 hist[kBins];      // later the weights of the border tokens
-  u64 list[kCap];       // this block's border tokens
-  u64 all[kCap];        // the cluster's
+  uint32_t part[3][kBins];  // the block's histogram: bits 0..14, 15..29, 30..44 of the weights
+  u64 hist[kBins];          // the same as sums; later the weights of the listed tokens
+  u64 list[kCap];           // this block's listed tokens (order keys)
+  u64 all[kCap];            // the cluster's
   u64 warp_sum[kWarps];
-  u64 border;           // order key of the last kept token
-  u64 excl;             // sum before the chosen bin
+  u64 sums[kMaxSplits * kWarps];  // warp_sum of every block
+  uint32_t powers[kPowers];
+  u64 border;               // order key of the last kept token
+  u64 excl;                 // sum before the chosen bin
   int bin;
-  int count;            // entries of list (may exceed kCap: then not all are stored)
-  float mx, mn;         // this block's extremes, then the row's
-  int first;            // lowest index of the maximum in this block
+  int count;                // entries of list (may exceed kCap: then not all are stored)
+  float mx, mn;             // this block's extremes
+  int first;                // lowest index of the maximum in this block
   float warp_mx[kWarps], warp_mn[kWarps];
   int warp_first[kWarps];
-  int token;
 };
+static_assert(kCap <= kBins, "the listed tokens' weights reuse the histogram");
 
 // The order: larger keys first.  Equal logits (-0 and 0 too) share the upper half.
 __device__ __forceinline__ u64 order_key(float l, int idx) {
@@ -70,49 +82,66 @@ __device__ __forceinline__ float key_logit(u64 key) {
   return __uint_as_float(k);
 }
 
+// 2^(i / 64) in units of 2^-31, from the series of exp
+struct Powers {
+  uint32_t v[kPowers];
+};
+constexpr Powers make_powers() {
+  Powers p{};
+  for (int i = 0; i < kPowers; ++i) {
+    const double y = 0.69314718055994530942 * i / kPowers;
+    double e = 1.0, term = 1.0;
+    for (int k = 1; k < 24; ++k) {
+      term *= y / k;
+      e += term;
+    }
+    p.v[i] = (uint32_t)(e * 2147483648.0 + 0.5);
+  }
+  return p;
+}
+__constant__ Powers kPowerTable = make_powers();
+
 struct Row {
-  float mx;       // largest logit
-  double mxd, c;  // the same; log2(e) / temperature
-  float cf;
+  float mx;        // largest logit
+  float ch, cl;    // log2(e) / temperature as a sum of two fp32 numbers
 };
 
-// log2 of the weight in 32 bits: 0 for the maximum itself (also where it is infinite)
-__device__ __forceinline__ float log2_weight(const Row& r, float l) {
-  return l == r.mx ? 0.f : (l - r.mx) * r.cf;
+// 2^44 * 2^((l - max) c): 2^(k / 64) from the table and 2^r - 1 from its series, |r| <= 1/128
+__device__ __forceinline__ u64 weight(const Row& row, const uint32_t* powers, float l) {
+  // x = p + q = (l - max) * c to about 2^-46 of itself
+  const float d = l == row.mx ? 0.f : l - row.mx, bb = d - l;
+  const float e = (l - (d - bb)) + (-row.mx - bb);
+  const float p = d * row.ch;
+  const float q = fmaf(d, row.cl, fmaf(l == row.mx ? 0.f : e, row.ch, fmaf(d, row.ch, -p)));
+  if (!(p > -46.f)) return 0;
+  const float kf = rintf(p * (float)kPowers);
+  const float t = (fmaf(kf, -1.f / kPowers, p) + q) * 0.69314718f;
+  const float em1 = fmaf(fmaf(fmaf(t, 1.f / 24, 1.f / 6), t, 0.5f), t * t, t);
+  const int k = (int)kf;
+  const uint32_t m = powers[k & (kPowers - 1)];
+  const u64 w = (u64)m + (u64)(int64_t)__float2int_rn((float)m * em1);
+  return (w << 13) >> (-(k >> 6));
 }
 
-// round(2^44 * 2^((l - max) c))
-__device__ __forceinline__ u64 weight(const Row& r, float l) {
-  const float xf = log2_weight(r, l);
-  if (xf < kFine) return __float2ull_rn(ex2_approx(xf) * 17592186044416.f);
-  const double x = l == r.mx ? 0.0 : ((double)l - r.mxd) * r.c;
-  const float nf = rintf(xf);
-  const double y = (x - (double)nf) * 0.69314718055994530942;  // |y| < 0.35: y^10 / 10! < 2^-36
-  double e = 1.0 / 362880;
-  e = fma(e, y, 1.0 / 40320);
-  e = fma(e, y, 1.0 / 5040);
-  e = fma(e, y, 1.0 / 720);
-  e = fma(e, y, 1.0 / 120);
-  e = fma(e, y, 1.0 / 24);
-  e = fma(e, y, 1.0 / 6);
-  e = fma(e, y, 0.5);
-  e = fma(e, y, 1.0);
-  e = fma(e, y, 1.0);
-  return __double2ull_rn(e * __hiloint2double((1023 + 44 + (int)nf) << 20, 0));
-}
-
+// (no memory clobber: the barriers around them order these loads, and several are in flight at once)
 __device__ __forceinline__ u64 peer_u64(const u64* p, int rank) {
   u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(smem_cluster_addr(p, rank)) : "memory");
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(smem_cluster_addr(p, rank)));
   return v;
 }
 __device__ __forceinline__ int peer_int(const int* p, int rank) {
   int v;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(smem_cluster_addr(p, rank)) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(smem_cluster_addr(p, rank)));
   return v;
 }
 __device__ __forceinline__ float peer_float(const float* p, int rank) {
   return __int_as_float(peer_int(reinterpret_cast<const int*>(p), rank));
+}
+
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 template <typename T>
@@ -123,6 +152,7 @@ struct Sampler {
   int w_len;            // tokens per warp, a multiple of 8
   int splits;
   Row row;
+  float step;           // histogram steps per unit of the logit
 
   __device__ __forceinline__ void sync() const {
     if (splits > 1) cluster_sync_all();
@@ -143,19 +173,62 @@ struct Sampler {
     }
   }
 
+  __device__ __forceinline__ u64 weigh(float l) const { return weight(row, sh.powers, l); }
+
+  // equal steps of the logit; the last takes everything 2^64 below the largest weight
+  __device__ __forceinline__ int bin_of(float l) const {
+    return l == row.mx ? 0 : (int)fminf((row.mx - l) * step, (float)(kBins - 1));
+  }
+
+  __device__ __forceinline__ void clear(int words, int bins) {
+    for (int k = 0; k < words; ++k)
+      for (int i = threadIdx.x; i < bins; i += kThreads) sh.part[k][i] = 0;
+    __syncthreads();
+  }
+  // adds to the block's histogram; kWeights: a weight below 2^45, else a count
+  template <bool kWeights>
+  __device__ __forceinline__ void add(int bin, u64 w) {
+    if constexpr (!kWeights) {
+      atomicAdd(&sh.part[0][bin], 1u);
+    } else {
+      const uint32_t a = (uint32_t)w & 0x7fffu, b = (uint32_t)(w >> 15) & 0x7fffu, c = (uint32_t)(w >> 30);
+      if (a) atomicAdd(&sh.part[0][bin], a);
+      if (b) atomicAdd(&sh.part[1][bin], b);
+      if (c) atomicAdd(&sh.part[2][bin], c);
+    }
+  }
+
   // First bin whose inclusive sum over the cluster reaches the goal, a whole number
   // from 1 to the sum of all bins that goal_of(sum) gives; sets sh.bin and sh.excl.
   template <class Fn>
-  __device__ __forceinline__ u64 find_bin(int bins, Fn&& goal_of) {
+  __device__ __forceinline__ u64 find_bin(int words, int bins, Fn&& goal_of) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __syncthreads();
     u64 v[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int bin = threadIdx.x * 2 + i;
       if (bin < bins) {
-        if (splits == 1) v[i] = sh.hist[bin];
-        else
-          for (int r = 0; r < splits; ++r) v[i] += peer_u64(&sh.hist[bin], r);
+        v[i] = sh.part[0][bin];
+        if (words == 3) v[i] += ((u64)sh.part[1][bin] << 15) + ((u64)sh.part[2][bin] << 30);
+        if (splits > 1) sh.hist[bin] = v[i];
+      }
+    }
+    if (splits > 1) {
+      cluster_sync_all();
+      u64 x[2][kMaxSplits];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) {
+          const int bin = threadIdx.x * 2 + i;
+          x[i][r] = r < splits && bin < bins ? peer_u64(&sh.hist[bin], r) : 0;
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[i] = 0;
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) v[i] += x[i][r];
       }
     }
     u64 incl = v[0] + v[1];
@@ -186,59 +259,67 @@ struct Sampler {
     return goal;
   }
 
-  // Order key of the token at which the running sum, in order, of val(logit) over the
-  // tokens at or before `border` reaches its goal.
-  template <class Val, class Goal>
-  __device__ u64 select(float mn, u64 border, Val&& val, Goal&& goal_of) {
-    // equal steps of the logit; the last takes everything 2^64 below the largest weight
-    const float range = fminf(row.mx - mn, 64.f / row.cf);
-    const float step = range > 0.f ? (kBins - 1) / range : 0.f;
-    auto bin_of = [&](float l) {
-      return l == row.mx ? 0 : (int)fminf((row.mx - l) * step, (float)(kBins - 1));
-    };
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
+  // Lists the cluster's tokens for which open(logit, index) holds.  Returns how many;
+  // up to kCap of them, `keys` (sh.list or sh.all) holds their order keys, unordered.
+  template <class Open>
+  __device__ __forceinline__ int gather(Open&& open, const u64*& keys) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     each([&](float l, int idx) {
-      if (order_key(l, idx) >= border) {
-        const u64 w = val(l);
-        if (w) atomicAdd(&sh.hist[bin_of(l)], w);
+      if (open(l, idx)) {
+        const int n = atomicAdd(&sh.count, 1);
+        if (n < kCap) sh.list[n] = order_key(l, idx);
       }
     });
     sync();
-    const u64 goal = find_bin(kBins, goal_of);
+    keys = sh.list;
+    if (splits == 1) return sh.count;
+    const int mine = lane < splits ? peer_int(&sh.count, lane) : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < kMaxSplits; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const int n = __shfl_sync(0xffffffffu, incl, splits - 1);
+    if (n > kCap) return n;
+    keys = sh.all;
+    // warp w copies the lists of blocks w, w + kWarps, ...
+    for (int r = threadIdx.x >> 5; r < splits; r += kWarps) {
+      const int m = __shfl_sync(0xffffffffu, mine, r), at = __shfl_sync(0xffffffffu, incl, r) - m;
+      for (int i = lane; i < m; i += 32) sh.all[at + i] = peer_u64(&sh.list[i], r);
+    }
+    __syncthreads();
+    return n;
+  }
+
+  // Order key of the token at which the running sum, in order, of the counts or weights
+  // of the tokens at or before `border` reaches its goal.
+  template <bool kWeights, class Goal>
+  __device__ u64 select(u64 border, Goal&& goal_of) {
+    constexpr int kWords = kWeights ? 3 : 1;
+    auto val = [&](float l) -> u64 { return kWeights ? weigh(l) : 1; };
+    clear(kWords, kBins);
+    each([&](float l, int idx) {
+      if (border == 0 || order_key(l, idx) >= border) add<kWeights>(bin_of(l), val(l));
+    });
+    const u64 goal = find_bin(kWords, kBins, goal_of);
     const int bin = sh.bin;
     u64 sum = sh.excl;   // of the tokens before those still in question
     int shift = 64;      // the upper 64 - shift bits of their keys are `prefix`
     u64 prefix = 0;
     while (true) {
-      auto open = [&](float l, u64 key) {
-        return key >= border && bin_of(l) == bin && (shift == 64 || (key >> shift) == prefix);
-      };
-      if (threadIdx.x == 0) sh.count = 0;
-      __syncthreads();
-      each([&](float l, int idx) {
-        const u64 key = order_key(l, idx);
-        if (open(l, key)) {
-          const int n = atomicAdd(&sh.count, 1);
-          if (n < kCap) sh.list[n] = key;
-        }
-      });
-      sync();
-      int n = 0;
-      for (int r = 0; r < splits; ++r) n += splits > 1 ? peer_int(&sh.count, r) : sh.count;
+      const u64* list;
+      const int n = gather(
+          [&](float l, int idx) {
+            if (bin_of(l) != bin) return false;
+            const u64 key = order_key(l, idx);
+            return key >= border && (shift == 64 || (key >> shift) == prefix);
+          },
+          list);
       if (n <= kCap) {
-        const u64* list = sh.list;
-        if (splits > 1) {
-          int at = 0;
-          for (int r = 0; r < splits; ++r) {
-            const int m = peer_int(&sh.count, r);
-            for (int i = threadIdx.x; i < m; i += kThreads) sh.all[at + i] = peer_u64(&sh.list[i], r);
-            at += m;
-          }
-          list = sh.all;
-          __syncthreads();
-        }
-        u64* w = sh.hist;
+        u64* w = sh.hist;  // (every block has passed the gather's barrier: the histogram has been read)
         for (int i = threadIdx.x; i < n; i += kThreads) w[i] = val(key_logit(list[i]));
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -253,24 +334,27 @@ struct Sampler {
       }
       // too many: the next 8 bits of the key, largest first
       shift -= 8;
-      for (int i = threadIdx.x; i < 256; i += kThreads) sh.hist[i] = 0;
-      sync();  // (the peers have read sh.count)
+      clear(kWords, 256);
       each([&](float l, int idx) {
         const u64 key = order_key(l, idx);
-        if (key >= border && bin_of(l) == bin && (shift == 56 || (key >> (shift + 8)) == prefix)) {
-          const u64 w = val(l);
-          if (w) atomicAdd(&sh.hist[255 - (int)((key >> shift) & 255)], w);
-        }
+        if (key >= border && bin_of(l) == bin && (shift == 56 || (key >> (shift + 8)) == prefix))
+          add<kWeights>(255 - (int)((key >> shift) & 255), val(l));
       });
-      sync();
       const u64 left = sum;
-      find_bin(256, [&](u64) { return goal - left; });
+      find_bin(kWords, 256, [&](u64) { return goal - left; });
       sum = left + sh.excl;
       prefix = (prefix << 8) | (u64)(255 - sh.bin);
-      sync();  // the histogram has been read
+      sync();  // the histogram and the counts have been read
     }
   }
 };
+
+// The running sum that the chosen token is the first to pass (0 <= goal < total)
+__device__ __forceinline__ u64 choice(float u, u64 total) {
+  const double want = fmin(fmax((double)u, 0.0), 1.0) * (double)total;  // NaN: 0
+  const u64 goal = want >= (double)total ? total - 1 : (u64)want;
+  return goal < total ? goal : total - 1;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
@@ -283,17 +367,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   const int w_len = a.warp_len, len = w_len * kWarps, base = rank * len;
   const T* src = static_cast<const T*>(a.logits) + r * a.ld;
 
+  if (threadIdx.x < kPowers) sh.powers[threadIdx.x] = kPowerTable.v[threadIdx.x];
+
   // 1. the slice; tokens that cannot be chosen (NaN, past the end) become -inf
   float mx = -INFINITY, mn = INFINITY;
-  for (int v = threadIdx.x * 8; v < len; v += kThreads * 8) {
-    float l[8];
-    const int left = a.vocab - (base + v);
-    if (a.vec && left >= 8) {
-      load8<T>(src + base + v, l);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) l[i] = i < left ? to_float<T>(src[base + v + i]) : -INFINITY;
-    }
+  auto take = [&](int v, float* l) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (!(l[i] > -INFINITY)) l[i] = -INFINITY;
@@ -303,7 +381,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       }
     }
     store8<T>(slice + v, l);
+  };
+  int v = threadIdx.x * 8;
+  constexpr int kStep = kThreads * 8;
+  if (a.vec) {
+    const int whole = min(len, a.vocab - base);  // (may be negative)
+    for (; v + 3 * kStep + 8 <= whole; v += 4 * kStep) {  // four loads in flight
+      float l[4][8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) load8<T>(src + base + v + k * kStep, l[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) take(v + k * kStep, l[k]);
+    }
+    for (; v + 8 <= whole; v += kStep) {
+      float l[8];
+      load8<T>(src + base + v, l);
+      take(v, l);
+    }
   }
+  for (; v < len; v += kStep) {
+    float l[8];
+    const int left = a.vocab - (base + v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l[i] = i < left ? to_float<T>(src[base + v + i]) : -INFINITY;
+    take(v, l);
+  }
+  const float own = mx;  // this thread's maximum
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -314,21 +417,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     sh.warp_mn[warp] = mn;
   }
   __syncthreads();
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     mx = fmaxf(mx, sh.warp_mx[w]);
     mn = fminf(mn, sh.warp_mn[w]);
   }
-  if (threadIdx.x == 0) {
-    sh.mx = mx;
-    sh.mn = mn;
-  }
-  Sampler<T> s{sh, slice, base, w_len, splits, Row{}};
-  s.sync();
-  if (splits > 1)
-    for (int k = 0; k < splits; ++k) {
-      mx = fmaxf(mx, peer_float(&sh.mx, k));
-      mn = fminf(mn, peer_float(&sh.mn, k));
+  if (splits > 1) {
+    if (threadIdx.x == 0) {
+      sh.mx = mx;
+      sh.mn = mn;
     }
+    cluster_sync_all();
+    if (lane < splits) {
+      mx = peer_float(&sh.mx, lane);
+      mn = peer_float(&sh.mn, lane);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+  }
+  Sampler<T> s{sh, slice, base, w_len, splits, Row{}, 0.f};
 
   const double temp = a.temperature_rows != nullptr ? (double)a.temperature_rows[r] : a.temperature;
   const int top_k = a.top_k_rows != nullptr ? a.top_k_rows[r] : a.top_k;
@@ -358,53 +468,126 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   }
 
   // between 1e-30 (below, only the largest logit has a weight) and 1e30 the products stay finite
+  const double c = 1.4426950408889634 / fmin(fmax(temp, 1e-30), 1e30);
   s.row.mx = mx;
-  s.row.mxd = (double)mx;
-  s.row.c = 1.4426950408889634 / fmin(fmax(temp, 1e-30), 1e30);
-  s.row.cf = (float)s.row.c;
-  const Row row = s.row;
+  s.row.ch = (float)c;
+  s.row.cl = (float)(c - (double)s.row.ch);
+  // min-p as the least weight; the largest weight, 2^44, always passes
+  const u64 least = min_p > 0.0 ? (u64)(fmin(min_p, 1.0) * 17592186044416.0) : 0;
+  const float range = fminf(mx - mn, 64.f / s.row.ch);
+  s.step = range > 0.f ? (kBins - 1) / range : 0.f;
+
   u64 border = 0;  // every token
-  if (top_k > 0 && top_k < a.vocab) {
+  const bool cut_k = top_k > 0 && top_k < a.vocab;
+  if (cut_k && top_k <= kShortK) {
+    // 2. step that the k-th of the threads' maxima falls into: k tokens at least lie at or above it
+    s.clear(1, kBins);
+    if (own > -INFINITY) s.template add<false>(s.bin_of(own), 1);
+    u64 maxima = 0;
+    s.find_bin(1, kBins, [&](u64 total) {
+      maxima = total;
+      return min((u64)top_k, total);
+    });
+    const int bin = maxima < (u64)top_k ? kBins - 1 : sh.bin;  // too few threads have tokens: all of them
+    const u64* list;
+    const int n = s.gather([&](float l, int) { return s.bin_of(l) <= bin; }, list);
+    if (n <= kCap) {
+      if (rank == 0) {
+        u64* w = sh.hist;
+        for (int i = threadIdx.x; i < n; i += kThreads) w[i] = s.weigh(key_logit(list[i]));
+        __syncthreads();
+        // entries i = thread, thread + kThreads: place in the order and sum before it
+        int place[kCap / kThreads];
+        u64 before[kCap / kThreads];
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < kCap / kThreads; ++e) {
+          const int i = threadIdx.x + e * kThreads;
+          place[e] = 0;
+          before[e] = 0;
+          if (i < n) {
+            const u64 key = list[i];
+            for (int j = 0; j < n; ++j)
+              if (list[j] > key) {
+                ++place[e];
+                before[e] += w[j];
+              }
+            if (place[e] < top_k) sum += w[i];
+          }
+        }
+        sum = warp_sum_u64(sum);
+        if (lane == 0) sh.warp_sum[warp] = sum;
+        __syncthreads();
+        u64 total = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) total += sh.warp_sum[k];
+        const u64 p_goal = top_p < 1.0 ? (u64)fmax(ceil(top_p * (double)total), 1.0) : ~0ull;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < kCap / kThreads; ++e) {
+          const int i = threadIdx.x + e * kThreads;
+          if (i < n) {
+            if (place[e] >= top_k || before[e] >= p_goal || w[i] < least) w[i] = 0;
+            sum += w[i];
+          }
+        }
+        sum = warp_sum_u64(sum);
+        if (lane == 0) sh.warp_sum[warp] = sum;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) total += sh.warp_sum[k];
+        const u64 goal = choice(u, total);
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+          const uint32_t back = (uint32_t)list[i];  // larger for lower indices
+          u64 at = 0;
+          for (int j = 0; j < n; ++j)
+            if ((uint32_t)list[j] > back) at += w[j];
+          if (at <= goal && goal < at + w[i]) a.tokens[r] = (int64_t)(0xffffffffu - back);
+        }
+      }
+      if (splits > 1) cluster_sync_all();  // no block leaves while its list is read
+      return;
+    }
+  }
+  if (cut_k) {
     // the k-th token of those that are not -inf, or the last of them
-    border = s.select(mn, border, [](float) { return (u64)1; },
-                      [&](u64 total) { return min((u64)top_k, total); });
+    s.sync();
+    border = s.template select<false>(border, [&](u64 total) { return min((u64)top_k, total); });
   }
   if (top_p < 1.0) {
     // the fewest whose sum is at least top_p of the whole; at least one unit, which keeps the first
-    border = s.select(mn, border, [&](float l) { return weight(row, l); },
-                      [&](u64 total) { return min((u64)fmax(ceil(top_p * (double)total), 1.0), total); });
+    border = s.template select<true>(
+        border, [&](u64 total) { return min((u64)fmax(ceil(top_p * (double)total), 1.0), total); });
   }
-  const float min_lw = min_p > 0.0 ? (float)fmin(log2(min_p), 0.0) : -INFINITY;
-  const double min_lwd = min_p > 0.0 ? fmin(log2(min_p), 0.0) : -INFINITY;
   auto kept = [&](float l, int idx) -> u64 {
-    if (order_key(l, idx) < border) return 0;
-    if (min_p > 0.0) {
-      // 64 bits where 32 cannot tell the sides apart
-      const float xf = log2_weight(row, l), slack = 1e-5f * (1.f - min_lw);
-      if (xf < min_lw - slack) return 0;
-      if (xf < min_lw + slack && l != row.mx && ((double)l - row.mxd) * row.c < min_lwd) return 0;
-    }
-    return weight(row, l);
+    if (border != 0 && order_key(l, idx) < border) return 0;
+    const u64 w = s.weigh(l);
+    return w >= least ? w : 0;
   };
 
   // 4. sums per warp, in the order of the vocabulary
   u64 sum = 0;
   s.each([&](float l, int idx) { sum += kept(l, idx); });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = warp_sum_u64(sum);
   if (lane == 0) sh.warp_sum[warp] = sum;
   s.sync();
+  const int n_sums = splits * kWarps;
+  if (threadIdx.x < n_sums)
+    sh.sums[threadIdx.x] = splits > 1 ? peer_u64(&sh.warp_sum[threadIdx.x % kWarps], threadIdx.x / kWarps)
+                                      : sh.warp_sum[threadIdx.x];
+  __syncthreads();
   u64 before = 0, total = 0;  // before: of the warps ahead of this one
-  for (int k = 0; k < splits; ++k)
-    for (int w = 0; w < kWarps; ++w) {
-      const u64 x = splits > 1 ? peer_u64(&sh.warp_sum[w], k) : sh.warp_sum[w];
-      if (k < rank || (k == rank && w < warp)) before += x;
-      total += x;
-    }
+  for (int i = lane; i < n_sums; i += 32) {
+    const u64 x = sh.sums[i];
+    if (i < rank * kWarps + warp) before += x;
+    total += x;
+  }
+  before = warp_sum_u64(before);
+  total = warp_sum_u64(total);
   // first token whose running sum passes u * total (the largest weight is 2^44 units: total > 0)
-  const double want = fmin(fmax((double)u, 0.0), 1.0) * (double)total;  // NaN: 0
-  u64 goal = want >= (double)total ? total - 1 : (u64)want;
-  if (goal >= total) goal = total - 1;
+  const u64 goal = choice(u, total);
   if (before <= goal && goal < before + sum) {
     const T* part = slice + warp * w_len;
     for (int v0 = 0; v0 < w_len; v0 += 256) {
@@ -448,7 +631,7 @@ void launch_sample(SampleArgs a, cudaStream_t s) {
   // takes to hold the row in 96 KB of each (two blocks on an SM).
   const int tile = kWarps * 8;
   int splits = 1;
-  while (splits < 8 && ((long long)a.rows * splits < 2 * 148 || (long long)a.vocab * (int)sizeof(T) > splits * 98304ll) &&
+  while (splits < kMaxSplits && ((long long)a.rows * splits < 2 * 148 || (long long)a.vocab * (int)sizeof(T) > splits * 98304ll) &&
          (long long)a.vocab > (long long)splits * kThreads * 4)
     splits *= 2;
   a.splits = splits;

@@ -113,6 +113,51 @@ def test_distribution_follows_the_softmax():
     assert (got - n * torch.softmax(x[0].double(), 0)).abs().max() <= 1
 
 
+def kernel_weight(l, mx, temperature):
+    """The CUDA kernel's integer weight, its fp32 steps one by one (csrc/kernels/sample.cu)."""
+    import numpy as np
+
+    f, d64 = np.float32, np.float64
+    fma = lambda a, b, c: f(d64(a) * d64(b) + d64(c))  # noqa: E731  (the sum's rounding to 53 bits is far below fp32's)
+    c = 1.4426950408889634 / temperature
+    ch = f(c)
+    cl = f(c - d64(ch))
+    l, mx = f(l), f(mx)
+    d = l - mx
+    bb = d - l
+    e = (l - (d - bb)) + (-mx - bb)
+    p = d * ch
+    q = fma(d, cl, fma(e, ch, fma(d, ch, -p)))
+    kf = np.rint(p * f(64))
+    t = (fma(kf, f(-1 / 64), p) + q) * f(0.69314718)
+    em1 = fma(fma(fma(t, f(1 / 24), f(1 / 6)), t, f(0.5)), t * t, t)
+    k = kf.astype(np.int64)
+    m = np.floor(2.0 ** ((k & 63) / 64.0) * 2.0**31 + 0.5).astype(np.int64)
+    w = m + np.rint(m.astype(f) * em1).astype(np.int64)
+    return np.where(p > f(-46), (w << 13) >> np.minimum(-(k >> 6), 62), 0)
+
+
+@pytest.mark.parametrize("temperature", [0.05, 0.7, 1.0, 1.3, 30.0])
+@pytest.mark.parametrize("kind", ["fp32", "bf16", "near", "wide"])
+def test_kernel_weights_hold_their_error(temperature, kind):
+    """2^-29 of the weight and one unit of 2^-44: r, its product with ln 2, the series and the
+    integer conversion round to 2^-24 of at most 2^-7.5, four times at most; the table to 2^-32."""
+    import numpy as np
+
+    g = np.random.default_rng(1)
+    mx = np.float32({"fp32": 11.7, "bf16": 13.0625, "near": 7.1, "wide": 900.0}[kind])
+    l = (mx - np.abs(g.standard_normal(200000)) * 8 * temperature).astype(np.float32)
+    if kind == "bf16":
+        l = torch.from_numpy(l).bfloat16().float().numpy()
+    if kind == "near":
+        l = (mx - np.abs(g.standard_normal(200000)) * 1e-3).astype(np.float32)
+    l = np.minimum(l, mx)
+    want = np.exp((l.astype(np.float64) - np.float64(mx)) / temperature) * 2.0**44
+    got = kernel_weight(l, mx, temperature).astype(np.float64)
+    assert (np.abs(got - want) <= want * 2.0**-29 + 1).all()
+    assert kernel_weight(np.full(3, mx), mx, temperature).tolist() == [2**44] * 3
+
+
 @pytest.mark.parametrize("kw,match", [
     (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
     (dict(top_k=-1), "top_k"), (dict(top_p=1.5), "top_p"), (dict(top_p=-0.1), "top_p"),

@@ -7,7 +7,6 @@ matching the reference's Python-float semantics.
 
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -119,8 +118,8 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     whose result does not depend on how the row is split; on the CPU it runs in
     float64.  No gradient flows through the choice.
     """
-    x = (logits._data if isinstance(logits, Tensor) else logits).detach()
-    u = (uniform._data if isinstance(uniform, Tensor) else uniform).detach()
+    x = logits._data if isinstance(logits, Tensor) else logits
+    u = uniform._data if isinstance(uniform, Tensor) else uniform
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"sample expects logits [..., vocab], got {list(x.shape)}")
     if not x.is_floating_point():
@@ -130,10 +129,10 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     if u.device != x.device:
         raise RuntimeError(f"uniform is on {u.device}, the logits on {x.device}")
     shape, vocab = x.shape[:-1], x.shape[-1]
-    x = x.reshape(-1, vocab)
+    x = x.detach() if x.dim() == 2 else x.detach().reshape(-1, vocab)
     rows = x.shape[0]
     real = torch.float32 if x.is_cuda else torch.float64
-    u = u.reshape(-1).to(real).contiguous()
+    u = u.detach().reshape(-1).to(real).contiguous()
     temperature = _setting(temperature, "temperature", rows, x.device, real, 0.0, 1e30)
     top_k = _setting(top_k, "top_k", rows, x.device, torch.int32, 0, 2**31 - 1)
     top_p = _setting(top_p, "top_p", rows, x.device, real, 0.0, 1.0)
@@ -143,14 +142,14 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
 
         if vocab > 393216:
             raise ValueError(f"the CUDA kernel takes vocabularies up to 393216, got {vocab}")
-        guard = contextlib.nullcontext()
-        if x.device.index != torch.cuda.current_device():
-            guard = torch.cuda.device(x.device)
-        with guard:
+        if x.device.index == torch._C._cuda_getDevice():
             token = K.sample_tokens(x, u, temperature, top_k, top_p, min_p)
+        else:
+            with torch.cuda.device(x.device):
+                token = K.sample_tokens(x, u, temperature, top_k, top_p, min_p)
     else:
         token = _sample_cpu(x.double(), u, temperature, top_k, top_p, min_p)
-    return Tensor._wrap(token.reshape(shape))
+    return Tensor._wrap(token if len(shape) == 1 else token.reshape(shape))
 
 
 def _sample_cpu(x: torch.Tensor, u: torch.Tensor, temperature, top_k, top_p, min_p) -> torch.Tensor:

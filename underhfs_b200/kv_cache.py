@@ -33,6 +33,9 @@ def _raw(t) -> torch.Tensor:
     return t if isinstance(t, torch.Tensor) else t._data
 
 
+_HERE = contextlib.nullcontext()
+
+
 def quantize_groups(x: torch.Tensor) -> torch.Tensor:
     """The values (float64) that the 4-bit codes of x [..., D] stand for.
 
@@ -62,9 +65,10 @@ class QuantizedKVCache:
             if int(value) < 1:
                 raise ValueError(f"{name} must be at least 1, got {value}")
         self.device = torch.device(device)
+        self._cuda = self.device.type == "cuda"
         self.layers, self.batch, self.kv_heads = int(layers), int(batch), int(kv_heads)
         self.head_dim, self.max_len = int(head_dim), int(max_len)
-        if self.device.type == "cuda":
+        if self._cuda:
             if self.head_dim not in (64, 128):
                 raise ValueError(f"the CUDA cache takes head_dim 64 or 128, got {head_dim}")
             pages = (self.max_len + PAGE - 1) // PAGE
@@ -84,7 +88,7 @@ class QuantizedKVCache:
     @property
     def nbytes(self) -> int:
         """Device bytes of the keys and values."""
-        if self.device.type == "cuda":
+        if self._cuda:
             return self.pages.numel()
         return self._k.element_size() * 2 * self._k.numel()
 
@@ -96,18 +100,16 @@ class QuantizedKVCache:
     # ------------------------------------------------------------- checks
     def _on_device(self):
         """Launch on the cache's device, whichever is current."""
-        if self.device.type == "cuda" and self.device.index != torch.cuda.current_device():
-            return torch.cuda.device(self.device)
-        return contextlib.nullcontext()
+        if not self._cuda or self.device.index == torch._C._cuda_getDevice():
+            return _HERE
+        return torch.cuda.device(self.device)
 
     def _check_layer(self, layer: int) -> int:
         if not 0 <= layer < self.layers:
             raise IndexError(f"layer {layer} outside [0, {self.layers})")
         return layer
 
-    def _check_counts(self, counts):
-        if counts is None:
-            return None
+    def _check_counts(self, counts) -> torch.Tensor:
         counts = _raw(counts)
         if counts.shape != (self.batch,):
             raise ValueError(f"counts must have shape [{self.batch}], got {list(counts.shape)}")
@@ -117,12 +119,15 @@ class QuantizedKVCache:
             raise RuntimeError(f"counts are on {counts.device}, the cache on {self.device}")
         return counts.to(torch.int32).contiguous()
 
-    def _check_rows(self, t, name: str, heads: int | None):
-        t = _raw(t).detach()
-        want = f"[{self.batch}, tokens, {self.kv_heads if heads is None else 'heads'}, {self.head_dim}]"
-        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[3] != self.head_dim or (
-                heads is None and t.shape[2] != self.kv_heads):
-            raise ValueError(f"{name} must be {want}, got {list(t.shape)}")
+    def _check_rows(self, t, name: str, heads: int | None) -> torch.Tensor:
+        """t as [batch, tokens, heads (None: any), head_dim] on the cache's device."""
+        if not isinstance(t, torch.Tensor):
+            t = t._data
+        shape = t.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[3] != self.head_dim or (
+                heads is not None and shape[2] != heads):
+            want = f"[{self.batch}, tokens, {'heads' if heads is None else heads}, {self.head_dim}]"
+            raise ValueError(f"{name} must be {want}, got {list(shape)}")
         if t.device != self.device:
             raise RuntimeError(f"{name} is on {t.device}, the cache on {self.device}")
         if not t.is_floating_point():
@@ -144,20 +149,22 @@ class QuantizedKVCache:
         held on the device are checked there: tokens past ``max_len`` are left
         out and reported in the device status word."""
         self._check_layer(layer)
-        k, v = self._check_rows(k, "k", None), self._check_rows(v, "v", None)
+        k, v = self._check_rows(k, "k", self.kv_heads), self._check_rows(v, "v", self.kv_heads)
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError(f"k and v differ: {list(k.shape)} {k.dtype}, {list(v.shape)} {v.dtype}")
-        counts = self._check_counts(counts)
-        if counts is None:
+        if counts is not None:
+            counts = self._check_counts(counts)
+        else:
             self._check_room(k.shape[1])
         if k.shape[1] == 0:
             return
-        if self.device.type == "cuda":
+        if self._cuda:
             from underhfs_b200.ops import kernels as K
 
             with self._on_device():
                 K.kv4_append(self.pages[layer], k, v, self.lengths, counts, self.max_len)
             return
+        k, v = k.detach(), v.detach()
         for b in range(self.batch):
             n = k.shape[1] if counts is None else max(0, min(int(counts[b]), k.shape[1]))
             at = int(self.lengths[b])
@@ -175,24 +182,26 @@ class QuantizedKVCache:
         sees the keys up to its own; with ``window``, of those the last
         ``window`` and the first ``sinks``.  Rows t >= counts[b] are zeros."""
         self._check_layer(layer)
-        q = self._check_rows(q, "q", 0)
+        q = self._check_rows(q, "q", None)
         heads, tokens = q.shape[2], q.shape[1]
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads are not a multiple of {self.kv_heads} key / value heads")
-        counts = self._check_counts(counts)
-        if counts is None:
+        if counts is not None:
+            counts = self._check_counts(counts)
+        else:
             self._check_room(tokens)
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
         from underhfs_b200.ops import kernels as K
 
-        window, sinks = K.window_args(self.max_len, True, window, sinks)
-        if self.device.type == "cuda":
+        window, sinks = (0, 0) if window is None and sinks == 0 else K.window_args(self.max_len, True, window, sinks)
+        if self._cuda:
             if q.dtype not in (torch.bfloat16, torch.float16):
                 raise TypeError(f"q must be bf16 or fp16, got {q.dtype}")
             if tokens == 0:
                 return torch.empty_like(q)
             with self._on_device():
                 return K.kv4_attend(self.pages[layer], q, self.lengths, counts, self.max_len, scale, window, sinks)
+        q = q.detach()
         out = torch.zeros(q.shape, dtype=torch.float64)
         for b in range(self.batch):
             n = tokens if counts is None else max(0, min(int(counts[b]), tokens))
@@ -215,7 +224,7 @@ class QuantizedKVCache:
             raise ValueError(f"tokens {start}..{start + count - 1} are outside [0, {self.max_len})")
         if dtype not in (torch.float32, torch.float16, torch.bfloat16, torch.float64):
             raise TypeError(f"unsupported dtype {dtype}")
-        if self.device.type == "cuda":
+        if self._cuda:
             if dtype == torch.float64:
                 raise TypeError("the CUDA cache reads as fp32, fp16 or bf16")
             from underhfs_b200.ops import kernels as K

@@ -50,7 +50,9 @@ def dt(t: torch.Tensor) -> int:
 
 
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """Handle of the current stream of the current device (the raw query: a
+    torch.cuda.Stream object costs several microseconds a launch)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def ptr(t: torch.Tensor | None) -> int:

@@ -383,8 +383,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """`t` [B, T, H, D] itself where the cache kernels can read its rows in
     16-byte pieces (D contiguous, strides and start aligned), else a copy."""
-    per = 16 // t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in t.stride()[:3]):
+    b, n, h, d = t.stride()
+    if d == 1 and (t.data_ptr() | ((b | n | h) * t.element_size())) % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -396,7 +396,7 @@ def kv4_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: t
     of sequence b are written."""
     B, T, H, D = k.shape
     k, v = _rows16(k), _rows16(v)
-    core().kv4_append(dt(k), D, ptr(k), list(k.stride()[:3]), ptr(v), list(v.stride()[:3]), ptr(pages), ptr(lengths),
+    core().kv4_append(dt(k), D, ptr(k), k.stride(), ptr(v), v.stride(), ptr(pages), ptr(lengths),
                       ptr(counts), B, T, H, pages.shape[2], capacity, stream())
 
 
@@ -416,7 +416,7 @@ def kv4_attend(pages: torch.Tensor, q: torch.Tensor, lengths: torch.Tensor, coun
     B, Tq, Hq, D = q.shape
     q = _rows16(q)
     o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
-    core().kv4_attend(dt(q), D, ptr(q), list(q.stride()[:3]), ptr(pages), ptr(o), ptr(lengths), ptr(counts), B, Tq,
+    core().kv4_attend(dt(q), D, ptr(q), q.stride(), ptr(pages), ptr(o), ptr(lengths), ptr(counts), B, Tq,
                       Hq, pages.shape[1], pages.shape[2], capacity, float(scale), window, sinks, stream())
     return o
 
