@@ -535,6 +535,10 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The two halves of cluster_sync_all, for blocks that have work between them.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // Arrive on an mbarrier given by its shared::cluster address (either CTA).
 // Default semantics (release at CTA scope): used after tcgen05.wait::ld +
 // tcgen05.fence::before_thread_sync, which order the TMEM reads themselves.

@@ -172,7 +172,7 @@ struct SampleArgs {
   int top_k;
   const float *temperature_rows, *top_p_rows, *min_p_rows;
   const int* top_k_rows;
-  int splits, warp_len;    // set by the launcher, like vec
+  int splits, warp_len, long_cap;  // set by the launcher, like vec
   bool vec;
 };
 void sample_tokens(const SampleArgs& p, int dtype, cudaStream_t s);

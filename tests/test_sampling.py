@@ -113,7 +113,7 @@ def test_distribution_follows_the_softmax():
     assert (got - n * torch.softmax(x[0].double(), 0)).abs().max() <= 1
 
 
-def kernel_weight(l, mx, temperature):
+def kernel_weight(l, mx, temperature, exact):
     """The CUDA kernel's integer weight, its fp32 steps one by one (csrc/kernels/sample.cu)."""
     import numpy as np
 
@@ -123,25 +123,28 @@ def kernel_weight(l, mx, temperature):
     ch = f(c)
     cl = f(c - d64(ch))
     l, mx = f(l), f(mx)
-    d = l - mx
-    bb = d - l
-    e = (l - (d - bb)) + (-mx - bb)
+    d0, dmin = l - mx, f(f(-44.9) / ch)
+    d = np.maximum(d0, dmin)
     p = d * ch
-    q = fma(d, cl, fma(e, ch, fma(d, ch, -p)))
-    kf = np.rint(p * f(64))
-    t = (fma(kf, f(-1 / 64), p) + q) * f(0.69314718)
-    em1 = fma(fma(fma(t, f(1 / 24), f(1 / 6)), t, f(0.5)), t * t, t)
-    k = kf.astype(np.int64)
-    m = np.floor(2.0 ** ((k & 63) / 64.0) * 2.0**31 + 0.5).astype(np.int64)
-    w = m + np.rint(m.astype(f) * em1).astype(np.int64)
-    return np.where(p > f(-46), (w << 13) >> np.minimum(-(k >> 6), 62), 0)
+    q = fma(d, cl, fma(d, ch, -p))
+    if exact:
+        bb = d0 - l
+        e = (l - (d0 - bb)) + (-mx - bb)
+        q = fma(np.where(d0 < dmin, f(0), e), ch, q)
+    z = np.rint(d64(p) * 64)  # the sum with 1.5 * 2^23 rounds to a whole number
+    r = fma(f(z), f(-1 / 64), p) + q
+    em1 = r * fma(r, fma(r, f(0.055504109), f(0.24022651)), f(0.69314718))
+    k = z.astype(np.int64)
+    m0 = np.floor(2.0 ** ((k & 63) / 64.0) * 2.0**30 + 0.5).astype(np.int64)
+    m = m0 + np.rint(m0.astype(f) * em1).astype(np.int64)
+    return (m << 14) >> -(k >> 6)
 
 
 @pytest.mark.parametrize("temperature", [0.05, 0.7, 1.0, 1.3, 30.0])
 @pytest.mark.parametrize("kind", ["fp32", "bf16", "near", "wide"])
 def test_kernel_weights_hold_their_error(temperature, kind):
-    """2^-29 of the weight and one unit of 2^-44: r, its product with ln 2, the series and the
-    integer conversion round to 2^-24 of at most 2^-7.5, four times at most; the table to 2^-32."""
+    """2^-29 of the weight and one unit of 2^-44: r, the series, its product with the table's
+    entry and the conversion round to 2^-24 of at most 2^-7.5, about six times; the table to 2^-31."""
     import numpy as np
 
     g = np.random.default_rng(1)
@@ -153,9 +156,13 @@ def test_kernel_weights_hold_their_error(temperature, kind):
         l = (mx - np.abs(g.standard_normal(200000)) * 1e-3).astype(np.float32)
     l = np.minimum(l, mx)
     want = np.exp((l.astype(np.float64) - np.float64(mx)) / temperature) * 2.0**44
-    got = kernel_weight(l, mx, temperature).astype(np.float64)
-    assert (np.abs(got - want) <= want * 2.0**-29 + 1).all()
-    assert kernel_weight(np.full(3, mx), mx, temperature).tolist() == [2**44] * 3
+    for exact in (True, False) if kind == "bf16" else (True,):  # without the difference's error: 16-bit logits
+        got = kernel_weight(l, mx, temperature, exact).astype(np.float64)
+        near = np.abs(l) > np.abs(mx) * 2.0**-14 if not exact else np.full(l.shape, True)
+        assert (np.abs(got - want) <= want * 2.0**-29 + 1)[near].all()
+        assert kernel_weight(np.full(3, mx), mx, temperature, exact).tolist() == [2**44] * 3
+        far = np.array([-3.4e38, -np.inf, mx - 50 * temperature], dtype=np.float32)
+        assert kernel_weight(far, mx, temperature, exact).tolist() == [0, 0, 0]
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -214,6 +221,25 @@ def test_gpu_long_runs_of_equal_logits(vocab, kw, status_ok):
     for u in (0.0, 0.31, 0.999):
         check(x, torch.full((4,), u), "cuda", **kw)
     check(x.bfloat16(), torch.full((4,), 0.6), "cuda", **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("kw", [dict(k=200, p=0.8), dict(p=0.95), dict(p=0.99999), dict(t=20.0, p=0.9), dict(k=257),
+                                dict(t=0.0), dict(m=0.2)])
+def test_gpu_largest_vocabulary(kw, dtype, status_ok):
+    x, u = rows(2, 327680, 31, dtype)
+    check(x, u, "cuda", **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(p=0.9), dict(k=100, p=0.95), dict(k=100), dict(k=1000, p=0.6)])
+@pytest.mark.parametrize("shift", [0.0, 900.0, -30000.0])
+def test_gpu_list_and_slices_agree(kw, shift, status_ok):
+    """Peaked rows (a short list does) and flat ones (it does not), near 0 and far from it."""
+    for scale, t in ((4.0, 0.5), (0.01, 1.0), (3.0, 1e-4), (3.0, 60.0)):
+        x, u = rows(3, 9001, 41, scale=scale)
+        check(x + shift, u, "cuda", t=t, **kw)
 
 
 @pytest.mark.gpu
@@ -278,7 +304,7 @@ def test_gpu_captured_and_replayed_and_other_stream(status_ok):
 @pytest.mark.gpu
 def test_gpu_refusals():
     with pytest.raises(ValueError, match="vocabularies up to"):
-        F.sample(torch.zeros(1, 400000, device="cuda"), torch.zeros(1, device="cuda"))
+        F.sample(torch.zeros(1, 327681, device="cuda"), torch.zeros(1, device="cuda"))
     with pytest.raises(RuntimeError, match="uniform is on"):
         F.sample(torch.zeros(1, 40, device="cuda"), torch.zeros(1))
     with pytest.raises(RuntimeError, match="top_p is on"):

@@ -114,7 +114,7 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     least the largest logit is always kept).
 
     Logits of -inf and NaN are never chosen; a row without any other gives -1.
-    On CUDA (fp32, fp16, bf16, vocabularies up to 393216) this is one kernel
+    On CUDA (fp32, fp16, bf16, vocabularies up to 327680) this is one kernel
     whose result does not depend on how the row is split; on the CPU it runs in
     float64.  No gradient flows through the choice.
     """
@@ -140,8 +140,8 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     if x.is_cuda:
         from underhfs_b200.ops import kernels as K
 
-        if vocab > 393216:
-            raise ValueError(f"the CUDA kernel takes vocabularies up to 393216, got {vocab}")
+        if vocab > 327680:
+            raise ValueError(f"the CUDA kernel takes vocabularies up to 327680, got {vocab}")
         if x.device.index == torch._C._cuda_getDevice():
             token = K.sample_tokens(x, u, temperature, top_k, top_p, min_p)
         else:
