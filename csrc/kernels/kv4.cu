@@ -9,13 +9,14 @@
 //
 // Layout.  A page holds 32 tokens of one head, contiguous (D * 40 bytes), so a
 // warp fetches it with one bulk copy:
-//   K codes [32 tokens][D / 2 bytes], K (s, lo) pairs [32][D / 32],
-//   V codes [32 tokens][D / 2 bytes], V s [D / 32][32], V lo [D / 32][32].
-// Word (8 codes) w of a K row holds channels 32 * (w % NG) + 8 * (w / NG) ..+7
-// (NG = D / 32): the quarter-warp lane that owns word w / NG reads its words of
-// all groups with one load.  A V row is in channel order.  The V s / lo planes
-// are permuted within 16 tokens (vslot) so that the two tokens of an MMA operand
-// register are neighbours.
+//   K codes [32 tokens][D / 2 bytes], K s [32][NG], K lo [32][NG],
+//   V codes [32 tokens][D / 2 bytes], V s [16 pairs][NG][2], V lo [16 pairs][NG][2]
+// with NG = D / 32 groups.  Word (8 codes) w of a K row holds channels
+// 32 * (w % NG) + 8 * (w / NG) ..+7: the quarter-warp lane that owns w / NG reads its words
+// of all groups with one load.  Half word (4 codes) e of a V row holds channels
+// 32 * (2 * (w % NW) + (e & 1)) + 4 * (w / NW) ..+3, w = e / 2, NW = D / 64: lane w / NW reads
+// 4 channels of every group with one load.  Tokens t and t + 4 of 8 are a pair: the two
+// tokens of an MMA operand register.
 #include <stdexcept>
 #include <string>
 
@@ -36,15 +37,23 @@ struct Kv4 {
   static constexpr int NG = D / kGroup;
   static constexpr int kCodes = kPage * D / 2;    // bytes of K (or V) codes
   static constexpr int kMeta = kPage * NG * 4;    // bytes of K (or V) s / lo
-  static constexpr int kKM = kCodes, kVC = kCodes + kMeta, kVM = 2 * kCodes + kMeta;
+  static constexpr int kKS = kCodes, kKL = kKS + kMeta / 2, kVC = kCodes + kMeta, kVS = 2 * kCodes + kMeta,
+                       kVL = kVS + kMeta / 2;
   static constexpr int kBytes = 2 * (kCodes + kMeta);
   static_assert(kBytes == D * 40 && kBytes % 16 == 0, "page size");
 };
 
-// position of a token's V s / lo within its plane: tokens t and t + 4 of 8 adjacent
-__device__ __forceinline__ int vslot(int tok) {
-  const int r = tok & 7;
-  return (tok & ~7) + (r < 4 ? 2 * r : 2 * r - 7);
+// place of a token's V s (or lo) of group gi in its plane
+template <int D>
+__device__ __forceinline__ int vslot(int tok, int gi) {
+  const int pair = (tok >> 4) * 8 + (tok & 8 ? 4 : 0) + (tok & 3);
+  return (pair * Kv4<D>::NG + gi) * 2 + ((tok >> 2) & 1);
+}
+// place of the half word that holds channels 4 c .. 4 c + 3 in a V row
+template <int D>
+__device__ __forceinline__ int vhalf(int c) {
+  const int gi = c / 8;
+  return ((c % 8) * (D / 64) + gi / 2) * 2 + (gi & 1);
 }
 
 // ------------------------------------------------------------ write / read
@@ -116,13 +125,17 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
   const int tok = (int)(pos % kPage), gi = lw / 4;
   if (!is_v) {
     reinterpret_cast<uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi] = word;
-    if (lw % 4 == 0) reinterpret_cast<__half2*>(page + F::kKM)[tok * F::NG + gi] = __halves2half2(s_h, lo_h);
-  } else {
-    reinterpret_cast<uint32_t*>(page + F::kVC)[tok * LPR + lw] = word;
     if (lw % 4 == 0) {
-      __half* m = reinterpret_cast<__half*>(page + F::kVM);
-      m[gi * kPage + vslot(tok)] = s_h;
-      m[(F::NG + gi) * kPage + vslot(tok)] = lo_h;
+      reinterpret_cast<__half*>(page + F::kKS)[tok * F::NG + gi] = s_h;
+      reinterpret_cast<__half*>(page + F::kKL)[tok * F::NG + gi] = lo_h;
+    }
+  } else {
+    uint16_t* row_v = reinterpret_cast<uint16_t*>(page + F::kVC + tok * (D / 2));
+    row_v[vhalf<D>(2 * lw)] = (uint16_t)word;
+    row_v[vhalf<D>(2 * lw + 1)] = (uint16_t)(word >> 16);
+    if (lw % 4 == 0) {
+      reinterpret_cast<__half*>(page + F::kVS)[vslot<D>(tok, gi)] = s_h;
+      reinterpret_cast<__half*>(page + F::kVL)[vslot<D>(tok, gi)] = lo_h;
     }
   }
 }
@@ -144,14 +157,13 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
   __half s, lo;
   if (!is_v) {
     w = reinterpret_cast<const uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi];
-    const __half2 m = reinterpret_cast<const __half2*>(page + F::kKM)[tok * F::NG + gi];
-    s = __low2half(m);
-    lo = __high2half(m);
+    s = reinterpret_cast<const __half*>(page + F::kKS)[tok * F::NG + gi];
+    lo = reinterpret_cast<const __half*>(page + F::kKL)[tok * F::NG + gi];
   } else {
-    w = reinterpret_cast<const uint32_t*>(page + F::kVC)[tok * LPR + lw];
-    const __half* m = reinterpret_cast<const __half*>(page + F::kVM);
-    s = m[gi * kPage + vslot(tok)];
-    lo = m[(F::NG + gi) * kPage + vslot(tok)];
+    const uint16_t* row_v = reinterpret_cast<const uint16_t*>(page + F::kVC + tok * (D / 2));
+    w = row_v[vhalf<D>(2 * lw)] | ((uint32_t)row_v[vhalf<D>(2 * lw + 1)] << 16);
+    s = reinterpret_cast<const __half*>(page + F::kVS)[vslot<D>(tok, gi)];
+    lo = reinterpret_cast<const __half*>(page + F::kVL)[vslot<D>(tok, gi)];
   }
   const float sf = __half2float(s), lf = __half2float(lo);
   float f[8];
@@ -166,28 +178,30 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
 // out); the 16 side is 16 tokens for S^T = K Q^T and 16 channels for O^T = V^T P^T,
 // so the codes, the operand that costs instructions, are read with no padding.
 //
-// The kernel is bound by HBM (0.625 bytes a value) as long as unpacking stays
-// under about 3 instructions a value:
-//   K  (w & 0x000f000f) | 0x64006400 is the fp16 pair 1024 + code, and with mask
-//      0x00f000f0 it is 1024 + 16 code: one LOP3 for two codes.  The 16 goes into
-//      q (q / 16 in those places), the 1024 into the accumulator's start value
-//      (-1024 sum q), and s and lo are applied in fp32 to the 16 x 8 product of
-//      each group: S = sum over groups of s * (q . code) + lo * sum(q).
-//   V  the tokens of a register pair have their own s and lo, so the code is
-//      freed of its 1024 (exact) and s * code + lo is one fp16 FMA (one rounding,
-//      2^-11 of the value at most; P is rounded to fp16 the same way).
-// q is scaled by softmax scale * log2(e) and, per query, by a power of two that
-// brings it to [1, 2), then rounded to fp16.
-//
+// The kernel is bound by HBM (0.625 bytes a value) as long as unpacking stays under about
+// 3 instructions a value, so the codes go to the tensor core as they are: w & 0x000f000f is a
+// pair of fp16 subnormals, code * 2^-24 exactly, and w & 0x00f000f0 one of 16 code * 2^-24:
+// one instruction for two codes, and no scale on this side.
+//   K  s and lo are per token, a row of the 16 x 8 products: S = sum over groups of
+//      s (q . code) + lo sum(q), s in fp32 on the product of each group, the lo term as
+//      one more product for all groups (sum(q) as two fp16 numbers).  q / 16 stands in the
+//      places of the odd codes.  q is only scaled, by a power of two per query that
+//      brings it to [1, 2): a bf16 or fp16 q goes in without a rounding.
+//   V  s and lo are per token, the products' inner dimension: O = sum over tokens of
+//      r code - 8 r + P (lo + 8 s) with r = P s rounded to fp16 (P itself goes in as two
+//      fp16 numbers); the last two terms are products with one row per group.  The 8 makes
+//      the rounding's share that of code - 8, not of code: without it its error was twice as
+//      large.
+// So K is not rounded, and for V only P s and lo + 8 s are.
 // Every warp works alone: it owns a ring of pages filled by bulk copies and takes
 // every kWarps-th page of the block's share, with its own running maximum (raised
-// only when a score exceeds it by 2^8) and sum.  The warps of a block are joined in
+// only when a score exceeds it by 2^2, which keeps P s in fp16's range) and sum.  The warps of a block are joined in
 // shared memory and the blocks of a cluster, which share one head's tokens, through
 // distributed shared memory: one launch, no workspace, no atomics, and a sum order
 // that depends on sizes only.
 constexpr int kWarps = 8;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 8.0f;
+constexpr float kRescale = 2.0f;  // s <= 2 * kRange / 15 = 8192
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -195,6 +209,13 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_zero(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -210,18 +231,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }  // 1024 + code
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return (w & 0x00f000f0u) | 0x64006400u; }  // 1024 + 16 code
+// codes 0 and 4 (even) or 1 and 5 (odd, times 16) of a word as fp16 subnormals; >> 8: the next two
+__device__ __forceinline__ uint32_t even_codes(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t odd_codes(uint32_t w) { return w & 0x00f000f0u; }
+constexpr float kCodeUnit = 16777216.f;  // 2^24
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
-__device__ __forceinline__ uint32_t dequant_lo(uint32_t w, __half2 s, __half2 lo) {
-  const __half2 c = __hsub2(as_half2(codes_lo(w)), __float2half2_rn(1024.f));
-  return as_u32(__hfma2(c, s, lo));
-}
-__device__ __forceinline__ uint32_t dequant_hi(uint32_t w, __half2 s, __half2 lo) {
-  const __half2 c = __hfma2(as_half2(codes_hi(w)), __float2half2_rn(0.0625f), __float2half2_rn(-64.f));
-  return as_u32(__hfma2(c, s, lo));
+// N consecutive 32-bit words of shared memory (N = 1, 2, 4)
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* dst, const uint8_t* src) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  else *dst = *reinterpret_cast<const uint32_t*>(src);
 }
 
 __device__ __forceinline__ float dsmem_load(const float* p, uint32_t rank) {
@@ -244,7 +266,7 @@ template <int D, typename T>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Attend a) {
   using F = Kv4<D>;
   using C = Kv4Attn<D>;
-  constexpr int NG = F::NG, NS = C::kStages, NT = D / 16;  // channel tiles of O^T
+  constexpr int NG = F::NG, NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBody);
@@ -294,7 +316,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
 
   // ---- queries: column g of the tile, channels 32 gi + 8 t .. + 7 of each group
   uint32_t qf[NG][4];
-  float noffs[NG][2], qsum[NG][2], scale2[2];
+  uint32_t qs_hi, qs_lo;  // sum(q) of groups 2 t, 2 t + 1 (second operand of the lo product)
+  float scale2[2];
   {
     const int m = row0 + g;
     float q[NG][8];
@@ -309,10 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
         load8<T>(src, q[gi]);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        q[gi][i] *= a.scale * kLog2e;
-        mx = fmaxf(mx, fabsf(q[gi][i]));
-      }
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(q[gi][i]));
     }
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -320,33 +340,37 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
     const uint32_t eb = min(__float_as_uint(mx) & 0x7f800000u, 227u << 23);
     const float up = mx > 1e-30f ? __uint_as_float(eb) : 1.f;
     const float dn = mx > 1e-30f ? __uint_as_float((254u << 23) - eb) : 1.f;
+    float sums[NG];
 #pragma unroll
     for (int gi = 0; gi < NG; ++gi) {
-      float off = 0.f, sum = 0.f;
+      float sum = 0.f;
       __half hq[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool odd = i & 1;  // odd nibbles come as 16 code
+        const bool odd = i & 1;  // odd codes come times 16
         hq[i] = __float2half_rn(q[gi][i] * (odd ? dn * 0.0625f : dn));
-        const float f = __half2float(hq[i]);
-        off += f;
-        sum += odd ? 16.f * f : f;
+        sum += odd ? 16.f * __half2float(hq[i]) : __half2float(hq[i]);
       }
-      // register k of a word holds nibbles k and k + 4
+      // register k of a word holds codes k and k + 4
 #pragma unroll
       for (int k = 0; k < 4; ++k) qf[gi][k] = as_u32(__halves2half2(hq[k], hq[k + 4]));
-      off += __shfl_xor_sync(0xffffffffu, off, 1);
-      off += __shfl_xor_sync(0xffffffffu, off, 2);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {  // columns 2 t and 2 t + 1 of the products
-        noffs[gi][c] = -1024.f * __shfl_sync(0xffffffffu, off, (2 * t + c) * 4);
-        qsum[gi][c] = __shfl_sync(0xffffffffu, sum, (2 * t + c) * 4);
-      }
+      sums[gi] = sum;
     }
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) scale2[c] = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4);
+    for (int gi = 0; gi < NG; gi += 2)
+      if (2 * t == gi) {
+        s0 = sums[gi];
+        s1 = sums[gi + 1];
+      }
+    const __half h0 = __float2half_rn(s0), h1 = __float2half_rn(s1);
+    qs_hi = as_u32(__halves2half2(h0, h1));
+    qs_lo = as_u32(__floats2half2_rn(s0 - __half2float(h0), s1 - __half2float(h1)));
+#pragma unroll
+    for (int c = 0; c < 2; ++c)  // columns 2 t and 2 t + 1 of the products
+      scale2[c] = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4) * (a.scale * kLog2e);
   }
   // tokens visible to columns 2 t, 2 t + 1: [low, lim) and [0, sinks)
   int lim[2], low[2];
@@ -363,9 +387,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   const int lim_all = (int)max(0ll, min(len + row0 / G + 1, (long long)a.capacity));  // visible to every live query
   const int low_all = rows > 0 && a.window > 0 ? (int)max(0ll, hi - a.window) : 0;
 
-  float o[NT][4];
+  float o[NG][2][4], o_lo[4] = {0.f, 0.f, 0.f, 0.f};  // code part by group; lo part: row = group
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < NG; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[i][j >> 2][j & 3] = 0.f;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   const int prow = (g & 1) ? (g >> 1) + 4 : (g >> 1);  // token of product row g within 8
 
@@ -381,33 +407,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       const int ra = mt * 16 + prow, rb = ra + 8;
-      uint32_t wa[NG], wb[NG], ma[NG], mb[NG];
-      if constexpr (NG == 4) {
-        *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(pg + ra * 64 + t * 16);
-        *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(pg + rb * 64 + t * 16);
-        *reinterpret_cast<uint4*>(ma) = *reinterpret_cast<const uint4*>(pg + F::kKM + ra * 16);
-        *reinterpret_cast<uint4*>(mb) = *reinterpret_cast<const uint4*>(pg + F::kKM + rb * 16);
-      } else {
-        *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(pg + ra * 32 + t * 8);
-        *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(pg + rb * 32 + t * 8);
-        *reinterpret_cast<uint2*>(ma) = *reinterpret_cast<const uint2*>(pg + F::kKM + ra * 8);
-        *reinterpret_cast<uint2*>(mb) = *reinterpret_cast<const uint2*>(pg + F::kKM + rb * 8);
-      }
-      s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+      uint32_t wa[NG], wb[NG], sa[NG / 2], sb[NG / 2], la, lb;
+      load_words<NG>(wa, pg + ra * (D / 2) + t * (4 * NG));
+      load_words<NG>(wb, pg + rb * (D / 2) + t * (4 * NG));
+      load_words<NG / 2>(sa, pg + F::kKS + ra * (2 * NG));
+      load_words<NG / 2>(sb, pg + F::kKS + rb * (2 * NG));
+      load_words<1>(&la, pg + F::kKL + ra * (2 * NG) + (t % (NG / 2)) * 4);
+      load_words<1>(&lb, pg + F::kKL + rb * (2 * NG) + (t % (NG / 2)) * 4);
+      float lo_part[4];
+      mma_f16_zero(lo_part, la, lb, la, lb, qs_hi, qs_lo);
+      float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
-        float c[4] = {noffs[gi][0], noffs[gi][1], noffs[gi][0], noffs[gi][1]};
-        mma_f16(c, codes_lo(wa[gi]), codes_lo(wb[gi]), codes_hi(wa[gi]), codes_hi(wb[gi]), qf[gi][0], qf[gi][1]);
-        mma_f16(c, codes_lo(wa[gi] >> 8), codes_lo(wb[gi] >> 8), codes_hi(wa[gi] >> 8), codes_hi(wb[gi] >> 8),
-                qf[gi][2], qf[gi][3]);
-        const float2 fa = __half22float2(as_half2(ma[gi])), fb = __half22float2(as_half2(mb[gi]));
-        s[mt][0] += fmaf(fa.x, c[0], fa.y * qsum[gi][0]);
-        s[mt][1] += fmaf(fa.x, c[1], fa.y * qsum[gi][1]);
-        s[mt][2] += fmaf(fb.x, c[2], fb.y * qsum[gi][0]);
-        s[mt][3] += fmaf(fb.x, c[3], fb.y * qsum[gi][1]);
+        float c[4];
+        mma_f16_zero(c, even_codes(wa[gi]), even_codes(wb[gi]), odd_codes(wa[gi]), odd_codes(wb[gi]), qf[gi][0],
+                     qf[gi][1]);
+        const uint32_t xa = wa[gi] >> 8, xb = wb[gi] >> 8;
+        mma_f16(c, even_codes(xa), even_codes(xb), odd_codes(xa), odd_codes(xb), qf[gi][2], qf[gi][3]);
+        const __half2 ha = as_half2(sa[gi / 2]), hb = as_half2(sb[gi / 2]);
+        const float fa = gi & 1 ? __high2float(ha) : __low2float(ha), fb = gi & 1 ? __high2float(hb) : __low2float(hb);
+        sc[0] = fmaf(fa, c[0], sc[0]);
+        sc[1] = fmaf(fa, c[1], sc[1]);
+        sc[2] = fmaf(fb, c[2], sc[2]);
+        sc[3] = fmaf(fb, c[3], sc[3]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[mt][e] *= scale2[e & 1];
+      for (int e = 0; e < 4; ++e) s[mt][e] = fmaf(sc[e], kCodeUnit, lo_part[e]) * scale2[e & 1];
     }
     if (key0 + kPage > lim_all || key0 < low_all) {
 #pragma unroll
@@ -436,15 +461,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
         l_run[c] *= alpha[c];
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        o[n][0] *= alpha[0];
-        o[n][1] *= alpha[1];
-        o[n][2] *= alpha[0];
-        o[n][3] *= alpha[1];
-      }
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[n][j >> 2][j & 3] *= alpha[j & 1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o_lo[j] *= alpha[j & 1];
     }
     const float base[2] = {m_run[0] == -INFINITY ? 0.f : m_run[0], m_run[1] == -INFINITY ? 0.f : m_run[1]};
-    uint32_t pb[2][2];  // P as the products' second operand: [16 tokens][8 queries]
+    // O^T += (s V)^T P^T: lane's tokens t, t + 4, t + 8, t + 12 of 16, channels 4 g .. + 3 of each group
+    constexpr int NW = D / 64;  // words per lane and token
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -452,38 +477,44 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
         s[mt][e] = ex2_approx(s[mt][e] - base[e & 1]);
         l_run[e & 1] += s[mt][e];
       }
-      pb[mt][0] = transpose8x8(as_u32(__floats2half2_rn(s[mt][0], s[mt][1])));
-      pb[mt][1] = transpose8x8(as_u32(__floats2half2_rn(s[mt][2], s[mt][3])));
-    }
-    // O^T += V^T P^T: lane's tokens t, t + 4, t + 8, t + 12 of 16, channels D/8 g .. + D/8 - 1
-    constexpr int NW = D / 64;  // words per lane and token
-    const int vg = g * NW / 4;  // their group
+      // P as the products' second operand [16 tokens][8 queries], in two fp16 parts
+      uint32_t ph[2], pl[2];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      uint32_t w[4][NW];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint8_t* src = pg + F::kVC + (mt * 16 + 4 * k + t) * (D / 2) + g * (4 * NW);
-        if constexpr (NW == 2) *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(src);
-        else w[k][0] = *reinterpret_cast<const uint32_t*>(src);
+      for (int i = 0; i < 2; ++i) {
+        const __half2 hi2 = __floats2half2_rn(s[mt][2 * i], s[mt][2 * i + 1]);
+        const float2 back = __half22float2(hi2);
+        ph[i] = transpose8x8(as_u32(hi2));
+        pl[i] = transpose8x8(as_u32(__floats2half2_rn(s[mt][2 * i] - back.x, s[mt][2 * i + 1] - back.y)));
       }
-      const uint8_t* meta = pg + F::kVM + (vg * kPage + mt * 16 + 2 * t) * 2;
-      const __half2 s0 = *reinterpret_cast<const __half2*>(meta), s1 = *reinterpret_cast<const __half2*>(meta + 16);
-      const __half2 l0 = *reinterpret_cast<const __half2*>(meta + NG * kPage * 2),
-                    l1 = *reinterpret_cast<const __half2*>(meta + NG * kPage * 2 + 16);
+      uint32_t w[4][NW], s0[NG], s1[NG], l0, l1;
 #pragma unroll
-      for (int nw = 0; nw < NW; ++nw) {
+      for (int k = 0; k < 4; ++k)
+        load_words<NW>(w[k], pg + F::kVC + (mt * 16 + 4 * k + t) * (D / 2) + g * (4 * NW));
+      const int pair0 = mt * 8 + t, pair1 = pair0 + 4;
+      load_words<NG>(s0, pg + F::kVS + pair0 * (4 * NG));
+      load_words<NG>(s1, pg + F::kVS + pair1 * (4 * NG));
+      load_words<1>(&l0, pg + F::kVL + (pair0 * NG + g % NG) * 4);
+      load_words<1>(&l1, pg + F::kVL + (pair1 * NG + g % NG) * 4);
+      uint32_t c0, c1;  // s of the lo product's row
+      load_words<1>(&c0, pg + F::kVS + (pair0 * NG + g % NG) * 4);
+      load_words<1>(&c1, pg + F::kVS + (pair1 * NG + g % NG) * 4);
+      l0 = as_u32(__hfma2(as_half2(c0), __float2half2_rn(8.f), as_half2(l0)));
+      l1 = as_u32(__hfma2(as_half2(c1), __float2half2_rn(8.f), as_half2(l1)));
+      mma_f16(o_lo, l0, 0u, l1, 0u, ph[0], ph[1]);
+      mma_f16(o_lo, l0, 0u, l1, 0u, pl[0], pl[1]);
 #pragma unroll
-        for (int q4 = 0; q4 < 2; ++q4) {  // nibbles 0..3, 4..7 of the word pair
-          const uint32_t x = __byte_perm(w[0][nw], w[1][nw], q4 ? 0x7632 : 0x5410);
-          const uint32_t y = __byte_perm(w[2][nw], w[3][nw], q4 ? 0x7632 : 0x5410);
-          float* acc = o[nw * 4 + q4 * 2];
-          mma_f16(acc, dequant_lo(x, s0, l0), dequant_hi(x, s0, l0), dequant_lo(y, s1, l1), dequant_hi(y, s1, l1),
-                  pb[mt][0], pb[mt][1]);
-          acc = o[nw * 4 + q4 * 2 + 1];
-          mma_f16(acc, dequant_lo(x >> 8, s0, l0), dequant_hi(x >> 8, s0, l0), dequant_lo(y >> 8, s1, l1),
-                  dequant_hi(y >> 8, s1, l1), pb[mt][0], pb[mt][1]);
-        }
+      for (int gi = 0; gi < NG; ++gi) {
+        const __half2 a0 = as_half2(s0[gi]), a1 = as_half2(s1[gi]);
+        const uint32_t b0 = as_u32(__hfma2(as_half2(ph[0]), a0, __hmul2(as_half2(pl[0]), a0)));
+        const uint32_t b1 = as_u32(__hfma2(as_half2(ph[1]), a1, __hmul2(as_half2(pl[1]), a1)));
+        const int nw = gi / 2;
+        const uint32_t x = __byte_perm(w[0][nw], w[1][nw], gi & 1 ? 0x7632 : 0x5410);
+        const uint32_t y = __byte_perm(w[2][nw], w[3][nw], gi & 1 ? 0x7632 : 0x5410);
+        mma_f16(o[gi][0], even_codes(x), odd_codes(x), even_codes(y), odd_codes(y), b0, b1);
+        const uint32_t x2 = x >> 8, y2 = y >> 8;
+        mma_f16(o[gi][1], even_codes(x2), odd_codes(x2), even_codes(y2), odd_codes(y2), b0, b1);
+        const uint32_t m8 = g == gi ? 0xc800c800u : 0u;  // -8 in row gi
+        mma_f16(o_lo, m8, 0u, m8, 0u, b0, b1);
       }
     }
     __syncwarp();  // every lane has read the page
@@ -502,6 +533,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
 #pragma unroll
     for (int w = 4; w <= 16; w <<= 1) l_run[c] += __shfl_xor_sync(0xffffffffu, l_run[c], w);
 
+  float lo_sum[NG][2];  // the lo part of this lane's channels and columns: lane (group, t) has it
+#pragma unroll
+  for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) lo_sum[gi][c] = __shfl_sync(0xffffffffu, o_lo[c], gi * 4 + t);
+
   // ---- join the block's warps
   float* wo = reinterpret_cast<float*>(smem);   // [kWarps][8][D]
   float* wm = wo + kWarps * 8 * D;              // [kWarps][8]
@@ -514,9 +551,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   for (int c = 0; c < 2; ++c) {
     const int col = 2 * t + c;
     if (col >= rows) continue;
-    float* dst = wo + (warp * 8 + col) * D + g * (D / 8);
+    float* dst = wo + (warp * 8 + col) * D + 4 * g;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(dst + 2 * n) = make_float2(o[n][c], o[n][2 + c]);
+    for (int gi = 0; gi < NG; ++gi)
+      *reinterpret_cast<float4*>(dst + gi * kGroup) =
+          make_float4(fmaf(o[gi][0][c], kCodeUnit, lo_sum[gi][c]), fmaf(o[gi][0][2 + c], kCodeUnit / 16, lo_sum[gi][c]),
+                      fmaf(o[gi][1][c], kCodeUnit, lo_sum[gi][c]), fmaf(o[gi][1][2 + c], kCodeUnit / 16, lo_sum[gi][c]));
     if (g == 0) {
       wm[warp * 8 + col] = m_run[c];
       wl[warp * 8 + col] = l_run[c];

@@ -207,25 +207,31 @@ def fill(B, keys, Hkv, D, lens, tq, dtype, seed=0):
 def check_attend(cache, q, got, lens, tq, window, sinks, scale=None):
     """Against 64 bits over the cached values.
 
-    The kernel rounds q to fp16 (a score moves by H16 sum|q||k| at most, and by a
-    few 2^-23 of 1024 s sum|q| per group in its fp32 sums, s < 1 here), P and the
-    dequantised v to fp16, and the result to q's type; a P below fp16's normal range
-    is off by 2^-25 of the largest.
+    q and the codes go in exactly (q may lose what is 2^-25 of its largest element: a score
+    moves by that times sum|k|), the fp32 sums of a score by a few 2^-23 of sum|q| (|lo| + 15 s).
+    Of v, P s and lo + 8 s are rounded to fp16 (H16), the first for s (code - 8), |code - 8| <= 8;
+    below fp16's normal range P s is off by 2^-25, for at most 8 steps.  Then the result's rounding.
     """
     D, G = q.shape[3], q.shape[2] // cache.kv_heads
     scale = D**-0.5 if scale is None else scale
     half = torch.finfo(q.dtype).eps / 2
     kk, vv = (t.double().repeat_interleave(G, 2) for t in cache.read(0, dtype=torch.float32))
+    # 8 s + |lo + 8 s| of each value's group: codes 0 and 15 are both in it
+    g = vv.unflatten(-1, (-1, 32))
+    lo, step = g.amin(-1, keepdim=True), (g.amax(-1, keepdim=True) - g.amin(-1, keepdim=True)) / 15
+    part = (8 * step + (lo + 8 * step).abs()).expand(g.shape).flatten(-2)
     for b, (n, t) in enumerate(zip(lens, tq)):
         assert (got[b, t:] == 0).all()
         if t == 0:
             continue
         pos = torch.arange(n - t, n, device="cuda")
         qb = q[b, :t].double()
-        o, size, score = attention(qb, kk[b, :n], vv[b, :n], pos, window, sinks, scale)
-        move = H16 * score + 1024 * 2.0**-21 * scale * qb.abs().sum(-1)
-        err = (torch.expm1(2 * move) + 2 * H16).unsqueeze(-1) * size + half * o.abs()
-        err = err + n * 2.0**-24 * vv[b, :n].abs().max() + 1e-6
+        o, _, score = attention(qb, kk[b, :n], vv[b, :n], pos, window, sinks, scale)
+        size, rounded = (attention(qb, kk[b, :n], x[b, :n], pos, window, sinks, scale)[0] for x in (vv.abs(), part))
+        big = scale * kk[b, :n].abs().max() * q.shape[3] * qb.abs().amax(-1)
+        move = 2.0**-25 * big + 2.0**-20 * (score + big)
+        err = torch.expm1(2 * move).unsqueeze(-1) * size + H16 * rounded + half * o.abs()
+        err = 1.01 * err + n * 2.0**-22 + 1e-6
         over = ((got[b, :t].double() - o).abs() - err).max().item()
         assert over <= 0, (b, over)
 
