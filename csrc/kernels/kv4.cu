@@ -57,34 +57,50 @@ __device__ __forceinline__ int vhalf(int c) {
 }
 
 // ------------------------------------------------------------ write / read
-// One thread per word (8 channels): 4 threads share a group, D / 8 a row.
-template <int D, typename T>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
-  using F = Kv4<D>;
-  constexpr int LPR = D / 8;  // threads per row
-  const bool is_v = blockIdx.y != 0;
-  const T* src = static_cast<const T*>(is_v ? a.v : a.k);
-  const long long sb = is_v ? a.v_stride_b : a.k_stride_b, st = is_v ? a.v_stride_t : a.k_stride_t,
-                  sh = is_v ? a.v_stride_h : a.k_stride_h;
-  const long long rows = (long long)a.B * a.T * a.H;
-  const long long idx = blockIdx.x * 256ll + threadIdx.x;
-  const long long row = idx / LPR;
-  const int lw = (int)(idx % LPR);  // channels [8 lw, 8 lw + 8)
-  const int h = (int)(row % a.H), t = (int)(row / a.H % a.T), b = (int)(row / ((long long)a.H * a.T));
-  bool live = row < rows;
-  long long pos = 0;
-  if (live) {
-    if (a.counts != nullptr && t >= a.counts[b]) live = false;
-    pos = (long long)a.lengths[b] + t;
-    if (live && (pos < 0 || pos >= a.capacity)) {
-      if (lw == 0) report_error(a.status, kErrBounds, 60);
-      live = false;
-    }
-  }
-  float x[8];
+// A thread takes 8 channels of K and the same of V: 4 threads share a group, D / 8 a row.
+// Both kernels move about 2.6 bytes a value, so a value may cost some 12 instructions
+// before they bound them; the batch is blockIdx.y, which leaves one 32-bit division.
+
+// round(y) for y = d / s in 0..15 as the low bits of a float (the sum with 1.5 * 2^23)
+constexpr float kMagic = 12582912.f;
+
+// The codes of x[8], code i in bits 4 i .. 4 i + 3: round-half-even((x - lo) / s).
+// y = (x - lo) * (1 / s) is off by less than 2^-17.2, so where it is at least 2^-17 away from a
+// half, which all but one in 2^13 threads see for all their values, its rounding is
+// right; the others take the remainder, which an FMA gives exactly, and the difference's
+// rounding error into account.
+__device__ __forceinline__ uint32_t quantize8(const float* x, float lo, float s) {
+  if (!(s > 0.f)) return 0;
+  const float inv = __fdividef(1.f, s), inv15 = inv * (1.f / 15.f);
+  uint32_t word = 0;
+  float worst = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (live) load8<T>(src + b * sb + t * st + h * sh + lw * 8, x);
+  for (int i = 7; i >= 0; --i) {
+    const float y = __saturatef((x[i] - lo) * inv15);  // (NaN: 0)
+    const float z = fmaf(y, 15.f, kMagic);
+    worst = fmaxf(worst, fabsf(fmaf(y, 15.f, kMagic - z)));
+    word = word * 16u + __float_as_uint(z);  // (the constant of all z is taken off below)
+  }
+  word -= 0x4B400000u * 0x11111111u;
+  if (worst < 0.5f - 1.f / 131072) return word;
+  const float half_s = 0.5f * s;
+  word = 0;
+  for (int i = 7; i >= 0; --i) {
+    const float d = x[i] - lo, bb = d - x[i];
+    const float e = (x[i] - (d - bb)) + (-lo - bb);  // x - lo = d + e
+    int k = __float2int_rn(fminf(fmaxf(d * inv, 0.f), 15.f));
+    const float r = fmaf(-(float)k, s, d);
+    const float up = (r - half_s) + e, dn = (r + half_s) + e;
+    const int odd = k & 1;
+    if (up > 0.f || (up == 0.f && odd)) ++k;
+    if (dn < 0.f || (dn == 0.f && odd)) --k;
+    word = word * 16u + (uint32_t)min(max(k, 0), 15);
+  }
+  return word;
+}
+
+// lo and s of a group (the values of four neighbouring threads)
+__device__ __forceinline__ void group_scale(const float* x, __half* lo_h, __half* s_h) {
   float mn = INFINITY, mx = -INFINITY;  // fminf / fmaxf pass over NaN
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -96,80 +112,84 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
-  if (!live) return;
   if (mn > mx) mn = mx = 0.f;  // nothing but NaN
   mn = fminf(fmaxf(mn, -kRange), kRange);
   mx = fminf(fmaxf(mx, -kRange), kRange);
-  const __half lo_h = __float2half_rn(mn);
-  const float lo = __half2float(lo_h);
-  const __half s_h = __float2half_rn(fmaxf((mx - lo) * (1.f / 15.f), 0.f));
-  const float s = __half2float(s_h), half_s = 0.5f * s;
-  const float inv = s > 0.f ? __fdividef(1.f, s) : 0.f;
-  uint32_t word = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // d + e = x - lo without a rounding; k = rhe((d + e) / s): a guess by the
-    // reciprocal, put right by the remainder, which an FMA gives without a rounding
-    const float d = x[i] - lo, bb = d - x[i];
-    const float e = (x[i] - (d - bb)) + (-lo - bb);
-    int k = __float2int_rn(fminf(fmaxf(d * inv, 0.f), 15.f));
-    const float r = fmaf(-(float)k, s, d);
-    const float up = (r - half_s) + e, dn = (r + half_s) + e;
-    const int odd = k & 1;
-    if (up > 0.f || (up == 0.f && odd)) ++k;
-    if (dn < 0.f || (dn == 0.f && odd)) --k;
-    k = s > 0.f ? min(max(k, 0), 15) : 0;
-    word |= (uint32_t)k << (4 * i);
+  *lo_h = __float2half_rn(mn);
+  *s_h = __float2half_rn(fmaxf((mx - __half2float(*lo_h)) * (1.f / 15.f), 0.f));
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
+  using F = Kv4<D>;
+  constexpr int LPR = D / 8;  // threads per row
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, row = idx / LPR;
+  const int lw = (int)(idx % LPR), gi = lw / 4, b = blockIdx.y;  // channels [8 lw, 8 lw + 8)
+  const int t = (int)(row / (uint32_t)a.H), h = (int)(row - (uint32_t)t * a.H);
+  bool live = t < (a.counts != nullptr ? min(a.counts[b], a.T) : a.T);
+  const long long pos = (long long)a.lengths[b] + t;
+  if (live && (pos < 0 || pos >= a.capacity)) {
+    if (lw == 0) report_error(a.status, kErrBounds, 60);
+    live = false;
   }
-  unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
-  const int tok = (int)(pos % kPage), gi = lw / 4;
-  if (!is_v) {
-    reinterpret_cast<uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi] = word;
-    if (lw % 4 == 0) {
-      reinterpret_cast<__half*>(page + F::kKS)[tok * F::NG + gi] = s_h;
-      reinterpret_cast<__half*>(page + F::kKL)[tok * F::NG + gi] = lo_h;
-    }
+  float k[8], v[8];
+  if (live) {
+    load8<T>(static_cast<const T*>(a.k) + b * a.k_stride_b + t * a.k_stride_t + h * a.k_stride_h + lw * 8, k);
+    load8<T>(static_cast<const T*>(a.v) + b * a.v_stride_b + t * a.v_stride_t + h * a.v_stride_h + lw * 8, v);
   } else {
-    uint16_t* row_v = reinterpret_cast<uint16_t*>(page + F::kVC + tok * (D / 2));
-    row_v[vhalf<D>(2 * lw)] = (uint16_t)word;
-    row_v[vhalf<D>(2 * lw + 1)] = (uint16_t)(word >> 16);
-    if (lw % 4 == 0) {
-      reinterpret_cast<__half*>(page + F::kVS)[vslot<D>(tok, gi)] = s_h;
-      reinterpret_cast<__half*>(page + F::kVL)[vslot<D>(tok, gi)] = lo_h;
-    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+  }
+  __half klo, ks, vlo, vs;
+  group_scale(k, &klo, &ks);
+  group_scale(v, &vlo, &vs);
+  const uint32_t kw = quantize8(k, __half2float(klo), __half2float(ks));
+  const uint32_t vw = quantize8(v, __half2float(vlo), __half2float(vs));
+  // V words hold 4 channels of an even group and 4 of the next: the threads of the two exchange
+  // halves, the even one takes the word of its first 4 channels
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
+  const uint32_t vword = gi & 1 ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
+  if (!live) return;
+  unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
+  const int tok = (int)(pos % kPage);
+  reinterpret_cast<uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi] = kw;
+  reinterpret_cast<uint32_t*>(page + F::kVC)[tok * LPR + vhalf<D>(2 * lw + (gi & 1)) / 2] = vword;
+  if (lw % 4 == 0) {
+    reinterpret_cast<__half*>(page + F::kKS)[tok * F::NG + gi] = ks;
+    reinterpret_cast<__half*>(page + F::kKL)[tok * F::NG + gi] = klo;
+    reinterpret_cast<__half*>(page + F::kVS)[vslot<D>(tok, gi)] = vs;
+    reinterpret_cast<__half*>(page + F::kVL)[vslot<D>(tok, gi)] = vlo;
   }
 }
 
-// out[b][t][h][:] = token start + t; one thread per word.
-template <int D, typename T>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
-  using F = Kv4<D>;
-  constexpr int LPR = D / 8;
-  const bool is_v = blockIdx.y != 0;
-  const long long idx = blockIdx.x * 256ll + threadIdx.x;
-  const long long row = idx / LPR;
-  if (row >= (long long)a.B * a.n * a.H) return;
-  const int lw = (int)(idx % LPR), gi = lw / 4;
-  const int h = (int)(row % a.H), t = (int)(row / a.H % a.n), b = (int)(row / ((long long)a.H * a.n));
-  const int pos = a.start + t, tok = pos % kPage;
-  const unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
-  uint32_t w;
-  __half s, lo;
-  if (!is_v) {
-    w = reinterpret_cast<const uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi];
-    s = reinterpret_cast<const __half*>(page + F::kKS)[tok * F::NG + gi];
-    lo = reinterpret_cast<const __half*>(page + F::kKL)[tok * F::NG + gi];
-  } else {
-    const uint16_t* row_v = reinterpret_cast<const uint16_t*>(page + F::kVC + tok * (D / 2));
-    w = row_v[vhalf<D>(2 * lw)] | ((uint32_t)row_v[vhalf<D>(2 * lw + 1)] << 16);
-    s = reinterpret_cast<const __half*>(page + F::kVS)[vslot<D>(tok, gi)];
-    lo = reinterpret_cast<const __half*>(page + F::kVL)[vslot<D>(tok, gi)];
-  }
+template <typename T>
+__device__ __forceinline__ void store_values(T* dst, uint32_t w, __half s, __half lo) {
   const float sf = __half2float(s), lf = __half2float(lo);
   float f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = fmaf(sf, (float)((w >> (4 * i)) & 15u), lf);
-  store8<T>(static_cast<T*>(is_v ? a.v : a.k) + row * D + lw * 8, f);
+  store8<T>(dst, f);
+}
+
+// out[b][t][h][:] = token start + t
+template <int D, typename T>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
+  using F = Kv4<D>;
+  constexpr int LPR = D / 8;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, row = idx / LPR;
+  const int lw = (int)(idx % LPR), gi = lw / 4, b = blockIdx.y;
+  const int t = (int)(row / (uint32_t)a.H), h = (int)(row - (uint32_t)t * a.H);
+  if (t >= a.n) return;
+  const int pos = a.start + t, tok = pos % kPage;
+  const unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
+  const uint32_t kw = reinterpret_cast<const uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi];
+  const uint16_t* vrow = reinterpret_cast<const uint16_t*>(page + F::kVC + tok * (D / 2));
+  const uint32_t vw = vrow[vhalf<D>(2 * lw)] | ((uint32_t)vrow[vhalf<D>(2 * lw + 1)] << 16);
+  const long long at = (((long long)b * a.n + t) * a.H + h) * D + lw * 8;
+  store_values<T>(static_cast<T*>(a.k) + at, kw, reinterpret_cast<const __half*>(page + F::kKS)[tok * F::NG + gi],
+                  reinterpret_cast<const __half*>(page + F::kKL)[tok * F::NG + gi]);
+  store_values<T>(static_cast<T*>(a.v) + at, vw, reinterpret_cast<const __half*>(page + F::kVS)[vslot<D>(tok, gi)],
+                  reinterpret_cast<const __half*>(page + F::kVL)[vslot<D>(tok, gi)]);
 }
 
 // --------------------------------------------------------------- attention
@@ -652,10 +672,11 @@ void check_rows(const void* p, int elem, long long sb, long long st, long long s
     throw std::runtime_error(std::string(what) + ": rows must be 16-byte aligned");
 }
 
-unsigned row_blocks(long long rows, int D, const char* what) {
-  const long long blocks = (rows * (D / 8) + 255) / 256;
-  if (blocks > 0x7fffffffll) throw std::runtime_error(std::string(what) + ": too many rows");
-  return (unsigned)blocks;
+// 256 threads a block, D / 8 a row; x: rows of one sequence, y: sequences
+dim3 row_grid(int B, int tokens, int H, int D, const char* what) {
+  const long long threads = (long long)tokens * H * (D / 8);
+  if (threads > 0x7fffff00ll || B > 65535) throw std::runtime_error(std::string(what) + ": too many rows");
+  return dim3((unsigned)((threads + 255) / 256), (unsigned)B);
 }
 
 }  // namespace
@@ -676,7 +697,7 @@ void kv4_append(const Kv4Append& p, int dtype, int D, cudaStream_t s) {
   check_rows(p.v, elem, p.v_stride_b, p.v_stride_t, p.v_stride_h, "kv4 append");
   Kv4Append a = p;
   a.status = device_status_ptr();
-  const dim3 grid(row_blocks((long long)p.B * p.T * p.H, D, "kv4 append"), 2);
+  const dim3 grid = row_grid(p.B, p.T, p.H, D, "kv4 append");
   UHFS_KV4_TYPES(dtype, if (D == 64) kv4_append_kernel<64, T><<<grid, 256, 0, s>>>(a);
                  else kv4_append_kernel<128, T><<<grid, 256, 0, s>>>(a));
   note_launch();
@@ -690,7 +711,7 @@ void kv4_read(const Kv4Read& a, int dtype, int D, cudaStream_t s) {
     throw std::runtime_error("kv4 read: tokens outside the cache");
   check_rows(a.k, 4, 0, 0, 0, "kv4 read");
   check_rows(a.v, 4, 0, 0, 0, "kv4 read");
-  const dim3 grid(row_blocks((long long)a.B * a.n * a.H, D, "kv4 read"), 2);
+  const dim3 grid = row_grid(a.B, a.n, a.H, D, "kv4 read");
   UHFS_KV4_TYPES(dtype, if (D == 64) kv4_read_kernel<64, T><<<grid, 256, 0, s>>>(a);
                  else kv4_read_kernel<128, T><<<grid, 256, 0, s>>>(a));
   note_launch();
