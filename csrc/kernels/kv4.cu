@@ -19,6 +19,7 @@
 // tokens of an MMA operand register.
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -57,108 +58,172 @@ __device__ __forceinline__ int vhalf(int c) {
 }
 
 // ------------------------------------------------------------ write / read
-// A thread takes 8 channels of K and the same of V: 4 threads share a group, D / 8 a row.
-// Both kernels move about 2.6 bytes a value, so a value may cost some 12 instructions
-// before they bound them; the batch is blockIdx.y, which leaves one 32-bit division.
+// A thread takes 8 channels of K and the same of V of kRows consecutive tokens: 4 threads
+// share a group, D / 8 a row.  Both kernels move about 2.6 bytes a value, so a value may
+// cost some 12 instructions before they bound them: the threads of a block span the heads
+// (and, where those are few, several runs of tokens), so that a place costs no division by
+// the number of heads and is worked out once for kRows tokens, whose loads overlap.
+template <int D>
+struct Place {
+  int h, lw, t0;  // head, 8 channels of it, first token
+  bool on;
+};
+template <int D, int kRows>
+__device__ __forceinline__ Place<D> place(int H) {
+  constexpr int LPR = D / 8;
+  const int span = H * LPR, per_block = span < 256 ? 256 / span : 1;  // runs of tokens per block
+  int u = blockIdx.x * 256 + threadIdx.x, run = 0;
+  if (span < 256) {
+    run = (int)threadIdx.x / span;
+    u = (int)threadIdx.x - run * span;
+  }
+  return Place<D>{u / LPR, u % LPR, ((int)blockIdx.y * per_block + run) * kRows, u < span && run < per_block};
+}
 
-// round(y) for y = d / s in 0..15 as the low bits of a float (the sum with 1.5 * 2^23)
+// y + kMagic has round(y) in its low bits, for |y| < 2^22
 constexpr float kMagic = 12582912.f;
 
-// The codes of x[8], code i in bits 4 i .. 4 i + 3: round-half-even((x - lo) / s).
-// y = (x - lo) * (1 / s) is off by less than 2^-17.2, so where it is at least 2^-17 away from a
-// half, which all but one in 2^13 threads see for all their values, its rounding is
-// right; the others take the remainder, which an FMA gives exactly, and the difference's
-// rounding error into account.
-__device__ __forceinline__ uint32_t quantize8(const float* x, float lo, float s) {
-  if (!(s > 0.f)) return 0;
-  const float inv = __fdividef(1.f, s), inv15 = inv * (1.f / 15.f);
+// The codes of x[8], code i in bits 4 i .. 4 i + 3: round-half-even((x - lo) / s) in 0..15.
+// kSure: at least 2^-17 away from a half, (x - lo) * (1 / s), which is off by less than 2^-17.2,
+// rounds to the code.
+constexpr float kSure = 0.5f - 1.f / 131072;
+__device__ __noinline__ uint32_t quantize8_exact(float4 x0, float4 x1, float lo, float s) {
+  const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+  const float inv = s > 0.f ? __fdividef(1.f, s) : 0.f, half_s = 0.5f * s;
   uint32_t word = 0;
-  float worst = 0.f;
 #pragma unroll
   for (int i = 7; i >= 0; --i) {
-    const float y = __saturatef((x[i] - lo) * inv15);  // (NaN: 0)
-    const float z = fmaf(y, 15.f, kMagic);
-    worst = fmaxf(worst, fabsf(fmaf(y, 15.f, kMagic - z)));
-    word = word * 16u + __float_as_uint(z);  // (the constant of all z is taken off below)
-  }
-  word -= 0x4B400000u * 0x11111111u;
-  if (worst < 0.5f - 1.f / 131072) return word;
-  const float half_s = 0.5f * s;
-  word = 0;
-  for (int i = 7; i >= 0; --i) {
-    const float d = x[i] - lo, bb = d - x[i];
-    const float e = (x[i] - (d - bb)) + (-lo - bb);  // x - lo = d + e
-    int k = __float2int_rn(fminf(fmaxf(d * inv, 0.f), 15.f));
-    const float r = fmaf(-(float)k, s, d);
-    const float up = (r - half_s) + e, dn = (r + half_s) + e;
-    const int odd = k & 1;
-    if (up > 0.f || (up == 0.f && odd)) ++k;
-    if (dn < 0.f || (dn == 0.f && odd)) --k;
-    word = word * 16u + (uint32_t)min(max(k, 0), 15);
+    const float d = x[i] - lo;
+    const float y = fminf(fmaxf(d * inv, 0.f), 15.f), z = y + kMagic;  // (NaN: 0)
+    int k = (int)(__float_as_uint(z) - __float_as_uint(kMagic));
+    if (!(fabsf(y - (z - kMagic)) < kSure)) {
+      // the remainder, which an FMA gives exactly, and the rounding error of x - lo = d + e
+      const float bb = d - x[i], e = (x[i] - (d - bb)) + (-lo - bb);
+      const float r = fmaf(-(float)k, s, d), up = (r - half_s) + e, dn = (r + half_s) + e;
+      const int odd = k & 1;
+      if (up > 0.f || (up == 0.f && odd)) ++k;
+      if (dn < 0.f || (dn == 0.f && odd)) --k;
+      k = s > 0.f ? min(max(k, 0), 15) : 0;
+    }
+    word = word * 16u + (uint32_t)k;
   }
   return word;
 }
 
-// lo and s of a group (the values of four neighbouring threads)
-__device__ __forceinline__ void group_scale(const float* x, __half* lo_h, __half* s_h) {
-  float mn = INFINITY, mx = -INFINITY;  // fminf / fmaxf pass over NaN
+// A group's lo and s (its values are those of four neighbouring threads) and this thread's codes.
+// Where every value is sure, within the codes' range and finite, the rounded product is the
+// code; about one in 2^11 values of a bf16 tensor is not (mostly ties), and its thread's eight go
+// the exact way.
+__device__ __forceinline__ uint32_t quantize8(const float* x, float mn, float mx, __half* lo_h, __half* s_h) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    mn = fminf(mn, x[i]);
-    mx = fmaxf(mx, x[i]);
-  }
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
+  for (int o = 1; o <= 2; o <<= 1) {  // (fminf and fmaxf pass over NaN)
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (mn > mx) mn = mx = 0.f;  // nothing but NaN
-  mn = fminf(fmaxf(mn, -kRange), kRange);
-  mx = fminf(fmaxf(mx, -kRange), kRange);
-  *lo_h = __float2half_rn(mn);
-  *s_h = __float2half_rn(fmaxf((mx - __half2float(*lo_h)) * (1.f / 15.f), 0.f));
+  const float lo0 = fminf(fmaxf(mn, -kRange), kRange), hi = fminf(fmaxf(mx, -kRange), kRange);
+  *lo_h = __float2half_rn(lo0);
+  const float lo = __half2float(*lo_h);
+  *s_h = __float2half_rn(fmaxf((hi - lo) * (1.f / 15.f), 0.f));
+  const float s = __half2float(*s_h), inv = __fdividef(1.f, s);  // (s = 0: infinite, and nothing is sure)
+  uint32_t word = 0;
+  bool sure = (mn - lo) * inv > -kSure && (mx - lo) * inv < 15.f + kSure;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const float d = x[i] - lo, z = fmaf(d, inv, kMagic);
+    sure = sure && fabsf(fmaf(d, inv, kMagic - z)) < kSure;  // (NaN and infinities are not)
+    word = word * 16u + __float_as_uint(z);                 // (their constant is taken off below)
+  }
+  word -= 0x4B400000u * 0x11111111u;
+  if (!sure)
+    word = quantize8_exact(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), lo, s);
+  return word;
 }
 
-template <int D, typename T>
+// 8 values as loaded
+template <typename T>
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  // the values, their least and their largest (NaN passed over), 16-bit types two at a time
+  __device__ __forceinline__ void range(float* x, float* mn, float* mx) const {
+    const T* h = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(h[i]);
+    if constexpr (sizeof(T) == 2) {
+      using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+      const T2* w = reinterpret_cast<const T2*>(v);
+      const T2 lo = __hmin2(__hmin2(w[0], w[1]), __hmin2(w[2], w[3]));
+      const T2 hi = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+      // (all NaN: fminf and fmaxf drop one at a time, the last is dropped by the neighbours')
+      *mn = fminf(fminf(to_float<T>(lo.x), to_float<T>(lo.y)), INFINITY);
+      *mx = fmaxf(fmaxf(to_float<T>(hi.x), to_float<T>(hi.y)), -INFINITY);
+    } else {
+      *mn = INFINITY;
+      *mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        *mn = fminf(*mn, x[i]);
+        *mx = fmaxf(*mx, x[i]);
+      }
+    }
+  }
+};
+
+template <int D, typename T, int kRows>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
   using F = Kv4<D>;
   constexpr int LPR = D / 8;  // threads per row
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, row = idx / LPR;
-  const int lw = (int)(idx % LPR), gi = lw / 4, b = blockIdx.y;  // channels [8 lw, 8 lw + 8)
-  const int t = (int)(row / (uint32_t)a.H), h = (int)(row - (uint32_t)t * a.H);
-  bool live = t < (a.counts != nullptr ? min(a.counts[b], a.T) : a.T);
-  const long long pos = (long long)a.lengths[b] + t;
-  if (live && (pos < 0 || pos >= a.capacity)) {
-    if (lw == 0) report_error(a.status, kErrBounds, 60);
-    live = false;
-  }
-  float k[8], v[8];
-  if (live) {
-    load8<T>(static_cast<const T*>(a.k) + b * a.k_stride_b + t * a.k_stride_t + h * a.k_stride_h + lw * 8, k);
-    load8<T>(static_cast<const T*>(a.v) + b * a.v_stride_b + t * a.v_stride_t + h * a.v_stride_h + lw * 8, v);
-  } else {
+  const Place<D> pl = place<D, kRows>(a.H);
+  const int lw = pl.lw, gi = lw / 4, b = blockIdx.z;  // channels [8 lw, 8 lw + 8)
+  const int count = a.counts != nullptr ? min(a.counts[b], a.T) : a.T;
+  const long long start = a.lengths[b];
+  Raw8<T> k[kRows], v[kRows];
+  bool live[kRows];
+  const T* src_k = static_cast<const T*>(a.k) + b * a.k_stride_b + (long long)pl.h * (int)a.k_stride_h + lw * 8;
+  const T* src_v = static_cast<const T*>(a.v) + b * a.v_stride_b + (long long)pl.h * (int)a.v_stride_h + lw * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+  for (int i = 0; i < kRows; ++i) {
+    const int t = pl.t0 + i;
+    live[i] = pl.on && t < count;
+    if (live[i] && (start + t < 0 || start + t >= a.capacity)) {
+      if (lw == 0) report_error(a.status, kErrBounds, 60);
+      live[i] = false;
+    }
+    k[i] = v[i] = Raw8<T>{};
+    if (live[i]) {
+      k[i].load(src_k + (long long)t * (int)a.k_stride_t);
+      v[i].load(src_v + (long long)t * (int)a.v_stride_t);
+    }
   }
-  __half klo, ks, vlo, vs;
-  group_scale(k, &klo, &ks);
-  group_scale(v, &vlo, &vs);
-  const uint32_t kw = quantize8(k, __half2float(klo), __half2float(ks));
-  const uint32_t vw = quantize8(v, __half2float(vlo), __half2float(vs));
-  // V words hold 4 channels of an even group and 4 of the next: the threads of the two exchange
-  // halves, the even one takes the word of its first 4 channels
-  const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
-  const uint32_t vword = gi & 1 ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
-  if (!live) return;
-  unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
-  const int tok = (int)(pos % kPage);
-  reinterpret_cast<uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi] = kw;
-  reinterpret_cast<uint32_t*>(page + F::kVC)[tok * LPR + vhalf<D>(2 * lw + (gi & 1)) / 2] = vword;
-  if (lw % 4 == 0) {
-    reinterpret_cast<__half*>(page + F::kKS)[tok * F::NG + gi] = ks;
-    reinterpret_cast<__half*>(page + F::kKL)[tok * F::NG + gi] = klo;
-    reinterpret_cast<__half*>(page + F::kVS)[vslot<D>(tok, gi)] = vs;
-    reinterpret_cast<__half*>(page + F::kVL)[vslot<D>(tok, gi)] = vlo;
+  unsigned char* head = a.pages + ((long long)b * a.H + pl.h) * a.pages_per_head * F::kBytes;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    if (!__any_sync(0xffffffffu, live[i])) continue;  // (a row's threads agree)
+    float x[8], mn, mx;
+    __half klo, ks, vlo, vs;
+    k[i].range(x, &mn, &mx);
+    const uint32_t kw = quantize8(x, mn, mx, &klo, &ks);
+    v[i].range(x, &mn, &mx);
+    const uint32_t vw = quantize8(x, mn, mx, &vlo, &vs);
+    // V words hold 4 channels of an even group and 4 of the next: the threads of the two exchange
+    // halves, the even one takes the word of its first 4 channels
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
+    const uint32_t vword = gi & 1 ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
+    if (!live[i]) continue;
+    const uint32_t pos = (uint32_t)(start + pl.t0 + i), tok = pos % kPage;
+    unsigned char* page = head + (long long)(pos / kPage) * F::kBytes;
+    reinterpret_cast<uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi] = kw;
+    reinterpret_cast<uint32_t*>(page + F::kVC)[tok * LPR + vhalf<D>(2 * lw + (gi & 1)) / 2] = vword;
+    if (lw % 4 == 0) {
+      reinterpret_cast<__half*>(page + F::kKS)[tok * F::NG + gi] = ks;
+      reinterpret_cast<__half*>(page + F::kKL)[tok * F::NG + gi] = klo;
+      reinterpret_cast<__half*>(page + F::kVS)[vslot<D>(tok, gi)] = vs;
+      reinterpret_cast<__half*>(page + F::kVL)[vslot<D>(tok, gi)] = vlo;
+    }
   }
 }
 
@@ -167,29 +232,43 @@ __device__ __forceinline__ void store_values(T* dst, uint32_t w, __half s, __hal
   const float sf = __half2float(s), lf = __half2float(lo);
   float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = fmaf(sf, (float)((w >> (4 * i)) & 15u), lf);
+  for (int i = 0; i < 8; ++i)  // the code as 2^23 + code without a conversion
+    f[i] = fmaf(sf, __uint_as_float(((w >> (4 * i)) & 15u) | 0x4B000000u) - 8388608.f, lf);
   store8<T>(dst, f);
 }
 
 // out[b][t][h][:] = token start + t
-template <int D, typename T>
+template <int D, typename T, int kRows>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
   using F = Kv4<D>;
   constexpr int LPR = D / 8;
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, row = idx / LPR;
-  const int lw = (int)(idx % LPR), gi = lw / 4, b = blockIdx.y;
-  const int t = (int)(row / (uint32_t)a.H), h = (int)(row - (uint32_t)t * a.H);
-  if (t >= a.n) return;
-  const int pos = a.start + t, tok = pos % kPage;
-  const unsigned char* page = a.pages + (((long long)b * a.H + h) * a.pages_per_head + pos / kPage) * F::kBytes;
-  const uint32_t kw = reinterpret_cast<const uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi];
-  const uint16_t* vrow = reinterpret_cast<const uint16_t*>(page + F::kVC + tok * (D / 2));
-  const uint32_t vw = vrow[vhalf<D>(2 * lw)] | ((uint32_t)vrow[vhalf<D>(2 * lw + 1)] << 16);
-  const long long at = (((long long)b * a.n + t) * a.H + h) * D + lw * 8;
-  store_values<T>(static_cast<T*>(a.k) + at, kw, reinterpret_cast<const __half*>(page + F::kKS)[tok * F::NG + gi],
-                  reinterpret_cast<const __half*>(page + F::kKL)[tok * F::NG + gi]);
-  store_values<T>(static_cast<T*>(a.v) + at, vw, reinterpret_cast<const __half*>(page + F::kVS)[vslot<D>(tok, gi)],
-                  reinterpret_cast<const __half*>(page + F::kVL)[vslot<D>(tok, gi)]);
+  const Place<D> pl = place<D, kRows>(a.H);
+  if (!pl.on) return;
+  const int lw = pl.lw, gi = lw / 4, b = blockIdx.z;
+  const unsigned char* head = a.pages + ((long long)b * a.H + pl.h) * a.pages_per_head * F::kBytes;
+  uint32_t kw[kRows], vw[kRows];
+  __half ks[kRows], kl[kRows], vs[kRows], vl[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    if (pl.t0 + i >= a.n) break;
+    const uint32_t pos = (uint32_t)(a.start + pl.t0 + i), tok = pos % kPage;
+    const unsigned char* page = head + (long long)(pos / kPage) * F::kBytes;
+    kw[i] = reinterpret_cast<const uint32_t*>(page)[tok * LPR + (lw % 4) * F::NG + gi];
+    const uint16_t* vrow = reinterpret_cast<const uint16_t*>(page + F::kVC + tok * (D / 2));
+    vw[i] = vrow[vhalf<D>(2 * lw)] | ((uint32_t)vrow[vhalf<D>(2 * lw + 1)] << 16);
+    ks[i] = reinterpret_cast<const __half*>(page + F::kKS)[tok * F::NG + gi];
+    kl[i] = reinterpret_cast<const __half*>(page + F::kKL)[tok * F::NG + gi];
+    vs[i] = reinterpret_cast<const __half*>(page + F::kVS)[vslot<D>(tok, gi)];
+    vl[i] = reinterpret_cast<const __half*>(page + F::kVL)[vslot<D>(tok, gi)];
+  }
+  const long long step = (long long)a.H * D;
+  long long at = ((long long)b * a.n + pl.t0) * step + pl.h * D + lw * 8;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i, at += step) {
+    if (pl.t0 + i >= a.n) break;
+    store_values<T>(static_cast<T*>(a.k) + at, kw[i], ks[i], kl[i]);
+    store_values<T>(static_cast<T*>(a.v) + at, vw[i], vs[i], vl[i]);
+  }
 }
 
 // --------------------------------------------------------------- attention
@@ -672,11 +751,12 @@ void check_rows(const void* p, int elem, long long sb, long long st, long long s
     throw std::runtime_error(std::string(what) + ": rows must be 16-byte aligned");
 }
 
-// 256 threads a block, D / 8 a row; x: rows of one sequence, y: sequences
-dim3 row_grid(int B, int tokens, int H, int D, const char* what) {
-  const long long threads = (long long)tokens * H * (D / 8);
-  if (threads > 0x7fffff00ll || B > 65535) throw std::runtime_error(std::string(what) + ": too many rows");
-  return dim3((unsigned)((threads + 255) / 256), (unsigned)B);
+// The grid of place<D, rows>: x over heads, y over runs of tokens, z over sequences
+dim3 row_grid(int B, int tokens, int H, int D, int rows, const char* what) {
+  const int span = H * (D / 8), per_block = span < 256 ? 256 / span : 1;
+  const long long y = ((long long)tokens + per_block * rows - 1) / (per_block * rows);
+  if (H > (1 << 24) || y > 65535 || B > 65535) throw std::runtime_error(std::string(what) + ": too many rows");
+  return dim3((unsigned)((span + 255) / 256), (unsigned)y, (unsigned)B);
 }
 
 }  // namespace
@@ -697,9 +777,14 @@ void kv4_append(const Kv4Append& p, int dtype, int D, cudaStream_t s) {
   check_rows(p.v, elem, p.v_stride_b, p.v_stride_t, p.v_stride_h, "kv4 append");
   Kv4Append a = p;
   a.status = device_status_ptr();
-  const dim3 grid = row_grid(p.B, p.T, p.H, D, "kv4 append");
-  UHFS_KV4_TYPES(dtype, if (D == 64) kv4_append_kernel<64, T><<<grid, 256, 0, s>>>(a);
-                 else kv4_append_kernel<128, T><<<grid, 256, 0, s>>>(a));
+  for (long long x : {p.k_stride_t, p.k_stride_h, p.v_stride_t, p.v_stride_h})
+    if (x < 0 || x > 0x7fffffffll) throw std::runtime_error("kv4 append: strides of tokens and heads must fit 32 bits");
+  UHFS_KV4_TYPES(dtype, {
+    constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
+    const dim3 grid = row_grid(p.B, p.T, p.H, D, kRows, "kv4 append");
+    if (D == 64) kv4_append_kernel<64, T, kRows><<<grid, 256, 0, s>>>(a);
+    else kv4_append_kernel<128, T, kRows><<<grid, 256, 0, s>>>(a);
+  });
   note_launch();
   UHFS_CUDA_CHECK(cudaGetLastError());
 }
@@ -711,9 +796,10 @@ void kv4_read(const Kv4Read& a, int dtype, int D, cudaStream_t s) {
     throw std::runtime_error("kv4 read: tokens outside the cache");
   check_rows(a.k, 4, 0, 0, 0, "kv4 read");
   check_rows(a.v, 4, 0, 0, 0, "kv4 read");
-  const dim3 grid = row_grid(a.B, a.n, a.H, D, "kv4 read");
-  UHFS_KV4_TYPES(dtype, if (D == 64) kv4_read_kernel<64, T><<<grid, 256, 0, s>>>(a);
-                 else kv4_read_kernel<128, T><<<grid, 256, 0, s>>>(a));
+  constexpr int kRows = 4;
+  const dim3 grid = row_grid(a.B, a.n, a.H, D, kRows, "kv4 read");
+  UHFS_KV4_TYPES(dtype, if (D == 64) kv4_read_kernel<64, T, kRows><<<grid, 256, 0, s>>>(a);
+                 else kv4_read_kernel<128, T, kRows><<<grid, 256, 0, s>>>(a));
   note_launch();
   UHFS_CUDA_CHECK(cudaGetLastError());
 }

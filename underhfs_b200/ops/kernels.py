@@ -384,7 +384,7 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     """`t` [B, T, H, D] itself where the cache kernels can read its rows in
     16-byte pieces (D contiguous, strides and start aligned), else a copy."""
     b, n, h, d = t.stride()
-    if d == 1 and (t.data_ptr() | ((b | n | h) * t.element_size())) % 16 == 0:
+    if d == 1 and (t.data_ptr() | ((b | n | h) * t.element_size())) % 16 == 0 and max(n, h) < 1 << 31:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
