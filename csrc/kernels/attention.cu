@@ -526,8 +526,9 @@ void bwd_impl(const AttnBwdParams& p, cudaStream_t s) {
     const char* e = getenv("UHFS_ATTN_BWD");
     return e != nullptr && std::string(e) == "mma_sync";
   }();
-  // a window runs on the tcgen05 kernel only (checked by flash_attn_bwd)
-  if (p.f.window > 0 || (!legacy && flash_attn_bwd_tc_supported(p))) {
+  if (p.f.window > 0) {  // (its layout was checked by flash_attn_bwd)
+    flash_attn_bwd_window(p, s);
+  } else if (!legacy && flash_attn_bwd_tc_supported(p)) {
     flash_attn_bwd_tc_main(p, s);
   } else {
     dim3 grid((p.f.T + 63) / 64, p.f.B * p.f.H);

@@ -43,11 +43,6 @@
 // Registers: 512 threads launch with 128 each; warpgroups 2 and 3 give back
 // down to 64 and the compute warpgroups take 192 (the host checks the launch
 // count).
-// Sliding window with sinks (kWin): key j is seen by query i >= j when
-// i - j < window or j < sinks, so a key block without sinks ends at query block
-// (n0 + 127 + window - 1) / 128 and the rest of the sequence is never loaded.
-// q / k / v and dO are read, and dQ is added, through [B][T][..] maps: rows past T
-// read as zeros and are not written, so ragged sequences never meet.
 // Every wait is bounded.
 #include <cudaTypedefs.h>
 
@@ -62,12 +57,6 @@ namespace uhfs {
 
 CUtensorMap make_tmap_bf16_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
                               uint32_t box_inner, uint32_t box_outer);
-CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
-                              uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
-                              uint32_t box_rows);
-CUtensorMap make_tmap_f32_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
-                             uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
-                             uint32_t box_rows);
 CUtensorMap make_tmap_f32_2d(const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_elems,
                              uint32_t box_inner, uint32_t box_outer);
 
@@ -120,7 +109,6 @@ struct BwdArgs {
   long long F;
   float sl2, scale;
   int causal;
-  int window, sinks;    // kWin only
   const float* lse;     // [B, H, T] log2 domain
   const float* delta;   // [B, H, T]
   float* dq_accum;      // [B, T, H, D] fp32
@@ -144,7 +132,7 @@ struct BwdArgs {
   } while (0)
 #endif
 
-template <int D, bool kWin>
+template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     fa_bwd_tc_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
                      const __grid_constant__ CUtensorMap tm_dq, const BwdArgs a) {
@@ -180,17 +168,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n0 = n_block * BK;
   const int T = a.T;
   const int i_start = a.causal ? n0 / BQ : 0;
-  int i_end = (T + BQ - 1) / BQ;
-  if constexpr (kWin) {
-    if (n0 >= a.sinks) i_end = min(i_end, (n0 + BK - 1 + a.window - 1) / BQ + 1);
-  }
+  const int i_end = (T + BQ - 1) / BQ;
   const int steps = i_end - i_start;
   const int row0 = b * T;
-  // one [128 rows][64 columns] box of a fused or a dO row block
-  auto load_box = [&](uint8_t* dst, const CUtensorMap* tm, uint64_t* bar, int col, int row) {
-    if constexpr (kWin) tma_load_3d(dst, tm, bar, col, row, b);
-    else tma_load_2d(dst, tm, bar, col, row0 + row);
-  };
   constexpr int kProducerWarp = 8, kMmaWarp = 9;
 
   if (warp == kProducerWarp && lane == 0) {
@@ -234,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       mbar_arrive_expect_tx(kv_full, 2 * Cfg::kTile);
       for (int kd = 0; kd < KD; ++kd) {
-        load_box(sK + kd * (BK * 128), &tm_qkv, kv_full, (int)(a.F + h * D + kd * 64), n0);
-        load_box(sV + kd * (BK * 128), &tm_qkv, kv_full, (int)(2 * a.F + h * D + kd * 64), n0);
+        tma_load_2d(sK + kd * (BK * 128), &tm_qkv, kv_full, (int)(a.F + h * D + kd * 64), row0 + n0);
+        tma_load_2d(sV + kd * (BK * 128), &tm_qkv, kv_full, (int)(2 * a.F + h * D + kd * 64), row0 + n0);
       }
     }
     for (int t = 0; t < steps; ++t) {
@@ -253,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t* sDO = sQ + Cfg::kTile;
         mbar_arrive_expect_tx(&qd_full[st], 2 * Cfg::kTile);
         for (int kd = 0; kd < KD; ++kd) {
-          load_box(sQ + kd * (BQ * 128), &tm_qkv, &qd_full[st], (int)(h * D + kd * 64), q0);
-          load_box(sDO + kd * (BQ * 128), &tm_do, &qd_full[st], (int)(h * D + kd * 64), q0);
+          tma_load_2d(sQ + kd * (BQ * 128), &tm_qkv, &qd_full[st], (int)(h * D + kd * 64), row0 + q0);
+          tma_load_2d(sDO + kd * (BQ * 128), &tm_do, &qd_full[st], (int)(h * D + kd * 64), row0 + q0);
         }
         issued |= 1u << st;
         iph = (iph & ~(1u << st)) | (ph << st);
@@ -427,9 +407,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4* dlt4 = reinterpret_cast<const float4*>(sVec + st * (2 * BQ) + BQ + half * 64);
         // causal diagonal block: query column qi is visible for this key when qi >= key - q0
         const int qmin = (!kvalid) ? BQ + 1 : ((a.causal && q0 < n0 + BK) ? key - q0 - half * 64 : 0);
-        // window: query column qi is visible up to key + window - 1 (any for a sink)
-        [[maybe_unused]] const int qmax =
-            (kWin && key >= a.sinks) ? key + a.window - 1 - q0 - half * 64 : BQ;
         uint32_t hp[32], hd[32];
 #pragma unroll
         for (int g = 0; g < 16; ++g) {
@@ -441,9 +418,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int i = g * 4 + e;
             float x = ex2_approx(fmaf(__uint_as_float(sv[i]), a.sl2, -lv[e]));
             if (i < qmin) x = 0.f;
-            if constexpr (kWin) {
-              if (i > qmax) x = 0.f;
-            }
             p[e] = x;
             ds[e] = x * (__uint_as_float(pv[i]) - dv[e]);
           }
@@ -565,8 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         named_barrier_sync(1, kReadout);
         if (leader && ok) {
-          if constexpr (kWin) tma_reduce_add_3d(&tm_dq, box, h * D + c * 32, q0, b);
-          else tma_reduce_add_2d(&tm_dq, box, h * D + c * 32, row0 + q0);
+          tma_reduce_add_2d(&tm_dq, box, h * D + c * 32, row0 + q0);
           bulk_commit_group();
         }
       }
@@ -583,30 +556,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int D, bool kWin>
+template <int D>
 void launch_bwd(const AttnBwdParams& p, cudaStream_t s) {
   using Cfg = BwdCfg<D>;
   static PerDeviceOnce once;
   once([] {
-    UHFS_CUDA_CHECK(cudaFuncSetAttribute(fa_bwd_tc_kernel<D, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+    UHFS_CUDA_CHECK(cudaFuncSetAttribute(fa_bwd_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
     // setmaxnreg redistributes the launch allocation; a different launch count
     // could make the increase wait for registers that never come
     cudaFuncAttributes fa{};
-    UHFS_CUDA_CHECK(cudaFuncGetAttributes(&fa, fa_bwd_tc_kernel<D, kWin>));
+    UHFS_CUDA_CHECK(cudaFuncGetAttributes(&fa, fa_bwd_tc_kernel<D>));
     if (fa.numRegs != kLaunchRegs)
       throw std::runtime_error("fa_bwd_tc_kernel: compiled with " + std::to_string(fa.numRegs) +
                                " registers per thread, the register split needs " + std::to_string(kLaunchRegs));
   });
   const long long F = (long long)p.f.H * D;
-  const uint64_t T = (uint64_t)p.f.T, B = (uint64_t)p.f.B;
-  CUtensorMap tq = kWin ? make_tmap_bf16_3d(p.f.q, (uint64_t)(3 * F), T, B, (uint64_t)(3 * F), T * 3 * F, 64, 128)
-                        : make_tmap_bf16_2d(p.f.q, (uint64_t)(3 * F), B * T, (uint64_t)(3 * F), 64, 128);
-  CUtensorMap td = kWin ? make_tmap_bf16_3d(p.dout, (uint64_t)F, T, B, (uint64_t)p.do_stride_t,
-                                            T * (uint64_t)p.do_stride_t, 64, 128)
-                        : make_tmap_bf16_2d(p.dout, (uint64_t)F, B * T, (uint64_t)p.do_stride_t, 64, 128);
+  CUtensorMap tq = make_tmap_bf16_2d(p.f.q, (uint64_t)(3 * F), (uint64_t)p.f.B * p.f.T, (uint64_t)(3 * F), 64, 128);
+  CUtensorMap td = make_tmap_bf16_2d(p.dout, (uint64_t)F, (uint64_t)p.f.B * p.f.T, (uint64_t)p.do_stride_t, 64, 128);
   // dQ accumulator [B*T, H*D] fp32, reduced into in boxes of 32 columns x 128 rows
-  CUtensorMap tdq = kWin ? make_tmap_f32_3d(p.dq_accum, (uint64_t)F, T, B, (uint64_t)F, T * F, 32, 128)
-                         : make_tmap_f32_2d(p.dq_accum, (uint64_t)F, B * T, (uint64_t)F, 32, 128);
+  CUtensorMap tdq = make_tmap_f32_2d(p.dq_accum, (uint64_t)F, (uint64_t)p.f.B * p.f.T, (uint64_t)F, 32, 128);
   BwdArgs a{};
   a.B = p.f.B;
   a.H = p.f.H;
@@ -615,8 +583,6 @@ void launch_bwd(const AttnBwdParams& p, cudaStream_t s) {
   a.sl2 = p.f.scale * kLog2e;
   a.scale = p.f.scale;
   a.causal = p.f.causal;
-  a.window = p.f.window;
-  a.sinks = p.f.sinks;
   a.lse = p.f.lse;
   a.delta = p.delta;
   a.dq_accum = p.dq_accum;
@@ -630,7 +596,7 @@ void launch_bwd(const AttnBwdParams& p, cudaStream_t s) {
   }
 #endif
   dim3 grid((p.f.T + BK - 1) / BK, p.f.B * p.f.H);
-  fa_bwd_tc_kernel<D, kWin><<<grid, kThreads, Cfg::kSmem, s>>>(tq, td, tdq, a);
+  fa_bwd_tc_kernel<D><<<grid, kThreads, Cfg::kSmem, s>>>(tq, td, tdq, a);
   note_launch();
   UHFS_CUDA_CHECK(cudaGetLastError());
 }
@@ -660,13 +626,8 @@ void set_attn_bwd_trace(unsigned long long* buf) {
 }
 
 void flash_attn_bwd_tc_main(const AttnBwdParams& p, cudaStream_t s) {
-  if (p.f.window > 0) {
-    if (p.f.D == 64) launch_bwd<64, true>(p, s);
-    else launch_bwd<128, true>(p, s);
-    return;
-  }
-  if (p.f.D == 64) launch_bwd<64, false>(p, s);
-  else launch_bwd<128, false>(p, s);
+  if (p.f.D == 64) launch_bwd<64>(p, s);
+  else launch_bwd<128>(p, s);
 }
 
 }  // namespace uhfs

@@ -1,0 +1,654 @@
+// Backward of causal attention with a sliding window and sinks on the tcgen05 tensor core.
+//
+// Key j is seen by query i >= j when i - j < window or j < sinks.  A work item is a block
+// of 128 keys of one (batch, head); it loops over the 128-query blocks that see it: from
+// the diagonal to (n0 + 127 + window - 1) / 128, or to the end for a block with sinks.  With a
+// window an item has few steps (three for a window of 256), so what an item costs besides
+// its steps -- loading K and V, filling the pipeline, storing dK and dV -- is as
+// large as they are.  The kernel is therefore persistent: one CTA per SM walks the items
+// (those with sinks, the longest, first), and an item's K / V load and first product run
+// while the item before is stored.  A CTA per item measured 145 us where this one takes
+// kMeasured64 (16 x 1024 tokens, 12 x 64, window 256).
+//
+// Per step i (S^T etc. are 128 keys x 128 queries):
+//   MMA      S^T = K Q_i^T; dP^T = V dO_i^T; dV += P^T dO_i; dQ_i = dS K; dK += dS^T Q_i
+//   compute  P^T = exp2(S^T * scale * log2e - lse) as soon as S^T is there, stored to TMEM (the
+//            A operand of dV), then dS^T = P^T (dP^T - delta), stored to shared memory.
+//            Warp w holds keys 32 (w % 4).. and queries 64 (w / 4).. of the block; of its two
+//            32-query pieces, one that no key of the warp sees costs nothing, one that
+//            all see no comparisons.
+//   read-out dQ_i from TMEM through shared fp32 boxes with TMA reduce-add
+// so dV runs while dS is computed, and S^T of the next step before this step's dK and dQ.
+//
+// TMEM (512 columns).  D = 64: S^T, dP^T, dV, dK, dQ and P^T side by side.  D = 128: P^T
+// takes S^T's place once both warps of a lane quarter hold S^T, and dQ takes dP^T's; S^T of
+// the next step then waits for dV, and dP^T for the read-out of dQ.  Before, with dQ in S^T's
+// place, P^T in shared memory and one Q / dO stage for both, every product waited for
+// the one before: 14 K cycles a step.
+//
+// q / k / v / dO are read and dQ is added through [B][T][..] maps: rows past T read as
+// zeros and are not written, so ragged sequences never meet.
+// Warps: 0..7 compute, 8 TMA producer, 9 MMA issuer, 12..15 dQ read-out.  512 threads launch
+// with 128 registers; the compute warpgroups take kComputeRegs of the total.
+// Every wait is bounded.
+#include <cudaTypedefs.h>
+
+#include <stdexcept>
+#include <string>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace uhfs {
+
+CUtensorMap make_tmap_bf16_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
+                              uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
+                              uint32_t box_rows);
+CUtensorMap make_tmap_f32_3d(const void* base, uint64_t inner, uint64_t rows, uint64_t batch,
+                             uint64_t row_stride_elems, uint64_t batch_stride_elems, uint32_t box_inner,
+                             uint32_t box_rows);
+
+namespace {
+
+constexpr int BK = 128;  // keys per item
+constexpr int BQ = 128;  // queries per step
+constexpr int kCompute = 256;
+constexpr int kReadout = 128;
+constexpr int kThreads = 512;
+constexpr int kLaunchRegs = 128;
+constexpr int kComputeRegs = 184;
+constexpr int kServiceRegs = 72;
+static_assert(2 * 128 * kComputeRegs + 2 * 128 * kServiceRegs <= kThreads * kLaunchRegs, "register split");
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct WinCfg {
+  static constexpr bool kAlias = D == 128;   // P^T in S^T's columns, dQ in dP^T's
+  static constexpr int kTile = 128 * D * 2;  // one [128][D] bf16 tile (D / 64 swizzled sub-tiles)
+  static constexpr int kKV = kAlias ? 1 : 2;  // K / V buffers
+  static constexpr int kNQ = 2, kNDO = kAlias ? 1 : 2;  // Q (with lse) and dO (with delta) stages
+  static constexpr int kDST = BK * BQ * 2;
+  static constexpr int kBox = 128 * 32 * 4;  // fp32 dQ box: 128 rows x 32 columns
+  static constexpr int kVec = (kNQ + kNDO) * BQ * 4;
+  static constexpr int kBars = 2 * kKV + 2 * kNQ + 2 * kNDO + 10;
+  static constexpr int kSmem =
+      1024 + kKV * 2 * kTile + (kNQ + kNDO) * kTile + kDST + 2 * kBox + kVec + kBars * 8 + 16;
+  static_assert(kSmem <= 227 * 1024, "attention backward shared memory");
+  static constexpr uint32_t kST = 0, kDPT = 128, kDV = 256, kDK = 256 + D;
+  static constexpr uint32_t kDQ = kAlias ? kDPT : 384, kPT = kAlias ? kST : 448;
+};
+
+struct WinArgs {
+  int B, H, T, BH;
+  long long F;
+  float sl2, scale;
+  int window, sinks;
+  const float* lse;    // [B, H, T] log2 domain
+  const float* delta;  // [B, H, T]
+  __nv_bfloat16* dqkv;  // [B*T, 3F]
+  DeviceStatus* status;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    fa_bwd_window_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
+                         const __grid_constant__ CUtensorMap tm_dq, const WinArgs a) {
+  using Cfg = WinCfg<D>;
+  constexpr int KD = D / 64;
+  constexpr uint32_t KV = Cfg::kKV, NQ = Cfg::kNQ, ND = Cfg::kNDO;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_align1024(smem_raw);
+  uint8_t* sKV = smem;                          // [KV][K | V]
+  uint8_t* sQ = sKV + KV * 2 * Cfg::kTile;      // [NQ]
+  uint8_t* sDO = sQ + NQ * Cfg::kTile;          // [ND]
+  uint8_t* sDST = sDO + ND * Cfg::kTile;        // dS^T
+  uint8_t* sBox = sDST + Cfg::kDST;             // [2]
+  float* sLse = reinterpret_cast<float*>(sBox + 2 * Cfg::kBox);  // [NQ][128]
+  float* sDelta = sLse + NQ * BQ;                                // [ND][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sDelta + ND * BQ);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = kv_full + KV;   // an item's products are done with K / V
+  uint64_t* q_full = kv_empty + KV;
+  uint64_t* q_empty = q_full + NQ;     // dK of the step is done
+  uint64_t* do_full = q_empty + NQ;
+  uint64_t* do_empty = do_full + ND;   // dV of the step is done
+  uint64_t* s_full = do_empty + ND;
+  uint64_t* dp_full = s_full + 1;
+  uint64_t* p_full = s_full + 2;       // P^T stored, S^T read
+  uint64_t* ds_full = s_full + 3;      // dS^T stored, dP^T read
+  uint64_t* dv_done = s_full + 4;      // dV of the step is done: P^T may be overwritten
+  uint64_t* ds_free = s_full + 5;      // dQ and dK of the step are done: dS^T may be overwritten
+  uint64_t* dq_full = s_full + 6;
+  uint64_t* dq_free = s_full + 7;      // dQ of the step read out
+  uint64_t* dkv_free = s_full + 8;     // an item's dK / dV read out
+  uint64_t* done = s_full + 9;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 10);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int T = a.T;
+  const int n_blocks = (T + BK - 1) / BK, n_qblocks = (T + BQ - 1) / BQ;
+  const int n_sink = min(n_blocks, (a.sinks + BK - 1) / BK);  // key blocks with sinks
+  const int n_items = n_blocks * a.BH;
+  struct Item {
+    int bh, b, h, n0, i_start, steps;
+  };
+  // items with sinks first; the others head by head, so that CTAs share a head's Q and dO in L2
+  auto decode = [&](int it) {
+    Item w;
+    int n_block;
+    if (it < n_sink * a.BH) {
+      w.bh = it % a.BH;
+      n_block = it / a.BH;
+    } else {
+      const int r = it - n_sink * a.BH, rest = n_blocks - n_sink;
+      w.bh = r / rest;
+      n_block = n_sink + r % rest;
+    }
+    w.b = w.bh / a.H;
+    w.h = w.bh % a.H;
+    w.n0 = n_block * BK;
+    w.i_start = n_block;  // BQ == BK
+    const int end = w.n0 < a.sinks ? n_qblocks : min(n_qblocks, (w.n0 + BK - 1 + a.window - 1) / BQ + 1);
+    w.steps = end - w.i_start;
+    return w;
+  };
+  static_assert(BQ == BK, "the diagonal block of key block n is query block n");
+  constexpr int kProducerWarp = 8, kMmaWarp = 9;
+
+  if (warp == kProducerWarp && lane == 0) {
+    tma_prefetch_desc(&tm_qkv);
+    tma_prefetch_desc(&tm_do);
+    tma_prefetch_desc(&tm_dq);
+    for (uint32_t i = 0; i < KV; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (uint32_t i = 0; i < NQ; ++i) {
+      mbar_init(&q_full[i], 2);  // TMA bytes + the producer's lse stores
+      mbar_init(&q_empty[i], 1);
+    }
+    for (uint32_t i = 0; i < ND; ++i) {
+      mbar_init(&do_full[i], 2);
+      mbar_init(&do_empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(dp_full, 1);
+    mbar_init(p_full, kCompute);
+    mbar_init(ds_full, kCompute);
+    mbar_init(dv_done, 1);
+    mbar_init(ds_free, 1);
+    mbar_init(dq_full, 1);
+    mbar_init(dq_free, kReadout);
+    mbar_init(dkv_free, kCompute);
+    mbar_init(done, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    uint32_t g = 0, k = 0;  // steps and items of this CTA so far
+    bool ok = true;
+    // waits in lane 0; the same answer in every lane
+    auto wait = [&](uint64_t* bar, uint32_t phase, int where) {
+      int good = 1;
+      if (lane == 0) good = mbar_wait_bounded(bar, phase, a.status, kErrWaitTimeoutEmpty, where);
+      return __shfl_sync(0xffffffffu, good, 0) != 0;
+    };
+    uint32_t gq = 0, gd = 0;  // Q and dO tiles issued
+    auto load_q = [&](const Item& w, int t) {
+      const uint32_t st = gq % NQ;
+      if (!wait(&q_empty[st], ((gq / NQ) & 1u) ^ 1u, 400)) return false;
+      const int q0 = (w.i_start + t) * BQ;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&q_full[st], Cfg::kTile);
+        for (int kd = 0; kd < KD; ++kd)
+          tma_load_3d(sQ + st * Cfg::kTile + kd * (BQ * 128), &tm_qkv, &q_full[st], w.h * D + kd * 64, q0, w.b);
+      }
+      float v[BQ / 32];
+#pragma unroll
+      for (int i = 0; i < BQ / 32; ++i) {
+        const int qq = q0 + i * 32 + lane;
+        v[i] = qq < T ? __ldg(a.lse + (long long)w.bh * T + qq) : INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < BQ / 32; ++i) sLse[st * BQ + i * 32 + lane] = v[i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[st]);
+      ++gq;
+      return true;
+    };
+    auto load_do = [&](const Item& w, int t) {
+      const uint32_t st = gd % ND;
+      if (!wait(&do_empty[st], ((gd / ND) & 1u) ^ 1u, 401)) return false;
+      const int q0 = (w.i_start + t) * BQ;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&do_full[st], Cfg::kTile);
+        for (int kd = 0; kd < KD; ++kd)
+          tma_load_3d(sDO + st * Cfg::kTile + kd * (BQ * 128), &tm_do, &do_full[st], w.h * D + kd * 64, q0, w.b);
+      }
+      float v[BQ / 32];
+#pragma unroll
+      for (int i = 0; i < BQ / 32; ++i) {
+        const int qq = q0 + i * 32 + lane;
+        v[i] = qq < T ? __ldg(a.delta + (long long)w.bh * T + qq) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < BQ / 32; ++i) sDelta[st * BQ + i * 32 + lane] = v[i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&do_full[st]);
+      ++gd;
+      return true;
+    };
+    for (int it = blockIdx.x; it < n_items && ok; it += gridDim.x, ++k) {
+      const Item w = decode(it);
+      const uint32_t kb = k % KV;
+      // Q before K and V: with one K / V buffer those wait for the item before
+      if (!load_q(w, 0) || !wait(&kv_empty[kb], ((k / KV) & 1u) ^ 1u, 402)) {
+        ok = false;
+        break;
+      }
+      if (lane == 0) {
+        uint8_t* sK = sKV + kb * 2 * Cfg::kTile;
+        mbar_arrive_expect_tx(&kv_full[kb], 2 * Cfg::kTile);
+        for (int kd = 0; kd < KD; ++kd) {
+          tma_load_3d(sK + kd * (BK * 128), &tm_qkv, &kv_full[kb], (int)a.F + w.h * D + kd * 64, w.n0, w.b);
+          tma_load_3d(sK + Cfg::kTile + kd * (BK * 128), &tm_qkv, &kv_full[kb], (int)(2 * a.F) + w.h * D + kd * 64,
+                      w.n0, w.b);
+        }
+      }
+      for (int t = 0; t < w.steps && ok; ++t, ++g)
+        if (!load_do(w, t) || (t + 1 < w.steps && !load_q(w, t + 1))) ok = false;
+    }
+    // every issued copy lands before the CTA exits
+    if (lane == 0) {
+      for (uint32_t i = k > KV ? k - KV : 0; i < k; ++i)
+        mbar_wait_bounded(&kv_full[i % KV], (i / KV) & 1u, a.status, kErrWaitTimeoutFull, 403);
+      for (uint32_t i = gq > NQ ? gq - NQ : 0; i < gq; ++i)
+        mbar_wait_bounded(&q_full[i % NQ], (i / NQ) & 1u, a.status, kErrWaitTimeoutFull, 404);
+      for (uint32_t i = gd > ND ? gd - ND : 0; i < gd; ++i)
+        mbar_wait_bounded(&do_full[i % ND], (i / ND) & 1u, a.status, kErrWaitTimeoutFull, 405);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one_sync()) {
+      constexpr uint32_t id_s = make_idesc(1, 0, 0, BK, BQ);  // K / V K-major, Q / dO K-major
+      constexpr uint32_t id_kv = make_idesc(1, 0, 1, BK, D);  // P^T / dS^T K-major, dO / Q MN-major
+      constexpr uint32_t id_q = make_idesc(1, 1, 1, BQ, D);   // dS MN-major, K MN-major
+      const uint64_t kmaj = make_smem_desc(0, 16, 1024, kSwizzle128B);
+      const uint64_t mnmaj = make_smem_desc(0, 128 * 128, 1024, kSwizzle128B);
+      const uint32_t kv16 = smem_u32(sKV) >> 4, q16 = smem_u32(sQ) >> 4, do16 = smem_u32(sDO) >> 4,
+                     ds16 = smem_u32(sDST) >> 4;
+      constexpr uint32_t tile16 = Cfg::kTile >> 4;
+      uint32_t g = 0, k = 0;  // steps and items before the current ones
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t phase, int where) {
+        return mbar_wait_bounded(bar, phase & 1u, a.status, kErrWaitTimeoutAccum, where);
+      };
+      for (int it = blockIdx.x; it < n_items && ok; it += gridDim.x, ++k) {
+        const Item w = decode(it);
+        const uint32_t k16 = kv16 + (k % KV) * 2 * tile16, v16 = k16 + tile16;
+        auto issue_s = [&](uint32_t gs) {  // S^T of step gs; its columns are free
+          if (!wait(&q_full[gs % NQ], gs / NQ, 410)) return false;
+          tc_fence_after();
+          const uint32_t b16 = q16 + (gs % NQ) * tile16;
+#pragma unroll 1
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+            tc_mma_f16(tmem + Cfg::kST, kmaj + k16 + off, kmaj + b16 + off, id_s, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(s_full);
+          return true;
+        };
+        auto issue_dp = [&](uint32_t gs) {  // dP^T of step gs; its columns are free
+          if (!wait(&do_full[gs % ND], gs / ND, 411)) return false;
+          tc_fence_after();
+          const uint32_t b16 = do16 + (gs % ND) * tile16;
+#pragma unroll 1
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+            tc_mma_f16(tmem + Cfg::kDPT, kmaj + v16 + off, kmaj + b16 + off, id_s, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(dp_full);
+          return true;
+        };
+        // The item's first products: S^T's columns are free (p_full and, aliased, dv_done of the
+        // last step were waited for below), dP^T's too (ds_full and, aliased, dq_free)
+        if (!wait(&kv_full[k % KV], k / KV, 412) || !issue_s(g) ||
+            (Cfg::kAlias && g > 0 && !wait(dq_free, g - 1, 413)) || !issue_dp(g)) {
+          ok = false;
+          break;
+        }
+        for (int t = 0; t < w.steps; ++t, ++g) {
+          const bool more = t + 1 < w.steps;
+          // dV += P^T dO
+          if (!wait(p_full, g, 414) || (t == 0 && k > 0 && !wait(dkv_free, k - 1, 415))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t d16 = do16 + (g % ND) * tile16, qq16 = q16 + (g % NQ) * tile16;
+#pragma unroll 1
+          for (int kk = 0; kk < BQ / 16; ++kk)
+            tc_mma_f16_ts(tmem + Cfg::kDV, tmem + Cfg::kPT + (uint32_t)(kk * 8), mnmaj + d16 + ((kk * 16 * 128) >> 4),
+                          id_kv, (t > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(dv_done);
+          tc_commit(&do_empty[g % ND]);
+          // S^T of the next step
+          if (Cfg::kAlias && !wait(dv_done, g, 416)) {
+            ok = false;
+            break;
+          }
+          if (more && !issue_s(g + 1)) {
+            ok = false;
+            break;
+          }
+          // dQ = dS K, dK += dS^T Q
+          if (!wait(ds_full, g, 417) || (!Cfg::kAlias && g > 0 && !wait(dq_free, g - 1, 418))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            const uint32_t off = (kk * 16 * 128) >> 4;
+            tc_mma_f16(tmem + Cfg::kDQ, mnmaj + ds16 + off, mnmaj + k16 + off, id_q, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(dq_full);
+          if (!Cfg::kAlias && more && !issue_dp(g + 1)) {
+            ok = false;
+            break;
+          }
+#pragma unroll 1
+          for (int kk = 0; kk < BQ / 16; ++kk) {
+            const uint32_t aoff = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+            tc_mma_f16(tmem + Cfg::kDK, kmaj + ds16 + aoff, mnmaj + qq16 + ((kk * 16 * 128) >> 4), id_kv,
+                       (t > 0 || kk > 0) ? 1u : 0u);
+          }
+          tc_commit(ds_free);
+          tc_commit(&q_empty[g % NQ]);
+          if (!more) tc_commit(&kv_empty[k % KV]);
+          if (Cfg::kAlias && more && (!wait(dq_free, g, 419) || !issue_dp(g + 1))) {
+            ok = false;
+            break;
+          }
+        }
+      }
+      tc_commit(done);
+      mbar_wait_bounded(done, 0, a.status, kErrWaitTimeoutAccum, 420);
+    }
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
+    // ------------------------------------------------------------ compute
+    const int quarter = warp & 3, half = warp >> 2;
+    const int r = quarter * 32 + lane;  // key row
+    const uint32_t lb = tmem + ((uint32_t)(quarter * 32) << 16);
+    uint8_t* dst_row = sDST + half * (128 * 128) + r * 128;
+    uint32_t g = 0, k = 0;
+    // warp-uniform; after a failed wait a warp does no more work and waits no more, but still meets
+    // the named barrier that the other warp of its lanes waits at
+    bool ok = true;
+    for (int it = blockIdx.x; it < n_items; it += gridDim.x, ++k) {
+      const Item w = decode(it);
+      const int key = w.n0 + r, key_lo = w.n0 + quarter * 32;
+      for (int t = 0; t < w.steps; ++t, ++g) {
+        const int qh = (w.i_start + t) * BQ + half * 64;  // first query of this half
+        // queries [qmin, qmax] of the half are visible to this key
+        const int qmin = key < T ? key - qh : 64;
+        const int qmax = key < a.sinks ? 64 : key + a.window - 1 - qh;
+        // per 32-query piece: 0 none visible to the warp's keys, 1 some, 2 all
+        int piece[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int lo = qh + 32 * c, hi = lo + 31;
+          const bool none = key_lo >= T || hi < key_lo || (key_lo >= a.sinks && lo > key_lo + 31 + a.window - 1);
+          const bool all = key_lo + 31 < T && lo >= key_lo + 31 &&
+                           (key_lo + 31 < a.sinks || hi <= key_lo + a.window - 1);
+          piece[c] = none ? 0 : all ? 2 : 1;
+        }
+        // ---- P^T
+        if (ok && (!mbar_wait_warp(&q_full[g % NQ], (g / NQ) & 1u, a.status, kErrWaitTimeoutFull, 430) ||
+                   !mbar_wait_warp(s_full, g & 1u, a.status, kErrWaitTimeoutAccum, 431)))
+          ok = false;
+        uint32_t sv[64];
+        if (ok) {
+          tc_fence_after();
+          tmem_ld_32x32b_x32_async(lb + Cfg::kST + half * 64, sv);
+          tmem_ld_32x32b_x32_async(lb + Cfg::kST + half * 64 + 32, sv + 32);
+          tmem_wait_ld_regs<64>(sv);
+        }
+        if constexpr (Cfg::kAlias) {
+          // P^T overwrites S^T: the other warp of these lanes has its part too
+          tc_fence_before();
+          named_barrier_sync(2 + quarter, 64);
+          tc_fence_after();
+        }
+        if (!ok) continue;
+        const float4* lse4 = reinterpret_cast<const float4*>(sLse + (g % NQ) * BQ + half * 64);
+        uint32_t hp[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (piece[c] == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hp[c * 16 + i] = 0u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sv[c * 32 + i] = 0u;
+            continue;
+          }
+#pragma unroll
+          for (int q4 = 0; q4 < 8; ++q4) {
+            const float4 l = lse4[c * 8 + q4];
+            const float lv[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = c * 32 + q4 * 4 + e;
+              sv[i] = __float_as_uint(ex2_approx(fmaf(__uint_as_float(sv[i]), a.sl2, -lv[e])));
+            }
+          }
+          if (piece[c] == 1) {
+#pragma unroll
+            for (int i = c * 32; i < c * 32 + 32; ++i)
+              if (i < qmin || i > qmax) sv[i] = 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            hp[c * 16 + i] =
+                pack_bf16x2(__uint_as_float(sv[c * 32 + 2 * i]), __uint_as_float(sv[c * 32 + 2 * i + 1]));
+        }
+        // P^T of the step before has been read (aliased: S^T was issued after that)
+        if (!Cfg::kAlias && g > 0 && !mbar_wait_warp(dv_done, (g - 1) & 1u, a.status, kErrWaitTimeoutAccum, 432)) {
+          ok = false;
+          continue;
+        }
+        tmem_st_32x32b_x32(lb + Cfg::kPT + half * 32, hp);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(p_full);
+        // ---- dS^T
+        if (!mbar_wait_warp(&do_full[g % ND], (g / ND) & 1u, a.status, kErrWaitTimeoutFull, 433) ||
+            !mbar_wait_warp(dp_full, g & 1u, a.status, kErrWaitTimeoutAccum, 434)) {
+          ok = false;
+          continue;
+        }
+        tc_fence_after();
+        uint32_t pv[64];
+        tmem_ld_32x32b_x32_async(lb + Cfg::kDPT + half * 64, pv);
+        tmem_ld_32x32b_x32_async(lb + Cfg::kDPT + half * 64 + 32, pv + 32);
+        tmem_wait_ld_regs<64>(pv);
+        const float4* dlt4 = reinterpret_cast<const float4*>(sDelta + (g % ND) * BQ + half * 64);
+        uint32_t hd[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (piece[c] == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) hd[c * 16 + i] = 0u;
+            continue;
+          }
+#pragma unroll
+          for (int q4 = 0; q4 < 8; ++q4) {
+            const float4 d = dlt4[c * 8 + q4];
+            const int i = c * 32 + q4 * 4;
+            hd[i / 2] = pack_bf16x2(__uint_as_float(sv[i]) * (__uint_as_float(pv[i]) - d.x),
+                                    __uint_as_float(sv[i + 1]) * (__uint_as_float(pv[i + 1]) - d.y));
+            hd[i / 2 + 1] = pack_bf16x2(__uint_as_float(sv[i + 2]) * (__uint_as_float(pv[i + 2]) - d.z),
+                                        __uint_as_float(sv[i + 3]) * (__uint_as_float(pv[i + 3]) - d.w));
+          }
+        }
+        if (g > 0 && !mbar_wait_warp(ds_free, (g - 1) & 1u, a.status, kErrWaitTimeoutAccum, 435)) {
+          ok = false;
+          continue;
+        }
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch)
+          *reinterpret_cast<uint4*>(dst_row + ((ch ^ (r & 7)) << 4)) =
+              make_uint4(hd[ch * 4], hd[ch * 4 + 1], hd[ch * 4 + 2], hd[ch * 4 + 3]);
+        tc_fence_before();
+        fence_proxy_async_smem();
+        mbar_arrive(ds_full);
+      }
+      // ---- dK (scaled) and dV of the item: every product is done with the last dK
+      if (ok && !mbar_wait_warp(ds_free, (g - 1) & 1u, a.status, kErrWaitTimeoutAccum, 436)) ok = false;
+      if (!ok) continue;
+      tc_fence_after();
+      __nv_bfloat16* dk = a.dqkv + ((long long)w.b * T + key) * 3 * a.F + a.F + w.h * D + half * (D / 2);
+      __nv_bfloat16* dv = dk + a.F;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t kr[32], vr[32];
+        tmem_ld_32x32b_x32_async(lb + Cfg::kDK + half * (D / 2) + c * 32, kr);
+        tmem_ld_32x32b_x32_async(lb + Cfg::kDV + half * (D / 2) + c * 32, vr);
+        tmem_wait_ld_regs<32>(kr);
+        tmem_wait_ld_regs<32>(vr);
+        if (c == D / 64 - 1) {
+          tc_fence_before();
+          mbar_arrive(dkv_free);  // the next item may accumulate
+        }
+        if (key >= T) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t hk[4], hv[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = q * 8 + e * 2;
+            hk[e] = pack_bf16x2(__uint_as_float(kr[i]) * a.scale, __uint_as_float(kr[i + 1]) * a.scale);
+            hv[e] = pack_bf16x2(__uint_as_float(vr[i]), __uint_as_float(vr[i + 1]));
+          }
+          *reinterpret_cast<uint4*>(dk + c * 32 + q * 8) = make_uint4(hk[0], hk[1], hk[2], hk[3]);
+          *reinterpret_cast<uint4*>(dv + c * 32 + q * 8) = make_uint4(hv[0], hv[1], hv[2], hv[3]);
+        }
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------ dQ read-out
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // query row within the block
+    const uint32_t lb = tmem + ((uint32_t)(quarter * 32) << 16);
+    const bool leader = warp == 12 && lane == 0;  // issues the TMA reductions
+    uint32_t g = 0;
+    int chunk = 0;
+    bool ok = true;  // per warp; the named barriers are met in any case
+    for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+      const Item w = decode(it);
+      for (int t = 0; t < w.steps; ++t, ++g) {
+        if (ok && !mbar_wait_warp(dq_full, g & 1u, a.status, kErrWaitTimeoutAccum, 440)) ok = false;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c, ++chunk) {
+          uint32_t v[32];
+          if (ok) {
+            tc_fence_after();
+            tmem_ld_32x32b_x32_async(lb + Cfg::kDQ + c * 32, v);
+            tmem_wait_ld_regs<32>(v);
+            if (c == D / 32 - 1) {
+              tc_fence_before();
+              mbar_arrive(dq_free);
+            }
+          }
+          uint8_t* box = sBox + (chunk & 1) * Cfg::kBox;
+          if (leader) bulk_wait_group_read1();  // the reduction that last used this box has read it
+          named_barrier_sync(1, kReadout);
+          if (ok) {
+#pragma unroll
+            for (int ch = 0; ch < 8; ++ch)
+              *reinterpret_cast<uint4*>(box + r * 128 + ((ch ^ (r & 7)) << 4)) =
+                  make_uint4(v[ch * 4], v[ch * 4 + 1], v[ch * 4 + 2], v[ch * 4 + 3]);
+            fence_proxy_async_smem();
+          }
+          named_barrier_sync(1, kReadout);
+          if (leader && ok) {
+            tma_reduce_add_3d(&tm_dq, box, w.h * D + c * 32, (w.i_start + t) * BQ, w.b);
+            bulk_commit_group();
+          }
+        }
+      }
+    }
+    if (leader) bulk_wait_group0();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D>
+void launch(const AttnBwdParams& p, cudaStream_t s) {
+  using Cfg = WinCfg<D>;
+  static PerDeviceOnce once;
+  once([] {
+    UHFS_CUDA_CHECK(
+        cudaFuncSetAttribute(fa_bwd_window_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem));
+    // setmaxnreg redistributes the launch allocation; a different launch count
+    // could make the increase wait for registers that never come
+    cudaFuncAttributes fa{};
+    UHFS_CUDA_CHECK(cudaFuncGetAttributes(&fa, fa_bwd_window_kernel<D>));
+    if (fa.numRegs != kLaunchRegs)
+      throw std::runtime_error("fa_bwd_window_kernel: compiled with " + std::to_string(fa.numRegs) +
+                               " registers per thread, the register split needs " + std::to_string(kLaunchRegs));
+  });
+  const uint64_t F = (uint64_t)p.f.H * D, T = (uint64_t)p.f.T, B = (uint64_t)p.f.B;
+  CUtensorMap tq = make_tmap_bf16_3d(p.f.q, 3 * F, T, B, 3 * F, T * 3 * F, 64, 128);
+  CUtensorMap td = make_tmap_bf16_3d(p.dout, F, T, B, (uint64_t)p.do_stride_t, T * (uint64_t)p.do_stride_t, 64, 128);
+  CUtensorMap tdq = make_tmap_f32_3d(p.dq_accum, F, T, B, F, T * F, 32, 128);
+  WinArgs a{};
+  a.B = p.f.B;
+  a.H = p.f.H;
+  a.T = p.f.T;
+  a.BH = p.f.B * p.f.H;
+  a.F = (long long)F;
+  a.sl2 = p.f.scale * kLog2e;
+  a.scale = p.f.scale;
+  a.window = p.f.window;
+  a.sinks = p.f.sinks;
+  a.lse = p.f.lse;
+  a.delta = p.delta;
+  a.dqkv = p.dq;
+  a.status = device_status_ptr();
+  const long long items = (long long)((p.f.T + BK - 1) / BK) * a.BH;
+  int dev = 0, sms = 0;
+  UHFS_CUDA_CHECK(cudaGetDevice(&dev));
+  UHFS_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (items > 0x7fffffffll) throw std::runtime_error("flash attention backward: too many key blocks");
+  fa_bwd_window_kernel<D><<<(int)(items < sms ? items : sms), kThreads, Cfg::kSmem, s>>>(tq, td, tdq, a);
+  note_launch();
+  UHFS_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace
+
+void flash_attn_bwd_window(const AttnBwdParams& p, cudaStream_t s) {
+  if (p.f.D == 64) launch<64>(p, s);
+  else launch<128>(p, s);
+}
+
+}  // namespace uhfs

@@ -125,6 +125,9 @@ void flash_attn_bwd(const AttnBwdParams& p, cudaStream_t s);
 // delta / dQ-zeroing prologue and the dQ conversion around it
 bool flash_attn_bwd_tc_supported(const AttnBwdParams& p);
 void flash_attn_bwd_tc_main(const AttnBwdParams& p, cudaStream_t s);
+// the same with a sliding window (attention_tc_bwd_window.cu), for the layouts that
+// flash_attn_bwd_tc_supported accepts
+void flash_attn_bwd_window(const AttnBwdParams& p, cudaStream_t s);
 
 // ---- key / value cache in 4 bits (kv4.cu): pages [B, Hkv, pages_per_head] of 32
 // tokens (D * 40 bytes each); `lengths` counts the tokens of each sequence
