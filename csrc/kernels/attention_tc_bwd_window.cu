@@ -66,11 +66,11 @@ struct WinCfg {
   static constexpr bool kAlias = D == 128;   // P^T in S^T's columns, dQ in dP^T's
   static constexpr int kTile = 128 * D * 2;  // one [128][D] bf16 tile (D / 64 swizzled sub-tiles)
   static constexpr int kKV = kAlias ? 1 : 2;  // K / V buffers
-  static constexpr int kNQ = 2, kNDO = kAlias ? 1 : 2;  // Q (with lse) and dO (with delta) stages
+  static constexpr int kNQ = kAlias ? 2 : 3, kNDO = kAlias ? 1 : 2;  // Q (with lse) and dO (with delta) stages
   static constexpr int kDST = BK * BQ * 2;
   static constexpr int kBox = 128 * 32 * 4;  // fp32 dQ box: 128 rows x 32 columns
   static constexpr int kVec = (kNQ + kNDO) * BQ * 4;
-  static constexpr int kBars = 2 * kKV + 2 * kNQ + 2 * kNDO + 10;
+  static constexpr int kBars = 2 * kKV + 2 * kNQ + 2 * kNDO + 12;
   static constexpr int kSmem =
       1024 + kKV * 2 * kTile + (kNQ + kNDO) * kTile + kDST + 2 * kBox + kVec + kBars * 8 + 16;
   static_assert(kSmem <= 227 * 1024, "attention backward shared memory");
@@ -85,14 +85,14 @@ struct WinArgs {
   int window, sinks;
   const float* lse;    // [B, H, T] log2 domain
   const float* delta;  // [B, H, T]
-  __nv_bfloat16* dqkv;  // [B*T, 3F]
   DeviceStatus* status;
 };
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     fa_bwd_window_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
-                         const __grid_constant__ CUtensorMap tm_dq, const WinArgs a) {
+                         const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ CUtensorMap tm_dqkv,
+                         const WinArgs a) {
   using Cfg = WinCfg<D>;
   constexpr int KD = D / 64;
   constexpr uint32_t KV = Cfg::kKV, NQ = Cfg::kNQ, ND = Cfg::kNDO;
@@ -121,8 +121,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* dq_full = s_full + 6;
   uint64_t* dq_free = s_full + 7;      // dQ of the step read out
   uint64_t* dkv_free = s_full + 8;     // an item's dK / dV read out
-  uint64_t* done = s_full + 9;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 10);
+  uint64_t* staged = s_full + 9;       // dK / dV is in the dS^T tile
+  uint64_t* stored = s_full + 10;      // the stores have read it
+  uint64_t* done = s_full + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 12);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int T = a.T;
@@ -153,12 +155,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     return w;
   };
   static_assert(BQ == BK, "the diagonal block of key block n is query block n");
-  constexpr int kProducerWarp = 8, kMmaWarp = 9;
+  constexpr int kProducerWarp = 8, kMmaWarp = 9, kProducerWarp2 = 10;
 
   if (warp == kProducerWarp && lane == 0) {
     tma_prefetch_desc(&tm_qkv);
     tma_prefetch_desc(&tm_do);
     tma_prefetch_desc(&tm_dq);
+    tma_prefetch_desc(&tm_dqkv);
     for (uint32_t i = 0; i < KV; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
@@ -180,6 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(dq_full, 1);
     mbar_init(dq_free, kReadout);
     mbar_init(dkv_free, kCompute);
+    mbar_init(staged, kCompute);
+    mbar_init(stored, 1);
     mbar_init(done, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -194,9 +199,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
-  if (warp == kProducerWarp) {
-    // ------------------------------------------------------------ producer
-    uint32_t g = 0, k = 0;  // steps and items of this CTA so far
+  if (warp == kProducerWarp || warp == kProducerWarp2) {
+    // ------------------------------------------------------------ producers: K, V, Q, lse; dO, delta
+    uint32_t k = 0;  // items of this CTA so far
     bool ok = true;
     // waits in lane 0; the same answer in every lane
     auto wait = [&](uint64_t* bar, uint32_t phase, int where) {
@@ -251,6 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (int it = blockIdx.x; it < n_items && ok; it += gridDim.x, ++k) {
       const Item w = decode(it);
+      if (warp == kProducerWarp2) {
+        for (int t = 0; t < w.steps && ok; ++t) ok = load_do(w, t);
+        continue;
+      }
       const uint32_t kb = k % KV;
       // Q before K and V: with one K / V buffer those wait for the item before
       if (!load_q(w, 0) || !wait(&kv_empty[kb], ((k / KV) & 1u) ^ 1u, 402)) {
@@ -266,13 +275,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                       w.n0, w.b);
         }
       }
-      for (int t = 0; t < w.steps && ok; ++t, ++g)
-        if (!load_do(w, t) || (t + 1 < w.steps && !load_q(w, t + 1))) ok = false;
+      for (int t = 1; t < w.steps && ok; ++t) ok = load_q(w, t);
     }
     // every issued copy lands before the CTA exits
     if (lane == 0) {
-      for (uint32_t i = k > KV ? k - KV : 0; i < k; ++i)
-        mbar_wait_bounded(&kv_full[i % KV], (i / KV) & 1u, a.status, kErrWaitTimeoutFull, 403);
+      if (warp == kProducerWarp)
+        for (uint32_t i = k > KV ? k - KV : 0; i < k; ++i)
+          mbar_wait_bounded(&kv_full[i % KV], (i / KV) & 1u, a.status, kErrWaitTimeoutFull, 403);
       for (uint32_t i = gq > NQ ? gq - NQ : 0; i < gq; ++i)
         mbar_wait_bounded(&q_full[i % NQ], (i / NQ) & 1u, a.status, kErrWaitTimeoutFull, 404);
       for (uint32_t i = gd > ND ? gd - ND : 0; i < gd; ++i)
@@ -297,41 +306,55 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int it = blockIdx.x; it < n_items && ok; it += gridDim.x, ++k) {
         const Item w = decode(it);
         const uint32_t k16 = kv16 + (k % KV) * 2 * tile16, v16 = k16 + tile16;
-        auto issue_s = [&](uint32_t gs) {  // S^T of step gs; its columns are free
+        auto issue_s = [&](uint32_t gs, uint32_t key16) {  // S^T of step gs; its columns are free
           if (!wait(&q_full[gs % NQ], gs / NQ, 410)) return false;
           tc_fence_after();
           const uint32_t b16 = q16 + (gs % NQ) * tile16;
 #pragma unroll 1
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-            tc_mma_f16(tmem + Cfg::kST, kmaj + k16 + off, kmaj + b16 + off, id_s, kk > 0 ? 1u : 0u);
+            tc_mma_f16(tmem + Cfg::kST, kmaj + key16 + off, kmaj + b16 + off, id_s, kk > 0 ? 1u : 0u);
           }
           tc_commit(s_full);
           return true;
         };
-        auto issue_dp = [&](uint32_t gs) {  // dP^T of step gs; its columns are free
+        auto issue_dp = [&](uint32_t gs, uint32_t value16) {  // dP^T of step gs; its columns are free
           if (!wait(&do_full[gs % ND], gs / ND, 411)) return false;
           tc_fence_after();
           const uint32_t b16 = do16 + (gs % ND) * tile16;
 #pragma unroll 1
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-            tc_mma_f16(tmem + Cfg::kDPT, kmaj + v16 + off, kmaj + b16 + off, id_s, kk > 0 ? 1u : 0u);
+            tc_mma_f16(tmem + Cfg::kDPT, kmaj + value16 + off, kmaj + b16 + off, id_s, kk > 0 ? 1u : 0u);
           }
           tc_commit(dp_full);
           return true;
         };
-        // The item's first products: S^T's columns are free (p_full and, aliased, dv_done of the
-        // last step were waited for below), dP^T's too (ds_full and, aliased, dq_free)
-        if (!wait(&kv_full[k % KV], k / KV, 412) || !issue_s(g) ||
-            (Cfg::kAlias && g > 0 && !wait(dq_free, g - 1, 413)) || !issue_dp(g)) {
+        // The item's first products, unless the item before issued them.  S^T's columns are free
+        // (p_full and, aliased, dv_done of the last step were waited for below), dP^T's too (ds_full
+        // and, aliased, dq_free)
+        if ((KV == 1 || k == 0) &&
+            (!wait(&kv_full[k % KV], k / KV, 412) || !issue_s(g, k16) ||
+             (Cfg::kAlias && g > 0 && !wait(dq_free, g - 1, 413)) || !issue_dp(g, v16))) {
           ok = false;
           break;
         }
         for (int t = 0; t < w.steps; ++t, ++g) {
-          const bool more = t + 1 < w.steps;
+          // whether, and with which K / V, the step after this one is begun from here
+          const bool more = t + 1 < w.steps, ahead = more || (KV == 2 && it + (int)gridDim.x < n_items);
+          const uint32_t next16 = more ? k16 : kv16 + ((k + 1) % KV) * 2 * tile16;
+          if (!wait(p_full, g, 414)) {
+            ok = false;
+            break;
+          }
+          // S^T of the next step, before dV where P^T has columns of its own
+          if (!Cfg::kAlias && ahead &&
+              ((!more && !wait(&kv_full[(k + 1) % KV], (k + 1) / KV, 421)) || !issue_s(g + 1, next16))) {
+            ok = false;
+            break;
+          }
           // dV += P^T dO
-          if (!wait(p_full, g, 414) || (t == 0 && k > 0 && !wait(dkv_free, k - 1, 415))) {
+          if (t == 0 && k > 0 && !wait(dkv_free, k - 1, 415)) {
             ok = false;
             break;
           }
@@ -343,12 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           id_kv, (t > 0 || kk > 0) ? 1u : 0u);
           tc_commit(dv_done);
           tc_commit(&do_empty[g % ND]);
-          // S^T of the next step
-          if (Cfg::kAlias && !wait(dv_done, g, 416)) {
-            ok = false;
-            break;
-          }
-          if (more && !issue_s(g + 1)) {
+          if (Cfg::kAlias && (!wait(dv_done, g, 416) || (more && !issue_s(g + 1, k16)))) {
             ok = false;
             break;
           }
@@ -364,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_mma_f16(tmem + Cfg::kDQ, mnmaj + ds16 + off, mnmaj + k16 + off, id_q, kk > 0 ? 1u : 0u);
           }
           tc_commit(dq_full);
-          if (!Cfg::kAlias && more && !issue_dp(g + 1)) {
+          if (!Cfg::kAlias && ahead && !issue_dp(g + 1, next16 + tile16)) {
             ok = false;
             break;
           }
@@ -377,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(ds_free);
           tc_commit(&q_empty[g % NQ]);
           if (!more) tc_commit(&kv_empty[k % KV]);
-          if (Cfg::kAlias && more && (!wait(dq_free, g, 419) || !issue_dp(g + 1))) {
+          if (Cfg::kAlias && more && (!wait(dq_free, g, 419) || !issue_dp(g + 1, v16))) {
             ok = false;
             break;
           }
@@ -392,11 +410,82 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;  // key row
     const uint32_t lb = tmem + ((uint32_t)(quarter * 32) << 16);
+    const bool storer = warp == 0 && lane == 0;  // issues the dK / dV stores
     uint8_t* dst_row = sDST + half * (128 * 128) + r * 128;
     uint32_t g = 0, k = 0;
     // warp-uniform; after a failed wait a warp does no more work and waits no more, but still meets
     // the named barrier that the other warp of its lanes waits at
     bool ok = true;
+    uint32_t n_staged = 0, n_read = 0;
+    // the stores so far have read the dS^T tile
+    auto tile_read = [&]() {
+      if (storer) {
+        bulk_wait_group_read0();
+        mbar_arrive(stored);
+      }
+      __syncwarp();
+      return mbar_wait_warp(stored, n_read++ & 1u, a.status, kErrWaitTimeoutAccum, 437);
+    };
+    // dK (scaled) and dV of item w, whose last step was end - 1: every product is done with the
+    // last dK.  They leave through the dS^T tile with TMA stores.
+    auto store_item = [&](const Item& w, uint32_t end) {
+      if (ok && !mbar_wait_warp(ds_free, (end - 1) & 1u, a.status, kErrWaitTimeoutAccum, 436)) ok = false;
+      // 32 columns from `col`, as the 16-byte chunks ch0.. of this key's row
+      auto put = [&](uint32_t col, float scale, uint8_t* row, int ch0) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32_async(lb + col, v);
+        tmem_wait_ld_regs<32>(v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t h4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = q * 8 + e * 2;
+            h4[e] = pack_bf16x2(__uint_as_float(v[i]) * scale, __uint_as_float(v[i + 1]) * scale);
+          }
+          *reinterpret_cast<uint4*>(row + (((ch0 + q) ^ (r & 7)) << 4)) = make_uint4(h4[0], h4[1], h4[2], h4[3]);
+        }
+      };
+      uint8_t* row0 = sDST + r * 128;
+      // the tile holds dK and dV for D = 64, one of them at a time for D = 128
+#pragma unroll 1
+      for (int i = 0; i < KD && ok; ++i) {
+        if (i == 1 && !tile_read()) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if constexpr (D == 64) {
+          put(Cfg::kDK + half * 32, a.scale, row0, 4 * half);
+          put(Cfg::kDV + half * 32, 1.f, row0 + 128 * 128, 4 * half);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c)
+            put((i == 0 ? Cfg::kDK : Cfg::kDV) + half * 64 + c * 32, i == 0 ? a.scale : 1.f,
+                row0 + half * (128 * 128), 4 * c);
+        }
+        if (i == KD - 1) {
+          tc_fence_before();
+          mbar_arrive(dkv_free);  // the next item may accumulate
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(staged);
+        if (warp == 0) {
+          ok = mbar_wait_warp(staged, n_staged & 1u, a.status, kErrWaitTimeoutAccum, 438);
+          if (storer && ok) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int part = D == 64 ? c : i, col = D == 64 ? 0 : c * 64;  // dK or dV, first column
+              tma_store_3d(&tm_dqkv, sDST + c * (128 * 128), (int)((part + 1) * a.F) + w.h * D + col, w.n0, w.b);
+            }
+            bulk_commit_group();
+          }
+          __syncwarp();
+        }
+        ++n_staged;
+      }
+    };
+    Item last{};
     for (int it = blockIdx.x; it < n_items; it += gridDim.x, ++k) {
       const Item w = decode(it);
       const int key = w.n0 + r, key_lo = w.n0 + quarter * 32;
@@ -455,9 +544,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (piece[c] == 1) {
+            // bits [qmin, qmax] of the piece
+            const int b0 = max(qmin - c * 32, 0), b1 = min(qmax - c * 32, 31);
+            const uint32_t vis = b0 > b1 ? 0u : (0xffffffffu >> (31 - (b1 - b0))) << b0;
 #pragma unroll
-            for (int i = c * 32; i < c * 32 + 32; ++i)
-              if (i < qmin || i > qmax) sv[i] = 0u;
+            for (int i = 0; i < 32; ++i) sv[c * 32 + i] = (vis >> i) & 1u ? sv[c * 32 + i] : 0u;
           }
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -473,6 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(p_full);
+        // the item before is stored here where its successor's first S^T did not have to wait for it
+        if (KV == 2 && t == 0 && k > 0) store_item(last, g);
         // ---- dS^T
         if (!mbar_wait_warp(&do_full[g % ND], (g / ND) & 1u, a.status, kErrWaitTimeoutFull, 433) ||
             !mbar_wait_warp(dp_full, g & 1u, a.status, kErrWaitTimeoutAccum, 434)) {
@@ -507,6 +600,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           continue;
         }
+        if (t == 0 && k > 0 && !tile_read()) {  // the stores of the item before
+          ok = false;
+          continue;
+        }
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch)
           *reinterpret_cast<uint4*>(dst_row + ((ch ^ (r & 7)) << 4)) =
@@ -515,38 +612,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_proxy_async_smem();
         mbar_arrive(ds_full);
       }
-      // ---- dK (scaled) and dV of the item: every product is done with the last dK
-      if (ok && !mbar_wait_warp(ds_free, (g - 1) & 1u, a.status, kErrWaitTimeoutAccum, 436)) ok = false;
-      if (!ok) continue;
-      tc_fence_after();
-      __nv_bfloat16* dk = a.dqkv + ((long long)w.b * T + key) * 3 * a.F + a.F + w.h * D + half * (D / 2);
-      __nv_bfloat16* dv = dk + a.F;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t kr[32], vr[32];
-        tmem_ld_32x32b_x32_async(lb + Cfg::kDK + half * (D / 2) + c * 32, kr);
-        tmem_ld_32x32b_x32_async(lb + Cfg::kDV + half * (D / 2) + c * 32, vr);
-        tmem_wait_ld_regs<32>(kr);
-        tmem_wait_ld_regs<32>(vr);
-        if (c == D / 64 - 1) {
-          tc_fence_before();
-          mbar_arrive(dkv_free);  // the next item may accumulate
-        }
-        if (key >= T) continue;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t hk[4], hv[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = q * 8 + e * 2;
-            hk[e] = pack_bf16x2(__uint_as_float(kr[i]) * a.scale, __uint_as_float(kr[i + 1]) * a.scale);
-            hv[e] = pack_bf16x2(__uint_as_float(vr[i]), __uint_as_float(vr[i + 1]));
-          }
-          *reinterpret_cast<uint4*>(dk + c * 32 + q * 8) = make_uint4(hk[0], hk[1], hk[2], hk[3]);
-          *reinterpret_cast<uint4*>(dv + c * 32 + q * 8) = make_uint4(hv[0], hv[1], hv[2], hv[3]);
-        }
-      }
+      if (KV == 1) store_item(w, g);
+      last = w;
     }
+    if (KV == 2) store_item(last, g);  // every CTA has an item
+    if (storer) bulk_wait_group0();
   } else if (warp >= 12) {
     // ------------------------------------------------------------ dQ read-out
     const int quarter = warp & 3;
@@ -620,6 +690,7 @@ void launch(const AttnBwdParams& p, cudaStream_t s) {
   CUtensorMap tq = make_tmap_bf16_3d(p.f.q, 3 * F, T, B, 3 * F, T * 3 * F, 64, 128);
   CUtensorMap td = make_tmap_bf16_3d(p.dout, F, T, B, (uint64_t)p.do_stride_t, T * (uint64_t)p.do_stride_t, 64, 128);
   CUtensorMap tdq = make_tmap_f32_3d(p.dq_accum, F, T, B, F, T * F, 32, 128);
+  CUtensorMap tdqkv = make_tmap_bf16_3d(p.dq, 3 * F, T, B, 3 * F, T * 3 * F, 64, 128);
   WinArgs a{};
   a.B = p.f.B;
   a.H = p.f.H;
@@ -632,14 +703,13 @@ void launch(const AttnBwdParams& p, cudaStream_t s) {
   a.sinks = p.f.sinks;
   a.lse = p.f.lse;
   a.delta = p.delta;
-  a.dqkv = p.dq;
   a.status = device_status_ptr();
   const long long items = (long long)((p.f.T + BK - 1) / BK) * a.BH;
   int dev = 0, sms = 0;
   UHFS_CUDA_CHECK(cudaGetDevice(&dev));
   UHFS_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   if (items > 0x7fffffffll) throw std::runtime_error("flash attention backward: too many key blocks");
-  fa_bwd_window_kernel<D><<<(int)(items < sms ? items : sms), kThreads, Cfg::kSmem, s>>>(tq, td, tdq, a);
+  fa_bwd_window_kernel<D><<<(int)(items < sms ? items : sms), kThreads, Cfg::kSmem, s>>>(tq, td, tdq, tdqkv, a);
   note_launch();
   UHFS_CUDA_CHECK(cudaGetLastError());
 }
