@@ -235,13 +235,15 @@ __global__ void __launch_bounds__(256) fa_fwd_kernel(const AttnParams p) {
 
 // --------------------------------------------------------- backward helpers
 // delta[b,h,t] = sum_d dO * O ; dq_accum zeroed.  Eight elements per thread
-// (16-byte loads), D/8 threads per (b, t, h) row.
+// (16-byte loads), D/8 threads per (b, t, h) row.  The windowed backward's work counter, behind
+// delta, is zeroed too.
 template <int D>
 __global__ void __launch_bounds__(256) fa_bwd_prep_kernel(const AttnBwdParams p) {
   constexpr int TPR = D / 8;  // threads per row
   const long long rows = (long long)p.f.B * p.f.T * p.f.H;
   const int sub = threadIdx.x % TPR;
   const long long stride = (long long)gridDim.x * (blockDim.x / TPR);
+  if (p.f.window > 0 && blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int*>(p.delta + rows) = 0;
   for (long long r = blockIdx.x * (long long)(blockDim.x / TPR) + threadIdx.x / TPR; r < rows; r += stride) {
     const int h = r % p.f.H;
     const int tt = (r / p.f.H) % p.f.T;

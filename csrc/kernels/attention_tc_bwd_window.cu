@@ -5,10 +5,19 @@
 // the diagonal to (n0 + 127 + window - 1) / 128, or to the end for a block with sinks.  With a
 // window an item has few steps (three for a window of 256), so what an item costs besides
 // its steps -- loading K and V, filling the pipeline, storing dK and dV -- is as
-// large as they are.  The kernel is therefore persistent: one CTA per SM walks the items
-// (those with sinks, the longest, first), and an item's K / V load and first product run
-// while the item before is stored.  A CTA per item measured 145 us where this one takes
-// kMeasured64 (16 x 1024 tokens, 12 x 64, window 256).
+// large as they are.  The kernel is therefore persistent, one CTA per SM, and with D = 64 an
+// item's loads and first products run while the item before is finished and stored (D = 128 has
+// shared memory for one K / V pair only).  Items are handed out from a counter, those with sinks,
+// the longest, first: dealt out in turn, 16 heads of 2 x 4096 tokens gave CTAs 45 to 84 steps
+// of a mean of 59, and the kernel 540 K cycles instead of 423 K.
+//
+// Measured with the sums before and the conversion after it (28 us of 16 x 1024), against
+// 175 and 484 us of a CTA per item with every product waiting for the one before:
+//   16 x 1024 tokens, 12 x 64, window 256, 4 sinks     166 us, 6.3 K cycles a step
+//   2 x 4096 tokens, 16 x 128, window 1024, 4 sinks    284 us, 6.5 K cycles a step
+// A step's five products are 1.3 K (D = 64) and 2.6 K cycles of the tensor core; what bounds
+// it is the chain S -> P -> dS -> dQ of a step, of which two steps do not fit in TMEM, and
+// the shared memory that the products, dS^T and the dQ boxes share.
 //
 // Per step i (S^T etc. are 128 keys x 128 queries):
 //   MMA      S^T = K Q_i^T; dP^T = V dO_i^T; dV += P^T dO_i; dQ_i = dS K; dK += dS^T Q_i
@@ -22,13 +31,12 @@
 //
 // TMEM (512 columns).  D = 64: S^T, dP^T, dV, dK, dQ and P^T side by side.  D = 128: P^T
 // takes S^T's place once both warps of a lane quarter hold S^T, and dQ takes dP^T's; S^T of
-// the next step then waits for dV, and dP^T for the read-out of dQ.  Before, with dQ in S^T's
-// place, P^T in shared memory and one Q / dO stage for both, every product waited for
-// the one before: 14 K cycles a step.
+// the next step then waits for dV, and dP^T for the read-out of dQ.
 //
 // q / k / v / dO are read and dQ is added through [B][T][..] maps: rows past T read as
 // zeros and are not written, so ragged sequences never meet.
-// Warps: 0..7 compute, 8 TMA producer, 9 MMA issuer, 12..15 dQ read-out.  512 threads launch
+// Warps: 0..7 compute, 8 items and K / V / Q / lse loads, 9 MMA issuer, 10 dO / delta loads,
+// 12..15 dQ read-out.  512 threads launch
 // with 128 registers; the compute warpgroups take kComputeRegs of the total.
 // Every wait is bounded.
 #include <cudaTypedefs.h>
@@ -67,13 +75,15 @@ struct WinCfg {
   static constexpr int kTile = 128 * D * 2;  // one [128][D] bf16 tile (D / 64 swizzled sub-tiles)
   static constexpr int kKV = kAlias ? 1 : 2;  // K / V buffers
   static constexpr int kNQ = kAlias ? 2 : 3, kNDO = kAlias ? 1 : 2;  // Q (with lse) and dO (with delta) stages
+  static constexpr int kRing = 4;  // items handed out ahead
   static constexpr int kDST = BK * BQ * 2;
   static constexpr int kBox = 128 * 32 * 4;  // fp32 dQ box: 128 rows x 32 columns
   static constexpr int kVec = (kNQ + kNDO) * BQ * 4;
-  static constexpr int kBars = 2 * kKV + 2 * kNQ + 2 * kNDO + 12;
+  static constexpr int kBars = 2 * kKV + 2 * kNQ + 2 * kNDO + 12 + 2 * kRing;
   static constexpr int kSmem =
-      1024 + kKV * 2 * kTile + (kNQ + kNDO) * kTile + kDST + 2 * kBox + kVec + kBars * 8 + 16;
+      1024 + kKV * 2 * kTile + (kNQ + kNDO) * kTile + kDST + 2 * kBox + kVec + kBars * 8 + (kRing + 4) * 16 + 16;
   static_assert(kSmem <= 227 * 1024, "attention backward shared memory");
+  static_assert(kBars % 2 == 0, "the items behind the barriers are 16-byte aligned");
   static constexpr uint32_t kST = 0, kDPT = 128, kDV = 256, kDK = 256 + D;
   static constexpr uint32_t kDQ = kAlias ? kDPT : 384, kPT = kAlias ? kST : 448;
 };
@@ -85,6 +95,7 @@ struct WinArgs {
   int window, sinks;
   const float* lse;    // [B, H, T] log2 domain
   const float* delta;  // [B, H, T]
+  int* counter;        // items taken, zero at the start
   DeviceStatus* status;
 };
 
@@ -124,35 +135,68 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* staged = s_full + 9;       // dK / dV is in the dS^T tile
   uint64_t* stored = s_full + 10;      // the stores have read it
   uint64_t* done = s_full + 11;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_full + 12);
+  uint64_t* item_full = s_full + 12;   // [kRing]
+  uint64_t* item_empty = item_full + Cfg::kRing;
+  int* sItem = reinterpret_cast<int*>(item_empty + Cfg::kRing);  // [kRing][4]
+  int* sGroup = sItem + 4 * Cfg::kRing;                           // [2][2][4] items of the compute / read-out warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sGroup + 16);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int T = a.T;
   const int n_blocks = (T + BK - 1) / BK, n_qblocks = (T + BQ - 1) / BQ;
   const int n_sink = min(n_blocks, (a.sinks + BK - 1) / BK);  // key blocks with sinks
   const int n_items = n_blocks * a.BH;
-  struct Item {
-    int bh, b, h, n0, i_start, steps;
+  struct Item {  // steps == 0: no more items
+    int b, h, n0, steps;
+    __device__ int i_start() const { return n0 / BQ; }  // BQ == BK: the diagonal block
   };
   // items with sinks first; the others head by head, so that CTAs share a head's Q and dO in L2
   auto decode = [&](int it) {
-    Item w;
-    int n_block;
+    if (it >= n_items) return Item{0, 0, 0, 0};
+    int bh, n_block;
     if (it < n_sink * a.BH) {
-      w.bh = it % a.BH;
+      bh = it % a.BH;
       n_block = it / a.BH;
     } else {
       const int r = it - n_sink * a.BH, rest = n_blocks - n_sink;
-      w.bh = r / rest;
+      bh = r / rest;
       n_block = n_sink + r % rest;
     }
-    w.b = w.bh / a.H;
-    w.h = w.bh % a.H;
-    w.n0 = n_block * BK;
-    w.i_start = n_block;  // BQ == BK
-    const int end = w.n0 < a.sinks ? n_qblocks : min(n_qblocks, (w.n0 + BK - 1 + a.window - 1) / BQ + 1);
-    w.steps = end - w.i_start;
+    const int n0 = n_block * BK;
+    const int end = n0 < a.sinks ? n_qblocks : min(n_qblocks, (n0 + BK - 1 + a.window - 1) / BQ + 1);
+    return Item{bh / a.H, bh % a.H, n0, end - n_block};
+  };
+  auto warp_arrive = [&](uint64_t* bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  // item k of this CTA; after a failed wait as if there were none
+  auto take = [&](uint32_t k, int where) {
+    const uint32_t st = k % Cfg::kRing;
+    if (!mbar_wait_bounded(&item_full[st], (k / Cfg::kRing) & 1u, a.status, kErrWaitTimeoutFull, where))
+      return Item{0, 0, 0, 0};
+    const int4 v = *reinterpret_cast<const int4*>(sItem + st * 4);
+    return Item{v.x, v.y, v.z, v.w};
+  };
+  auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+  // the same for a whole warp, which also gives the slot back
+  auto take_warp = [&](uint32_t k, int where) {
+    Item w = take(k, where);
+    w = Item{uniform(w.b), uniform(w.h), uniform(w.n0), uniform(w.steps)};
+    if (lane == 0) mbar_arrive(&item_empty[k % Cfg::kRing]);
     return w;
+  };
+  // the same for all warps of a group, which go on together after a failed wait too: they meet at
+  // named barriers
+  auto take_group = [&](uint32_t k, int where, bool first, int* shared, int barrier, int threads) {
+    int4* slot = reinterpret_cast<int4*>(shared + (k & 1) * 4);
+    if (first) {
+      const Item w = take_warp(k, where);
+      if (lane == 0) *slot = make_int4(w.b, w.h, w.n0, w.steps);
+    }
+    named_barrier_sync(barrier, threads);
+    const int4 v = *slot;
+    return Item{uniform(v.x), uniform(v.y), uniform(v.z), uniform(v.w)};
   };
   static_assert(BQ == BK, "the diagonal block of key block n is query block n");
   constexpr int kProducerWarp = 8, kMmaWarp = 9, kProducerWarp2 = 10;
@@ -176,16 +220,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
-    mbar_init(p_full, kCompute);
-    mbar_init(ds_full, kCompute);
+    mbar_init(p_full, kCompute / 32);
+    mbar_init(ds_full, kCompute / 32);
     mbar_init(dv_done, 1);
     mbar_init(ds_free, 1);
     mbar_init(dq_full, 1);
-    mbar_init(dq_free, kReadout);
-    mbar_init(dkv_free, kCompute);
-    mbar_init(staged, kCompute);
+    mbar_init(dq_free, kReadout / 32);
+    mbar_init(dkv_free, kCompute / 32);
+    mbar_init(staged, kCompute / 32);
     mbar_init(stored, 1);
     mbar_init(done, 1);
+    for (int i = 0; i < Cfg::kRing; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 4);  // compute, read-out, MMA, second producer
+    }
     fence_barrier_init();
     fence_proxy_async_smem();
   }
@@ -213,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto load_q = [&](const Item& w, int t) {
       const uint32_t st = gq % NQ;
       if (!wait(&q_empty[st], ((gq / NQ) & 1u) ^ 1u, 400)) return false;
-      const int q0 = (w.i_start + t) * BQ;
+      const int q0 = (w.i_start() + t) * BQ;
       if (lane == 0) {
         mbar_arrive_expect_tx(&q_full[st], Cfg::kTile);
         for (int kd = 0; kd < KD; ++kd)
@@ -223,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) {
         const int qq = q0 + i * 32 + lane;
-        v[i] = qq < T ? __ldg(a.lse + (long long)w.bh * T + qq) : INFINITY;
+        v[i] = qq < T ? __ldg(a.lse + ((long long)w.b * a.H + w.h) * T + qq) : INFINITY;
       }
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) sLse[st * BQ + i * 32 + lane] = v[i];
@@ -235,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto load_do = [&](const Item& w, int t) {
       const uint32_t st = gd % ND;
       if (!wait(&do_empty[st], ((gd / ND) & 1u) ^ 1u, 401)) return false;
-      const int q0 = (w.i_start + t) * BQ;
+      const int q0 = (w.i_start() + t) * BQ;
       if (lane == 0) {
         mbar_arrive_expect_tx(&do_full[st], Cfg::kTile);
         for (int kd = 0; kd < KD; ++kd)
@@ -245,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) {
         const int qq = q0 + i * 32 + lane;
-        v[i] = qq < T ? __ldg(a.delta + (long long)w.bh * T + qq) : 0.f;
+        v[i] = qq < T ? __ldg(a.delta + ((long long)w.b * a.H + w.h) * T + qq) : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) sDelta[st * BQ + i * 32 + lane] = v[i];
@@ -254,12 +302,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++gd;
       return true;
     };
-    for (int it = blockIdx.x; it < n_items && ok; it += gridDim.x, ++k) {
-      const Item w = decode(it);
-      if (warp == kProducerWarp2) {
-        for (int t = 0; t < w.steps && ok; ++t) ok = load_do(w, t);
-        continue;
+    // the first producer takes the items, one ahead, and hands them out
+    auto publish = [&](uint32_t n, const Item& w) {
+      if (!wait(&item_empty[n % Cfg::kRing], ((n / Cfg::kRing) & 1u) ^ 1u, 406)) return false;
+      if (lane == 0) {
+        *reinterpret_cast<int4*>(sItem + n % Cfg::kRing * 4) = make_int4(w.b, w.h, w.n0, w.steps);
+        mbar_arrive(&item_full[n % Cfg::kRing]);
       }
+      return true;
+    };
+    if (warp == kProducerWarp2) {
+      for (uint32_t n = 0; ok; ++n) {
+        const Item w = take_warp(n, 407);
+        if (w.steps == 0) break;
+        for (int t = 0; t < w.steps && ok; ++t) ok = load_do(w, t);
+      }
+    }
+    int taken = 0;
+    Item w = decode(blockIdx.x);
+    if (warp == kProducerWarp) {
+      if (lane == 0) taken = atomicAdd(a.counter, 1);
+      ok = publish(0, w);
+    }
+    for (; ok && warp == kProducerWarp && w.steps > 0; ++k) {
       const uint32_t kb = k % KV;
       // Q before K and V: with one K / V buffer those wait for the item before
       if (!load_q(w, 0) || !wait(&kv_empty[kb], ((k / KV) & 1u) ^ 1u, 402)) {
@@ -275,7 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                       w.n0, w.b);
         }
       }
+      const Item next = decode((int)gridDim.x + uniform(taken));
+      ok = publish(k + 1, next);
+      if (lane == 0 && next.steps > 0) taken = atomicAdd(a.counter, 1);  // used an item later
       for (int t = 1; t < w.steps && ok; ++t) ok = load_q(w, t);
+      w = next;
     }
     // every issued copy lands before the CTA exits
     if (lane == 0) {
@@ -303,8 +372,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait = [&](uint64_t* bar, uint32_t phase, int where) {
         return mbar_wait_bounded(bar, phase & 1u, a.status, kErrWaitTimeoutAccum, where);
       };
-      for (int it = blockIdx.x; it < n_items && ok; it += gridDim.x, ++k) {
-        const Item w = decode(it);
+      Item w = take(0, 422), next{};
+      for (; w.steps > 0 && ok; w = next, ++k) {
+        next.steps = 0;
         const uint32_t k16 = kv16 + (k % KV) * 2 * tile16, v16 = k16 + tile16;
         auto issue_s = [&](uint32_t gs, uint32_t key16) {  // S^T of step gs; its columns are free
           if (!wait(&q_full[gs % NQ], gs / NQ, 410)) return false;
@@ -341,7 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int t = 0; t < w.steps; ++t, ++g) {
           // whether, and with which K / V, the step after this one is begun from here
-          const bool more = t + 1 < w.steps, ahead = more || (KV == 2 && it + (int)gridDim.x < n_items);
+          const bool more = t + 1 < w.steps;
+          if (!more) {
+            mbar_arrive(&item_empty[k % Cfg::kRing]);
+            next = take(k + 1, 422);
+          }
+          const bool ahead = more || (KV == 2 && next.steps > 0);
           const uint32_t next16 = more ? k16 : kv16 + ((k + 1) % KV) * 2 * tile16;
           if (!wait(p_full, g, 414)) {
             ok = false;
@@ -414,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* dst_row = sDST + half * (128 * 128) + r * 128;
     uint32_t g = 0, k = 0;
     // warp-uniform; after a failed wait a warp does no more work and waits no more, but still meets
-    // the named barrier that the other warp of its lanes waits at
+    // the named barriers
     bool ok = true;
     uint32_t n_staged = 0, n_read = 0;
     // the stores so far have read the dS^T tile
@@ -466,10 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (i == KD - 1) {
           tc_fence_before();
-          mbar_arrive(dkv_free);  // the next item may accumulate
+          warp_arrive(dkv_free);  // the next item may accumulate
         }
         fence_proxy_async_smem();
-        mbar_arrive(staged);
+        warp_arrive(staged);
         if (warp == 0) {
           ok = mbar_wait_warp(staged, n_staged & 1u, a.status, kErrWaitTimeoutAccum, 438);
           if (storer && ok) {
@@ -486,11 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     Item last{};
-    for (int it = blockIdx.x; it < n_items; it += gridDim.x, ++k) {
-      const Item w = decode(it);
+    for (;; ++k) {
+      const Item w = take_group(k, 439, warp == 0, sGroup, 6, kCompute);
+      if (w.steps == 0) break;
       const int key = w.n0 + r, key_lo = w.n0 + quarter * 32;
       for (int t = 0; t < w.steps; ++t, ++g) {
-        const int qh = (w.i_start + t) * BQ + half * 64;  // first query of this half
+        const int qh = (w.i_start() + t) * BQ + half * 64;  // first query of this half
         // queries [qmin, qmax] of the half are visible to this key
         const int qmin = key < T ? key - qh : 64;
         const int qmax = key < a.sinks ? 64 : key + a.window - 1 - qh;
@@ -563,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_32x32b_x32(lb + Cfg::kPT + half * 32, hp);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(p_full);
+        warp_arrive(p_full);
         // the item before is stored here where its successor's first S^T did not have to wait for it
         if (KV == 2 && t == 0 && k > 0) store_item(last, g);
         // ---- dS^T
@@ -610,12 +686,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               make_uint4(hd[ch * 4], hd[ch * 4 + 1], hd[ch * 4 + 2], hd[ch * 4 + 3]);
         tc_fence_before();
         fence_proxy_async_smem();
-        mbar_arrive(ds_full);
+        warp_arrive(ds_full);
       }
       if (KV == 1) store_item(w, g);
       last = w;
     }
-    if (KV == 2) store_item(last, g);  // every CTA has an item
+    if (KV == 2 && ok) store_item(last, g);  // every CTA has an item
     if (storer) bulk_wait_group0();
   } else if (warp >= 12) {
     // ------------------------------------------------------------ dQ read-out
@@ -623,11 +699,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = quarter * 32 + lane;  // query row within the block
     const uint32_t lb = tmem + ((uint32_t)(quarter * 32) << 16);
     const bool leader = warp == 12 && lane == 0;  // issues the TMA reductions
-    uint32_t g = 0;
-    int chunk = 0;
+    uint32_t g = 0, chunk = 0;
     bool ok = true;  // per warp; the named barriers are met in any case
-    for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-      const Item w = decode(it);
+    for (uint32_t k = 0;; ++k) {
+      const Item w = take_group(k, 443, warp == 12, sGroup + 8, 1, kReadout);
+      if (w.steps == 0) break;
       for (int t = 0; t < w.steps; ++t, ++g) {
         if (ok && !mbar_wait_warp(dq_full, g & 1u, a.status, kErrWaitTimeoutAccum, 440)) ok = false;
 #pragma unroll 1
@@ -639,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_ld_regs<32>(v);
             if (c == D / 32 - 1) {
               tc_fence_before();
-              mbar_arrive(dq_free);
+              warp_arrive(dq_free);
             }
           }
           uint8_t* box = sBox + (chunk & 1) * Cfg::kBox;
@@ -654,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           named_barrier_sync(1, kReadout);
           if (leader && ok) {
-            tma_reduce_add_3d(&tm_dq, box, w.h * D + c * 32, (w.i_start + t) * BQ, w.b);
+            tma_reduce_add_3d(&tm_dq, box, w.h * D + c * 32, (w.i_start() + t) * BQ, w.b);
             bulk_commit_group();
           }
         }
@@ -703,12 +779,13 @@ void launch(const AttnBwdParams& p, cudaStream_t s) {
   a.sinks = p.f.sinks;
   a.lse = p.f.lse;
   a.delta = p.delta;
+  a.counter = reinterpret_cast<int*>(p.delta + (long long)p.f.B * p.f.H * p.f.T);
   a.status = device_status_ptr();
   const long long items = (long long)((p.f.T + BK - 1) / BK) * a.BH;
   int dev = 0, sms = 0;
   UHFS_CUDA_CHECK(cudaGetDevice(&dev));
   UHFS_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  if (items > 0x7fffffffll) throw std::runtime_error("flash attention backward: too many key blocks");
+  if (items > 0x7fff0000ll) throw std::runtime_error("flash attention backward: too many key blocks");
   fa_bwd_window_kernel<D><<<(int)(items < sms ? items : sms), kThreads, Cfg::kSmem, s>>>(tq, td, tdq, tdqkv, a);
   note_launch();
   UHFS_CUDA_CHECK(cudaGetLastError());

@@ -127,13 +127,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // could block.
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, DeviceStatus* st, int err,
                                                   int where) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t spins = 0;
-  while (true) {
+  // The clock is first read after 64 tries: most waits end before, and reading it is slow.
+  uint64_t t0 = 0;
+  for (uint32_t spins = 1;; ++spins) {
     if (mbar_try_wait(bar, parity)) return true;
-    if (((++spins) & 255u) == 0u) {
-      if (globaltimer_ns() - t0 > kWaitBoundNs) {
+    if ((spins & 63u) == 0u) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitBoundNs) {
         report_error(st, err, where);
         return false;
       }

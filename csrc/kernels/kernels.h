@@ -107,7 +107,7 @@ struct AttnBwdParams {
   long long dq_stride_b, dq_stride_t;
   long long dk_stride_b, dk_stride_t;
   long long dv_stride_b, dv_stride_t;
-  float* delta;      // [B, H, T] scratch
+  float* delta;      // [B, H, T] scratch; with a window one element more, the work counter
   float* dq_accum;   // [B, T, H, D] fp32 scratch (zeroed by the launcher's prologue kernel)
 };
 void flash_attn_fwd(const AttnParams& p, cudaStream_t s);

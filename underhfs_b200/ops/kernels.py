@@ -343,7 +343,8 @@ def flash_attn_qkv_backward(qkv, o, lse, do, B, T, H, D, causal, scale=None, win
     F = H * D
     scale = (1.0 / math.sqrt(D)) if scale is None else scale
     dqkv = torch.empty((B * T, 3 * F), dtype=torch.bfloat16, device=qkv.device)
-    delta = torch.empty((B, H, T), dtype=torch.float32, device=qkv.device)
+    # per-row sums; the windowed kernel's work counter behind them
+    delta = torch.empty(B * H * T + 1, dtype=torch.float32, device=qkv.device)
     dq_acc = torch.empty((B * T, F), dtype=torch.float32, device=qkv.device)
     base = qkv.data_ptr()
     dbase = dqkv.data_ptr()
