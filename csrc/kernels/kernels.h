@@ -156,7 +156,7 @@ struct Kv4Attend {
   int B, Tq, Hq, Hkv, pages_per_head, capacity;
   float scale;
   int window, sinks;     // window 0: none
-  int q_tiles, splits;   // set by the launcher
+  int q_tiles, splits, warps;  // set by the launcher: tiles of 8 queries; blocks per head; warps per block
   DeviceStatus* status;  // set by the launcher
 };
 void kv4_append(const Kv4Append& p, int dtype, int D, cudaStream_t s);

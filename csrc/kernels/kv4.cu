@@ -287,18 +287,19 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
 //      places of the odd codes.  q is only scaled, by a power of two per query that
 //      brings it to [1, 2): a bf16 or fp16 q goes in without a rounding.
 //   V  s and lo are per token, the products' inner dimension: O = sum over tokens of
-//      r code - 8 r + P (lo + 8 s) with r = P s rounded to fp16 (P itself goes in as two
-//      fp16 numbers); the last two terms are products with one row per group.  The 8 makes
+//      r (code - 8) + P (lo + 8 s) with r = P s rounded to fp16 (P itself goes in as two
+//      fp16 numbers); -8 r is one more product on the codes' rows (a constant operand: a row per
+//      group in the lo product cost an operand each time), the lo term one row per group.  The 8 makes
 //      the rounding's share that of code - 8, not of code: without it its error was twice as
 //      large.
 // So K is not rounded, and for V only P s and lo + 8 s are.
 // Every warp works alone: it owns a ring of pages filled by bulk copies and takes
-// every kWarps-th page of the block's share, with its own running maximum (raised
+// every n-th page of the block's share (n warps), with its own running maximum (raised
 // only when a score exceeds it by 2^2, which keeps P s in fp16's range) and sum.  The warps of a block are joined in
 // shared memory and the blocks of a cluster, which share one head's tokens, through
 // distributed shared memory: one launch, no workspace, no atomics, and a sum order
 // that depends on sizes only.
-constexpr int kWarps = 8;
+constexpr int kMaxWarps = 8;  // per block
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 2.0f;  // s <= 2 * kRange / 15 = 8192
 
@@ -354,21 +355,24 @@ __device__ __forceinline__ float dsmem_load(const float* p, uint32_t rank) {
 template <int D>
 struct Kv4Attn {
   static constexpr int kStages = D == 128 ? 2 : 4;  // pages in flight per warp
-  static constexpr int kRing = kWarps * kStages * Kv4<D>::kBytes;
-  // after the pages: the warps' sums [kWarps][8][D], their m and l, and the block's result
-  static constexpr int kJoin = (kWarps * 8 * D + 2 * kWarps * 8 + 8 * D + 2 * 8) * 4;
-  static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kSmem = 128 + kBody + kWarps * kStages * 8;
+  // a block of `warps`: their pages, then in the same place the warps' sums [warps][8][D], their
+  // m and l, and the block's result
+  static __host__ __device__ constexpr int body(int warps) {
+    const int ring = warps * kStages * Kv4<D>::kBytes, join = (warps * 8 * D + 2 * warps * 8 + 8 * D + 2 * 8) * 4;
+    return ring > join ? ring : join;
+  }
+  static __host__ __device__ constexpr int smem(int warps) { return 128 + body(warps) + warps * kStages * 8; }
 };
 
 template <int D, typename T>
-__global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Attend a) {
+__global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4Attend a) {
   using F = Kv4<D>;
   using C = Kv4Attn<D>;
   constexpr int NG = F::NG, NS = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBody);
+  const int n_warps = blockDim.x >> 5;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::body(n_warps));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int splits = a.splits;                  // blocks of a cluster
   const int rank = blockIdx.x % splits;
@@ -394,7 +398,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   const int n_pages = p_sink + p_hi - p_first;
   const int share = (n_pages + splits - 1) / splits;
   const int i_end = min(n_pages, (rank + 1) * share);
-  const int i_begin = rank * share + warp;  // this warp: i_begin, i_begin + kWarps, ...
+  const int i_begin = rank * share + warp;  // this warp: i_begin, i_begin + n_warps, ...
   auto page_of = [&](int i) { return i < p_sink ? i : p_first + i - p_sink; };
 
   uint8_t* ring = smem + warp * (NS * F::kBytes);
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
     fence_barrier_init();
     fence_proxy_async_smem();
     for (int s = 0; s < NS; ++s)
-      if (i_begin + s * kWarps < i_end) issue(i_begin + s * kWarps, s);
+      if (i_begin + s * n_warps < i_end) issue(i_begin + s * n_warps, s);
   }
   __syncwarp();
 
@@ -471,18 +475,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
     for (int c = 0; c < 2; ++c)  // columns 2 t and 2 t + 1 of the products
       scale2[c] = __shfl_sync(0xffffffffu, up, (2 * t + c) * 4) * (a.scale * kLog2e);
   }
-  // tokens visible to columns 2 t, 2 t + 1: [low, lim) and [0, sinks)
-  int lim[2], low[2];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int col = 2 * t + c;
-    lim[c] = low[c] = 0;
-    if (col < rows) {
-      const long long end = len + (row0 + col) / G + 1;
-      lim[c] = (int)min(max(end, 0ll), (long long)a.capacity);
-      low[c] = a.window > 0 ? (int)max(0ll, min(end - a.window, (long long)a.capacity)) : 0;
-    }
-  }
   const int lim_all = (int)max(0ll, min(len + row0 / G + 1, (long long)a.capacity));  // visible to every live query
   const int low_all = rows > 0 && a.window > 0 ? (int)max(0ll, hi - a.window) : 0;
 
@@ -495,7 +487,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   const int prow = (g & 1) ? (g >> 1) + 4 : (g >> 1);  // token of product row g within 8
 
   int n_done = 0;
-  for (int i = i_begin; i < i_end; i += kWarps, ++n_done) {
+  for (int i = i_begin; i < i_end; i += n_warps, ++n_done) {
     const int slot = n_done % NS;
     if (!mbar_wait_warp(&full[slot], (uint32_t)(n_done / NS) & 1u, a.status, kErrWaitTimeoutFull, 62)) break;
     const uint8_t* pg = ring + slot * F::kBytes;
@@ -534,6 +526,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
       for (int e = 0; e < 4; ++e) s[mt][e] = fmaf(sc[e], kCodeUnit, lo_part[e]) * scale2[e & 1];
     }
     if (key0 + kPage > lim_all || key0 < low_all) {
+      // tokens visible to columns 2 t, 2 t + 1: [low, lim) and [0, sinks)
+      int lim[2], low[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = 2 * t + c;
+        lim[c] = low[c] = 0;
+        if (col < rows) {
+          const long long end = len + (row0 + col) / G + 1;
+          lim[c] = (int)min(max(end, 0ll), (long long)a.capacity);
+          low[c] = a.window > 0 ? (int)max(0ll, min(end - a.window, (long long)a.capacity)) : 0;
+        }
+      }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -612,18 +616,19 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
         mma_f16(o[gi][0], even_codes(x), odd_codes(x), even_codes(y), odd_codes(y), b0, b1);
         const uint32_t x2 = x >> 8, y2 = y >> 8;
         mma_f16(o[gi][1], even_codes(x2), odd_codes(x2), even_codes(y2), odd_codes(y2), b0, b1);
-        const uint32_t m8 = g == gi ? 0xc800c800u : 0u;  // -8 in row gi
-        mma_f16(o_lo, m8, 0u, m8, 0u, b0, b1);
+        // -8 for every code (rows of the odd ones, times 16, are the upper eight)
+        mma_f16(o[gi][0], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+        mma_f16(o[gi][1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
       }
     }
     __syncwarp();  // every lane has read the page
-    if (lane == 0 && i + NS * kWarps < i_end) issue(i + NS * kWarps, slot);
+    if (lane == 0 && i + NS * n_warps < i_end) issue(i + NS * n_warps, slot);
   }
   // copies still in flight (only after a wait that gave up): they land before the memory is used again
-  if (i_begin + n_done * kWarps < i_end) {
+  if (i_begin + n_done * n_warps < i_end) {
     for (int s = 0; s < NS; ++s) {
       const int k = n_done + s;
-      if (i_begin + k * kWarps < i_end)
+      if (i_begin + k * n_warps < i_end)
         mbar_wait_warp(&full[k % NS], (uint32_t)(k / NS) & 1u, a.status, kErrWaitTimeoutFull, 63);
     }
   }
@@ -639,10 +644,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
     for (int c = 0; c < 2; ++c) lo_sum[gi][c] = __shfl_sync(0xffffffffu, o_lo[c], gi * 4 + t);
 
   // ---- join the block's warps
-  float* wo = reinterpret_cast<float*>(smem);   // [kWarps][8][D]
-  float* wm = wo + kWarps * 8 * D;              // [kWarps][8]
-  float* wl = wm + kWarps * 8;
-  float* bo = wl + kWarps * 8;                  // the block: [8][D], m, l
+  float* wo = reinterpret_cast<float*>(smem);   // [warps][8][D]
+  float* wm = wo + n_warps * 8 * D;              // [warps][8]
+  float* wl = wm + n_warps * 8;
+  float* bo = wl + n_warps * 8;                  // the block: [8][D], m, l
   float* bm = bo + 8 * D;
   float* bl = bm + 8;
   __syncthreads();  // the pages are done with
@@ -663,14 +668,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   }
   __syncthreads();
   const int live = max(rows, 0) * D;
-  for (int e = threadIdx.x; e < live; e += kWarps * 32) {
+  for (int e = threadIdx.x; e < live; e += n_warps * 32) {
     const int col = e / D;
     float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, wm[w * 8 + col]);
+    for (int w = 0; w < n_warps; ++w) m = fmaxf(m, wm[w * 8 + col]);
     float l = 0.f, v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < n_warps; ++w) {
       // no maximum: nothing was visible (all sums are 0) or every score was NaN (so is the sum)
       const float f = m == -INFINITY ? 1.f : ex2_approx(wm[w * 8 + col] - m);
       l = fmaf(f, wl[w * 8 + col], l);
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   if (splits > 1) cluster_sync_all();
   else __syncthreads();
   T* out = static_cast<T*>(a.o);
-  for (int e = threadIdx.x + rank * (kWarps * 32); e < live; e += splits * (kWarps * 32)) {
+  for (int e = threadIdx.x + rank * (n_warps * 32); e < live; e += splits * (n_warps * 32)) {
     const int col = e / D, mrow = row0 + col;
     float m = -INFINITY, l = 0.f, v = 0.f;
     if (splits == 1) {
@@ -706,7 +709,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv4_attend_kernel(const Kv4Att
   // queries past the sequence's own tokens: zeros
   if (rank == 0) {
     const int total = min(8, a.Tq * G - row0);
-    for (int e = live + threadIdx.x; e < total * D; e += kWarps * 32) {
+    for (int e = live + threadIdx.x; e < total * D; e += n_warps * 32) {
       const int mrow = row0 + e / D;
       out[(((long long)b * a.Tq + mrow / G) * a.Hq + h * G + mrow % G) * D + e % D] = from_float<T>(0.f);
     }
@@ -720,14 +723,14 @@ void launch_attend(const Kv4Attend& a, cudaStream_t s) {
   static PerDeviceOnce once;
   once([] {
     UHFS_CUDA_CHECK(
-        cudaFuncSetAttribute(kv4_attend_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        cudaFuncSetAttribute(kv4_attend_kernel<D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(kMaxWarps)));
   });
   const long long units = (long long)a.B * a.Hkv * a.q_tiles;
   if (units * a.splits > 0x7fffffffll) throw std::runtime_error("kv4 attention: too many blocks");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(units * a.splits));
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.blockDim = dim3(a.warps * 32);
+  cfg.dynamicSmemBytes = C::smem(a.warps);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -817,16 +820,23 @@ void kv4_attend(const Kv4Attend& p, int dtype, int D, cudaStream_t s) {
   const long long rows = (long long)p.Tq * (p.Hq / p.Hkv);
   if (rows > (1 << 28)) throw std::runtime_error("kv4 attention: too many new tokens");
   a.q_tiles = (int)((rows + 7) / 8);
-  // Blocks per head: enough for two blocks on each SM, as far as every warp of a
-  // block still has a page; 8 is the largest portable cluster.
   const long long units = (long long)p.B * p.Hkv * a.q_tiles;
   int seen = p.pages_per_head;
   if (p.window > 0) {
     const long long w = (long long)(p.window + p.Tq) / kPage + 2 + (p.sinks + kPage - 1) / kPage;
     if (w < seen) seen = (int)w;
   }
+  // An SM holds 16 warps.  Units are split, over as many blocks as fit at once and have a page
+  // for every warp; a second wave of blocks costs more than the shorter first one saves (16 x
+  // 8192 tokens, 8 heads: 57 us with 4 blocks of 8 warps, 47 with 2; 8 is the largest portable
+  // cluster).  Blocks of 4 warps where there are enough of them to fill the SMs: they
+  // leave less over (64 x 1024 tokens, 8 heads: 33 us, 39 with 8 warps); over several waves of
+  // blocks 8 (32 x 4096 tokens, 32 heads: 125 us, 131 with 4).
+  constexpr int kSmWarps = 16 * 148;
+  a.warps = units * 8 * 4 > kSmWarps && units * 4 <= kSmWarps ? 4 : 8;
   a.splits = 1;
-  while (a.splits < 8 && units * a.splits < 2 * 148 && a.splits * 2 * kWarps <= seen + kWarps - 1) a.splits *= 2;
+  while (a.splits < 8 && units * a.splits * 2 * a.warps <= kSmWarps && a.splits * 2 * a.warps <= seen + a.warps - 1)
+    a.splits *= 2;
   if (dtype == DT_BF16) {
     if (D == 64) launch_attend<64, __nv_bfloat16>(a, s);
     else launch_attend<128, __nv_bfloat16>(a, s);

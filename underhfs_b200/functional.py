@@ -86,8 +86,8 @@ def softmax(input: Tensor) -> Tensor:
 
 def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dtype, low: float, high: float):
     """A sampling setting: a checked number, or a tensor with one value per row."""
-    if isinstance(value, Tensor):
-        value = value._data
+    if not isinstance(value, (int, float)):
+        value = value._data if isinstance(value, Tensor) else value
     if isinstance(value, torch.Tensor):
         if value.numel() != rows:
             raise ValueError(f"{name} needs one value for each of {rows} rows, got {list(value.shape)}")
@@ -129,10 +129,12 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     if u.device != x.device:
         raise RuntimeError(f"uniform is on {u.device}, the logits on {x.device}")
     shape, vocab = x.shape[:-1], x.shape[-1]
-    x = x.detach() if x.dim() == 2 else x.detach().reshape(-1, vocab)
+    if x.dim() != 2:
+        x = x.detach().reshape(-1, vocab)
     rows = x.shape[0]
     real = torch.float32 if x.is_cuda else torch.float64
-    u = u.detach().reshape(-1).to(real).contiguous()
+    if u.dim() != 1 or u.dtype != real or not u.is_contiguous():
+        u = u.detach().reshape(-1).to(real).contiguous()
     temperature = _setting(temperature, "temperature", rows, x.device, real, 0.0, 1e30)
     top_k = _setting(top_k, "top_k", rows, x.device, torch.int32, 0, 2**31 - 1)
     top_p = _setting(top_p, "top_p", rows, x.device, real, 0.0, 1.0)
@@ -148,7 +150,7 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
             with torch.cuda.device(x.device):
                 token = K.sample_tokens(x, u, temperature, top_k, top_p, min_p)
     else:
-        token = _sample_cpu(x.double(), u, temperature, top_k, top_p, min_p)
+        token = _sample_cpu(x.detach().double(), u.detach(), temperature, top_k, top_p, min_p)
     return Tensor._wrap(token if len(shape) == 1 else token.reshape(shape))
 
 

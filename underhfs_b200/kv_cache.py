@@ -24,6 +24,8 @@ import math
 
 import torch
 
+from underhfs_b200.ops import kernels as K
+
 GROUP = 32   # channels that share a scale and a minimum
 PAGE = 32    # tokens per page of the CUDA layout
 RANGE = 61440.0  # values are held to +-RANGE, where lo + scale * code is a finite fp16 number
@@ -75,6 +77,7 @@ class QuantizedKVCache:
             self.pages = torch.zeros((self.layers, self.batch, self.kv_heads, pages, 40 * self.head_dim),
                                      dtype=torch.uint8, device=self.device)
             self.device = self.pages.device
+            self._pages = list(self.pages)  # one view a layer: making one costs as much as a launch
         else:
             if self.head_dim < GROUP or self.head_dim % GROUP:
                 raise ValueError(f"head_dim must be a multiple of {GROUP}, got {head_dim}")
@@ -159,10 +162,8 @@ class QuantizedKVCache:
         if k.shape[1] == 0:
             return
         if self._cuda:
-            from underhfs_b200.ops import kernels as K
-
             with self._on_device():
-                K.kv4_append(self.pages[layer], k, v, self.lengths, counts, self.max_len)
+                K.kv4_append(self._pages[layer], k, v, self.lengths, counts, self.max_len)
             return
         k, v = k.detach(), v.detach()
         for b in range(self.batch):
@@ -191,8 +192,6 @@ class QuantizedKVCache:
         else:
             self._check_room(tokens)
         scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        from underhfs_b200.ops import kernels as K
-
         window, sinks = (0, 0) if window is None and sinks == 0 else K.window_args(self.max_len, True, window, sinks)
         if self._cuda:
             if q.dtype not in (torch.bfloat16, torch.float16):
@@ -200,7 +199,7 @@ class QuantizedKVCache:
             if tokens == 0:
                 return torch.empty_like(q)
             with self._on_device():
-                return K.kv4_attend(self.pages[layer], q, self.lengths, counts, self.max_len, scale, window, sinks)
+                return K.kv4_attend(self._pages[layer], q, self.lengths, counts, self.max_len, scale, window, sinks)
         q = q.detach()
         out = torch.zeros(q.shape, dtype=torch.float64)
         for b in range(self.batch):
@@ -227,10 +226,8 @@ class QuantizedKVCache:
         if self._cuda:
             if dtype == torch.float64:
                 raise TypeError("the CUDA cache reads as fp32, fp16 or bf16")
-            from underhfs_b200.ops import kernels as K
-
             with self._on_device():
-                return K.kv4_read(self.pages[layer], start, count, self.head_dim, dtype)
+                return K.kv4_read(self._pages[layer], start, count, self.head_dim, dtype)
         return tuple(x[layer, :, start : start + count].to(dtype) for x in (self._k, self._v))
 
     def advance(self, tokens) -> None:
