@@ -31,8 +31,11 @@
 // or j < sinks, so tile A needs the sink blocks [0, ceil(sinks / 128)) and the
 // blocks from (m0 - window + 1) / 128 to its diagonal; blocks between the two
 // are never loaded.  Both tiles walk tile A's list (tile B ends one block
-// later and skips the first window block where the window has left it), and
-// the masks cost compares only in blocks that hold a mask edge.  q / k / v are
+// later and skips the first window block where the window has left it).  Of a
+// block's 32-column pieces a warp's 32 rows skip those that none of them sees
+// (zeros in P, no exponentials) and mask only those that hold an edge: 54 us
+// where masking whole blocks took 61 (16 x 1024 tokens, 12 x 64, window 256, 4
+// sinks), 109 and 112 (2 x 4096, 16 x 128, window 1024).  q / k / v are
 // read through a [B][T][3F] map whose rows past T are zeros, so a sequence of
 // ragged length never multiplies its zero probabilities with another
 // sequence's values.
@@ -438,13 +441,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (tracer && t == 0) FWD_TRACE(w.cta, kTrSRegsA, j);
         const int key0 = block_of(w, j) * BKV;
         const int lim = key_limit - key0;  // visible columns of this block: [0, lim)
+        // kWin, per 32 columns: 0 no row of the warp sees any, 1 some do, 2 all see all
+        int piece[BKV / 32];
         if constexpr (kWin) {
-          // and of those the columns from `low` on (the window) or below `snk` (the sinks)
+          const int q_lo = q - lane, q_hi = q_lo + 31;
+          // and of [0, lim) the columns from `low` on (the window) or below `snk` (the sinks)
           const int low = q - a.window + 1 - key0, snk = a.sinks - key0;
-          if (lim < BKV || (low > 0 && snk < BKV)) {
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
 #pragma unroll
-            for (int i = 0; i < BKV; ++i)
-              if (i >= lim || (i < low && i >= snk)) sr[i] = __float_as_uint(-INFINITY);
+          for (int c = 0; c < BKV / 32; ++c) {
+            const int k_lo = key0 + c * 32, k_hi = k_lo + 31;
+            const bool none = k_lo > q_hi || k_lo >= T || (k_hi <= q_lo - a.window && k_lo >= a.sinks);
+            const bool all = k_hi <= q_lo && k_hi < T && (k_hi < a.sinks || k_lo > q_hi - a.window);
+            piece[c] = none ? 0 : all ? 2 : 1;
+            if (piece[c] == 1) {
+              const uint32_t vis = below(lim - c * 32) & (~below(low - c * 32) | below(snk - c * 32));
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                sr[c * 32 + i] = (vis >> i) & 1u ? sr[c * 32 + i] : __float_as_uint(-INFINITY);
+            }
           }
         } else if (lim < BKV) {
 #pragma unroll
@@ -452,13 +467,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (i >= lim) sr[i] = __float_as_uint(-INFINITY);
         }
         // row max: four independent chains of three-input max (two scores each)
-        float mx4[4] = {__uint_as_float(sr[0]), __uint_as_float(sr[1]), __uint_as_float(sr[2]),
-                        __uint_as_float(sr[3])};
+        float mx4[4];
+        if constexpr (kWin) {
 #pragma unroll
-        for (int i = 4; i < BKV; i += 8) {
+          for (int e = 0; e < 4; ++e) mx4[e] = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            mx4[e] = max3f(mx4[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e < BKV ? i + 4 + e : i + e]));
+          for (int c = 0; c < BKV / 32; ++c) {
+            if (piece[c] == 0) continue;
+#pragma unroll
+            for (int i = c * 32; i < c * 32 + 32; i += 8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                mx4[e] = max3f(mx4[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e]));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx4[e] = __uint_as_float(sr[e]);
+#pragma unroll
+          for (int i = 4; i < BKV; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              mx4[e] =
+                  max3f(mx4[e], __uint_as_float(sr[i + e]), __uint_as_float(sr[i + 4 + e < BKV ? i + 4 + e : i + e]));
+          }
         }
         const float mx = max3f(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3]));
         const float m_blk = mx * a.sl2;
@@ -472,18 +504,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 sl2x2 = make_float2(a.sl2, a.sl2), nbase = make_float2(-base, -base);
         uint32_t pk[BKV / 2];
 #pragma unroll
-        for (int i = 0; i < BKV / 2; ++i) {
-          const float2 x =
-              f2_fma(make_float2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sl2x2, nbase);
-          float2 pr;
-          if ((i & 7) < kPoly) {
-            pr = exp2_poly3_x2(x);
-          } else {
-            pr.x = ex2_approx(x.x);
-            pr.y = ex2_approx(x.y);
+        for (int c = 0; c < BKV / 32; ++c) {
+          if (kWin && piece[c] == 0) {
+#pragma unroll
+            for (int i = c * 16; i < c * 16 + 16; ++i) pk[i] = 0u;
+            continue;
           }
-          rs2[i & 1] = f2_add(rs2[i & 1], pr);
-          pk[i] = pack_bf16x2(pr.x, pr.y);
+#pragma unroll
+          for (int i = c * 16; i < c * 16 + 16; ++i) {
+            const float2 x =
+                f2_fma(make_float2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), sl2x2, nbase);
+            float2 pr;
+            if ((i & 7) < kPoly) {
+              pr = exp2_poly3_x2(x);
+            } else {
+              pr.x = ex2_approx(x.x);
+              pr.y = ex2_approx(x.y);
+            }
+            rs2[i & 1] = f2_add(rs2[i & 1], pr);
+            pk[i] = pack_bf16x2(pr.x, pr.y);
+          }
         }
         const float2 rs = f2_add(rs2[0], rs2[1]);
         l_run = l_run * alpha + (rs.x + rs.y);
