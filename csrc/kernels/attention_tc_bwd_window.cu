@@ -13,8 +13,8 @@
 //
 // Measured with the sums before and the conversion after it (28 us of 16 x 1024), against
 // 175 and 484 us of a CTA per item with every product waiting for the one before:
-//   16 x 1024 tokens, 12 x 64, window 256, 4 sinks     166 us, 6.3 K cycles a step
-//   2 x 4096 tokens, 16 x 128, window 1024, 4 sinks    284 us, 6.5 K cycles a step
+//   16 x 1024 tokens, 12 x 64, window 256, 4 sinks     155 us, about 6 K cycles a step
+//   2 x 4096 tokens, 16 x 128, window 1024, 4 sinks    280 us, about 6.4 K cycles a step
 // A step's five products are 1.3 K (D = 64) and 2.6 K cycles of the tensor core; what bounds
 // it is the chain S -> P -> dS -> dQ of a step, of which two steps do not fit in TMEM, and
 // the shared memory that the products, dS^T and the dQ boxes share.
@@ -35,7 +35,7 @@
 //
 // q / k / v / dO are read and dQ is added through [B][T][..] maps: rows past T read as
 // zeros and are not written, so ragged sequences never meet.
-// Warps: 0..7 compute, 8 items and K / V / Q / lse loads, 9 MMA issuer, 10 dO / delta loads,
+// Warps: 0..7 compute, 8 items and K / V / Q / lse / delta loads, 9 MMA issuer, 10 dO loads,
 // 12..15 dQ read-out.  512 threads launch
 // with 128 registers; the compute warpgroups take kComputeRegs of the total.
 // Every wait is bounded.
@@ -74,14 +74,14 @@ struct WinCfg {
   static constexpr bool kAlias = D == 128;   // P^T in S^T's columns, dQ in dP^T's
   static constexpr int kTile = 128 * D * 2;  // one [128][D] bf16 tile (D / 64 swizzled sub-tiles)
   static constexpr int kKV = kAlias ? 1 : 2;  // K / V buffers
-  static constexpr int kNQ = kAlias ? 2 : 3, kNDO = kAlias ? 1 : 2;  // Q (with lse) and dO (with delta) stages
+  static constexpr int kNQ = kAlias ? 2 : 3, kNDO = kAlias ? 1 : 2;  // Q (with lse and delta) and dO stages
   static constexpr int kRing = 4;  // items handed out ahead
   static constexpr int kDST = BK * BQ * 2;
   static constexpr int kBox = 128 * 32 * 4;  // fp32 dQ box: 128 rows x 32 columns
-  static constexpr int kVec = (kNQ + kNDO) * BQ * 4;
+  static constexpr int kVec = 2 * kNQ * BQ * 4;
   static constexpr int kBars = 2 * kKV + 2 * kNQ + 2 * kNDO + 12 + 2 * kRing;
   static constexpr int kSmem =
-      1024 + kKV * 2 * kTile + (kNQ + kNDO) * kTile + kDST + 2 * kBox + kVec + kBars * 8 + (kRing + 4) * 16 + 16;
+      kKV * 2 * kTile + (kNQ + kNDO) * kTile + kDST + 2 * kBox + kVec + kBars * 8 + (kRing + 4) * 16 + 16;
   static_assert(kSmem <= 227 * 1024, "attention backward shared memory");
   static_assert(kBars % 2 == 0, "the items behind the barriers are 16-byte aligned");
   static constexpr uint32_t kST = 0, kDPT = 128, kDV = 256, kDK = 256 + D;
@@ -107,16 +107,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   using Cfg = WinCfg<D>;
   constexpr int KD = D / 64;
   constexpr uint32_t KV = Cfg::kKV, NQ = Cfg::kNQ, ND = Cfg::kNDO;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_align1024(smem_raw);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {  // the swizzled tiles need it, and there is no room to round up
+    if (threadIdx.x == 0) report_error(a.status, kErrBounds, 429);
+    return;
+  }
   uint8_t* sKV = smem;                          // [KV][K | V]
   uint8_t* sQ = sKV + KV * 2 * Cfg::kTile;      // [NQ]
   uint8_t* sDO = sQ + NQ * Cfg::kTile;          // [ND]
   uint8_t* sDST = sDO + ND * Cfg::kTile;        // dS^T
   uint8_t* sBox = sDST + Cfg::kDST;             // [2]
   float* sLse = reinterpret_cast<float*>(sBox + 2 * Cfg::kBox);  // [NQ][128]
-  float* sDelta = sLse + NQ * BQ;                                // [ND][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sDelta + ND * BQ);
+  float* sDelta = sLse + NQ * BQ;                                // [NQ][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sDelta + NQ * BQ);
   uint64_t* kv_full = bars;
   uint64_t* kv_empty = kv_full + KV;   // an item's products are done with K / V
   uint64_t* q_full = kv_empty + KV;
@@ -211,11 +214,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&kv_empty[i], 1);
     }
     for (uint32_t i = 0; i < NQ; ++i) {
-      mbar_init(&q_full[i], 2);  // TMA bytes + the producer's lse stores
+      mbar_init(&q_full[i], 2);  // TMA bytes + the producer's lse and delta stores
       mbar_init(&q_empty[i], 1);
     }
     for (uint32_t i = 0; i < ND; ++i) {
-      mbar_init(&do_full[i], 2);
+      mbar_init(&do_full[i], 1);
       mbar_init(&do_empty[i], 1);
     }
     mbar_init(s_full, 1);
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
   if (warp == kProducerWarp || warp == kProducerWarp2) {
-    // ------------------------------------------------------------ producers: K, V, Q, lse; dO, delta
+    // ------------------------------------------------------------ producers: K, V, Q, lse, delta; dO
     uint32_t k = 0;  // items of this CTA so far
     bool ok = true;
     // waits in lane 0; the same answer in every lane
@@ -267,14 +270,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int kd = 0; kd < KD; ++kd)
           tma_load_3d(sQ + st * Cfg::kTile + kd * (BQ * 128), &tm_qkv, &q_full[st], w.h * D + kd * 64, q0, w.b);
       }
-      float v[BQ / 32];
+      // lse and delta share Q's stage: it is given back after dK, for which every warp has used both
+      // (dV, which frees the dO stage, does not wait for delta's readers)
+      float v[BQ / 32], u[BQ / 32];
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) {
         const int qq = q0 + i * 32 + lane;
-        v[i] = qq < T ? __ldg(a.lse + ((long long)w.b * a.H + w.h) * T + qq) : INFINITY;
+        const long long at = ((long long)w.b * a.H + w.h) * T + qq;
+        v[i] = qq < T ? __ldg(a.lse + at) : INFINITY;
+        u[i] = qq < T ? __ldg(a.delta + at) : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < BQ / 32; ++i) sLse[st * BQ + i * 32 + lane] = v[i];
+      for (int i = 0; i < BQ / 32; ++i) {
+        sLse[st * BQ + i * 32 + lane] = v[i];
+        sDelta[st * BQ + i * 32 + lane] = u[i];
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[st]);
       ++gq;
@@ -289,16 +299,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int kd = 0; kd < KD; ++kd)
           tma_load_3d(sDO + st * Cfg::kTile + kd * (BQ * 128), &tm_do, &do_full[st], w.h * D + kd * 64, q0, w.b);
       }
-      float v[BQ / 32];
-#pragma unroll
-      for (int i = 0; i < BQ / 32; ++i) {
-        const int qq = q0 + i * 32 + lane;
-        v[i] = qq < T ? __ldg(a.delta + ((long long)w.b * a.H + w.h) * T + qq) : 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < BQ / 32; ++i) sDelta[st * BQ + i * 32 + lane] = v[i];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&do_full[st]);
       ++gd;
       return true;
     };
@@ -643,8 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the item before is stored here where its successor's first S^T did not have to wait for it
         if (KV == 2 && t == 0 && k > 0) store_item(last, g);
         // ---- dS^T
-        if (!mbar_wait_warp(&do_full[g % ND], (g / ND) & 1u, a.status, kErrWaitTimeoutFull, 433) ||
-            !mbar_wait_warp(dp_full, g & 1u, a.status, kErrWaitTimeoutAccum, 434)) {
+        if (!mbar_wait_warp(dp_full, g & 1u, a.status, kErrWaitTimeoutAccum, 434)) {
           ok = false;
           continue;
         }
@@ -653,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld_32x32b_x32_async(lb + Cfg::kDPT + half * 64, pv);
         tmem_ld_32x32b_x32_async(lb + Cfg::kDPT + half * 64 + 32, pv + 32);
         tmem_wait_ld_regs<64>(pv);
-        const float4* dlt4 = reinterpret_cast<const float4*>(sDelta + (g % ND) * BQ + half * 64);
+        const float4* dlt4 = reinterpret_cast<const float4*>(sDelta + (g % NQ) * BQ + half * 64);
         uint32_t hd[32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {

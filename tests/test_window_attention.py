@@ -200,6 +200,29 @@ def test_gradient_against_differences(status_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,T,H,D,window,sinks", [(16, 1024, 12, 64, 256, 4), (2, 2048, 16, 128, 500, 4)])
+def test_many_blocks_per_processor(status_ok, B, T, H, D, window, sinks):
+    """Each multiprocessor walks many key blocks: dK and dV, summed in a fixed order, come out
+    in the same bits every time; dQ, summed by atomics, within a bf16 rounding; and all of
+    a head agrees with 64 bits."""
+    qkv, do = _inputs(B, T, H, D)
+    first = _run(qkv, do, B, T, H, D, window, sinks)
+    F = H * D
+    for _ in range(12):
+        o, grad = _run(qkv, do, B, T, H, D, window, sinks)
+        assert torch.equal(o, first[0])
+        assert torch.equal(grad[:, F:], first[1][:, F:])
+        # fp32 sums of at most 17 tiles in another order, then a rounding each: a step apart
+        off = (grad[:, :F].double() - first[1][:, :F].double()).abs()
+        assert (off <= 2.02 * HALF * first[1][:, :F].double().abs() + 1e-5).all()
+    heads = torch.arange(0, H, 5, device="cuda")
+    part = lambda t, n: t.view(B, T, n, H, D)[:, :, :, heads].reshape(B * T, -1)  # noqa: E731
+    o, o_err, want, err = oracle(part(qkv, 3), part(do, 1), B, T, len(heads), D, window, sinks)
+    within(part(first[0], 1), o, o_err)
+    within(part(first[1], 3), want, err)
+
+
+@pytest.mark.gpu
 def test_sequences_do_not_touch_each_other(status_ok):
     """A ragged last block reads zeros, not the next sequence (here infinities and NaN)."""
     B, T, H, D = 3, 130, 1, 64
