@@ -176,6 +176,13 @@ def test_refuses_settings(kw, match):
         F.sample(torch.zeros(2, 5), torch.zeros(2), **kw)
 
 
+def test_large_top_k_is_off():
+    """int64 values beyond 32 bits do not wrap round to small ones."""
+    x, u = torch.randn(3, 40), torch.rand(3)
+    k = torch.tensor([2**32 + 1, 2**31 + 7, -(2**32) + 2])
+    assert torch.equal(F.sample(x, u, top_k=k).torch(), F.sample(x, u).torch())
+
+
 def test_refuses_shapes_and_types():
     with pytest.raises(ValueError, match="uniform"):
         F.sample(torch.zeros(2, 5), torch.zeros(3))

@@ -261,6 +261,13 @@ def test_captured_and_replayed(status_ok):
         within(out[1], grad, grad_err)
 
 
+def test_refuses_cpu_tensors():
+    from underhfs_b200.ops.functions import flash_attention
+
+    with pytest.raises(RuntimeError, match="CUDA"):
+        flash_attention(torch.zeros(32, 192, dtype=torch.bfloat16), 1, 32, 1, 64, True, window=4)
+
+
 @pytest.mark.gpu
 def test_refusals():
     from underhfs_b200.ops import kernels as K

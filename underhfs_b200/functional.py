@@ -93,7 +93,10 @@ def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dty
             raise ValueError(f"{name} needs one value for each of {rows} rows, got {list(value.shape)}")
         if value.device != device:
             raise RuntimeError(f"{name} is on {value.device}, the logits on {device}")
-        return value.detach().reshape(-1).to(dtype).contiguous()
+        value = value.detach().reshape(-1)
+        if dtype == torch.int32 and value.dtype == torch.int64:
+            value = value.clamp(0, 2**31 - 1)  # <= 0 is off
+        return value.to(dtype).contiguous()
     if not low <= value <= high:  # False for NaN
         raise ValueError(f"{name} must lie in [{low:g}, {high:g}], got {value}")
     return int(value) if dtype == torch.int32 else float(value)

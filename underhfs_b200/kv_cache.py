@@ -77,7 +77,6 @@ class QuantizedKVCache:
             self.pages = torch.zeros((self.layers, self.batch, self.kv_heads, pages, 40 * self.head_dim),
                                      dtype=torch.uint8, device=self.device)
             self.device = self.pages.device
-            self._pages = list(self.pages)  # one view a layer: making one costs as much as a launch
         else:
             if self.head_dim < GROUP or self.head_dim % GROUP:
                 raise ValueError(f"head_dim must be a multiple of {GROUP}, got {head_dim}")
@@ -87,6 +86,16 @@ class QuantizedKVCache:
         self.lengths = torch.zeros((self.batch,), dtype=torch.int32, device=self.device)
         # the same as one host number while every advance was a host number; None once they differ
         self._host_length: int | None = 0
+
+    @property
+    def pages(self) -> torch.Tensor:
+        """CUDA: the codes, scales and minima, uint8 [layers, batch, kv_heads, pages, 40 head_dim]."""
+        return self._pages
+
+    @pages.setter
+    def pages(self, value: torch.Tensor) -> None:
+        self._pages = value
+        self._layer_pages = list(value)  # making a view costs as much as a launch
 
     @property
     def nbytes(self) -> int:
@@ -163,7 +172,7 @@ class QuantizedKVCache:
             return
         if self._cuda:
             with self._on_device():
-                K.kv4_append(self._pages[layer], k, v, self.lengths, counts, self.max_len)
+                K.kv4_append(self._layer_pages[layer], k, v, self.lengths, counts, self.max_len)
             return
         k, v = k.detach(), v.detach()
         for b in range(self.batch):
@@ -199,7 +208,7 @@ class QuantizedKVCache:
             if tokens == 0:
                 return torch.empty_like(q)
             with self._on_device():
-                return K.kv4_attend(self._pages[layer], q, self.lengths, counts, self.max_len, scale, window, sinks)
+                return K.kv4_attend(self._layer_pages[layer], q, self.lengths, counts, self.max_len, scale, window, sinks)
         q = q.detach()
         out = torch.zeros(q.shape, dtype=torch.float64)
         for b in range(self.batch):
@@ -227,7 +236,7 @@ class QuantizedKVCache:
             if dtype == torch.float64:
                 raise TypeError("the CUDA cache reads as fp32, fp16 or bf16")
             with self._on_device():
-                return K.kv4_read(self._pages[layer], start, count, self.head_dim, dtype)
+                return K.kv4_read(self._layer_pages[layer], start, count, self.head_dim, dtype)
         return tuple(x[layer, :, start : start + count].to(dtype) for x in (self._k, self._v))
 
     def advance(self, tokens) -> None:

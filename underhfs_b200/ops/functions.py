@@ -283,6 +283,11 @@ def flash_attention(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: b
             raise ValueError("windowed attention takes bf16 q/k/v with head_dim 64 or 128")
         if tuple(qkv.shape) != (B * T, 3 * H * D):
             raise ValueError(f"qkv must be [{B * T}, {3 * H * D}], got {list(qkv.shape)}")
+        if not qkv.is_cuda:
+            raise RuntimeError(f"windowed attention runs on CUDA tensors, got one on {qkv.device}")
+        if qkv.device.index != torch._C._cuda_getDevice():
+            with torch.cuda.device(qkv.device):
+                return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal, window, sinks)
     return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal, window, sinks)
 
 
