@@ -93,6 +93,8 @@ def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dty
             raise ValueError(f"{name} needs one value for each of {rows} rows, got {list(value.shape)}")
         if value.device != device:
             raise RuntimeError(f"{name} is on {value.device}, the logits on {device}")
+        if value.dtype == dtype and value.dim() == 1 and value.is_contiguous():
+            return value
         value = value.detach().reshape(-1)
         if dtype == torch.int32 and value.dtype == torch.int64:
             value = value.clamp(0, 2**31 - 1)  # <= 0 is off

@@ -129,6 +129,8 @@ class QuantizedKVCache:
             raise TypeError(f"counts must be int32 or int64, got {counts.dtype}")
         if counts.device != self.device:
             raise RuntimeError(f"counts are on {counts.device}, the cache on {self.device}")
+        if counts.dtype == torch.int32 and counts.is_contiguous():
+            return counts
         return counts.to(torch.int32).contiguous()
 
     def _check_rows(self, t, name: str, heads: int | None) -> torch.Tensor:
@@ -161,14 +163,17 @@ class QuantizedKVCache:
         held on the device are checked there: tokens past ``max_len`` are left
         out and reported in the device status word."""
         self._check_layer(layer)
-        k, v = self._check_rows(k, "k", self.kv_heads), self._check_rows(v, "v", self.kv_heads)
+        k, v = self._check_rows(k, "k", self.kv_heads), _raw(v)
+        tokens = k.shape[1]
         if k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError(f"k and v differ: {list(k.shape)} {k.dtype}, {list(v.shape)} {v.dtype}")
+        if v.device != self.device:
+            raise RuntimeError(f"v is on {v.device}, the cache on {self.device}")
         if counts is not None:
             counts = self._check_counts(counts)
         else:
-            self._check_room(k.shape[1])
-        if k.shape[1] == 0:
+            self._check_room(tokens)
+        if tokens == 0:
             return
         if self._cuda:
             with self._on_device():

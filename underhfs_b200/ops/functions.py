@@ -287,7 +287,9 @@ def flash_attention(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: b
             raise RuntimeError(f"windowed attention runs on CUDA tensors, got one on {qkv.device}")
         if qkv.device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(qkv.device):
-                return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal, window, sinks)
+                return flash_attention(qkv, B, T, H, D, causal, window, sinks)
+    if not (qkv.requires_grad and torch.is_grad_enabled()):  # no graph to build: half the host's time
+        return K.flash_attn_qkv(qkv.contiguous(), B, T, H, D, causal, window=window, sinks=sinks)[0]
     return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal, window, sinks)
 
 

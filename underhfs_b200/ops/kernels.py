@@ -381,13 +381,15 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature, top_
 
 
 # ------------------------------------------------- 4-bit key / value cache
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """`t` [B, T, H, D] itself where the cache kernels can read its rows in
-    16-byte pieces (D contiguous, strides and start aligned), else a copy."""
-    b, n, h, d = t.stride()
-    if d == 1 and (t.data_ptr() | ((b | n | h) * t.element_size())) % 16 == 0 and max(n, h) < 1 << 31:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows16(t: torch.Tensor):
+    """(tensor, address, strides) of `t` [B, T, H, D], or of a copy where the cache
+    kernels cannot read its rows in 16-byte pieces (D contiguous, strides and start aligned)."""
+    stride, at = t.stride(), t.data_ptr()
+    b, n, h, d = stride
+    if d != 1 or (at | (b | n | h) * t.element_size()) & 15 or n >= 1 << 31 or h >= 1 << 31:
+        t = t.clone(memory_format=torch.contiguous_format)
+        stride, at = t.stride(), t.data_ptr()
+    return t, at, stride
 
 
 def kv4_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor,
@@ -396,8 +398,8 @@ def kv4_append(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: t
     sequence's `lengths` tokens (one launch); only the first counts[b] tokens
     of sequence b are written."""
     B, T, H, D = k.shape
-    k, v = _rows16(k), _rows16(v)
-    core().kv4_append(dt(k), D, ptr(k), k.stride(), ptr(v), v.stride(), ptr(pages), ptr(lengths),
+    (k, k_at, k_stride), (v, v_at, v_stride) = _rows16(k), _rows16(v)
+    core().kv4_append(dt(k), D, k_at, k_stride, v_at, v_stride, pages.data_ptr(), lengths.data_ptr(),
                       ptr(counts), B, T, H, pages.shape[2], capacity, stream())
 
 
@@ -415,10 +417,11 @@ def kv4_attend(pages: torch.Tensor, q: torch.Tensor, lengths: torch.Tensor, coun
     """Attention of the new tokens' q [B, Tq, Hq, D] (bf16 or fp16) over `pages`
     (one launch): token t of sequence b sees the cache up to lengths[b] + t."""
     B, Tq, Hq, D = q.shape
-    q = _rows16(q)
+    q, q_at, q_stride = _rows16(q)
     o = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
-    core().kv4_attend(dt(q), D, ptr(q), q.stride(), ptr(pages), ptr(o), ptr(lengths), ptr(counts), B, Tq,
-                      Hq, pages.shape[1], pages.shape[2], capacity, float(scale), window, sinks, stream())
+    _, Hkv, P, _ = pages.shape
+    core().kv4_attend(dt(q), D, q_at, q_stride, pages.data_ptr(), o.data_ptr(), lengths.data_ptr(), ptr(counts), B,
+                      Tq, Hq, Hkv, P, capacity, scale, window, sinks, stream())
     return o
 
 
