@@ -110,6 +110,13 @@ __device__ __noinline__ uint32_t quantize8_exact(float4 x0, float4 x1, float lo,
   return word;
 }
 
+// the largest of |a|, |b| and |c|, NaN if one is NaN
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // A group's lo and s (its values are those of four neighbouring threads) and this thread's codes.
 // Where every value is sure, within the codes' range and finite, the rounded product is the
 // code; about one in 2^11 values of a bf16 tensor is not (mostly ties), and its thread's eight go
@@ -126,15 +133,23 @@ __device__ __forceinline__ uint32_t quantize8(const float* x, float mn, float mx
   const float lo = __half2float(*lo_h);
   *s_h = __float2half_rn(fmaxf((hi - lo) * (1.f / 15.f), 0.f));
   const float s = __half2float(*s_h), inv = __fdividef(1.f, s);  // (s = 0: infinite, and nothing is sure)
-  uint32_t word = 0;
   bool sure = (mn - lo) * inv > -kSure && (mx - lo) * inv < 15.f + kSure;
+  // pairs of codes i and i + 4, as packed fp32
+  auto both = [](float y) { return make_float2(y, y); };
+  float2 n[4];  // minus the codes
+  float off = 0.f;  // the farthest of the quotients from its code
 #pragma unroll
-  for (int i = 7; i >= 0; --i) {
-    const float d = x[i] - lo, z = fmaf(d, inv, kMagic);
-    sure = sure && fabsf(fmaf(d, inv, kMagic - z)) < kSure;  // (NaN and infinities are not)
-    word = word * 16u + __float_as_uint(z);                 // (their constant is taken off below)
+  for (int i = 0; i < 4; ++i) {
+    const float2 d = f2_add(make_float2(x[i], x[i + 4]), both(-lo));
+    n[i] = f2_fma(f2_fma(d, both(inv), both(kMagic)), both(-1.f), both(kMagic));
+    const float2 e = f2_fma(d, both(inv), n[i]);
+    off = max3_abs_nan(off, e.x, e.y);  // (NaN and infinities are not sure)
   }
-  word -= 0x4B400000u * 0x11111111u;
+  sure = sure && off < kSure;
+  // the sums of four codes times powers of 16 are exact
+  const float2 m = f2_fma(f2_fma(f2_fma(n[3], both(16.f), n[2]), both(16.f), n[1]), both(16.f), n[0]);
+  const float2 z = f2_fma(m, both(-1.f), both(kMagic));
+  uint32_t word = __byte_perm(__float_as_uint(z.x), __float_as_uint(z.y), 0x5410);
   if (!sure)
     word = quantize8_exact(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), lo, s);
   return word;
@@ -174,7 +189,7 @@ struct Raw8 {
 };
 
 template <int D, typename T, int kRows>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4Append a) {
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4Append a) {
   using F = Kv4<D>;
   constexpr int LPR = D / 8;  // threads per row
   const Place<D> pl = place<D, kRows>(a.H);
