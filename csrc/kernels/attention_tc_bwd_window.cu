@@ -14,10 +14,12 @@
 // Measured with the sums before and the conversion after it (28 us of 16 x 1024), against
 // 175 and 484 us of a CTA per item with every product waiting for the one before:
 //   16 x 1024 tokens, 12 x 64, window 256, 4 sinks     155 us, about 6 K cycles a step
-//   2 x 4096 tokens, 16 x 128, window 1024, 4 sinks    280 us, about 6.4 K cycles a step
+//   2 x 4096 tokens, 16 x 128, window 1024, 4 sinks    268 us, about 6 K cycles a step
 // A step's five products are 1.3 K (D = 64) and 2.6 K cycles of the tensor core; what bounds
-// it is the chain S -> P -> dS -> dQ of a step, of which two steps do not fit in TMEM, and
-// the shared memory that the products, dS^T and the dQ boxes share.
+// it is the chain S -> P -> dS -> dQ of a step, of which two steps do not fit in TMEM (D = 128:
+// dV, then S^T in P^T's place, then its exponentials: 1.3, 1.2 and 2 K cycles), and the
+// shared memory that the products, dS^T and the dQ boxes share.  Measured without gain for
+// D = 128: dK before dQ, which frees Q earlier and dP^T later, and the next tiles brought to L2.
 //
 // Per step i (S^T etc. are 128 keys x 128 queries):
 //   MMA      S^T = K Q_i^T; dP^T = V dO_i^T; dV += P^T dO_i; dQ_i = dS K; dK += dS^T Q_i
@@ -64,9 +66,6 @@ constexpr int kCompute = 256;
 constexpr int kReadout = 128;
 constexpr int kThreads = 512;
 constexpr int kLaunchRegs = 128;
-constexpr int kComputeRegs = 184;
-constexpr int kServiceRegs = 72;
-static_assert(2 * 128 * kComputeRegs + 2 * 128 * kServiceRegs <= kThreads * kLaunchRegs, "register split");
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -76,6 +75,8 @@ struct WinCfg {
   static constexpr int kKV = kAlias ? 1 : 2;  // K / V buffers
   static constexpr int kNQ = kAlias ? 2 : 3, kNDO = kAlias ? 1 : 2;  // Q (with lse and delta) and dO stages
   static constexpr int kRing = 4;  // items handed out ahead
+  static constexpr int kComputeRegs = kAlias ? 160 : 184, kServiceRegs = kAlias ? 96 : 72;
+  static_assert(2 * 128 * kComputeRegs + 2 * 128 * kServiceRegs <= kThreads * kLaunchRegs, "register split");
   static constexpr int kDST = BK * BQ * 2;
   static constexpr int kBox = 128 * 32 * 4;  // fp32 dQ box: 128 rows x 32 columns
   static constexpr int kVec = 2 * kNQ * BQ * 4;
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kServiceRegs));
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kServiceRegs));
   if (warp == kProducerWarp || warp == kProducerWarp2) {
     // ------------------------------------------------------------ producers: K, V, Q, lse, delta; dO
     uint32_t k = 0;  // items of this CTA so far
@@ -263,15 +264,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t gq = 0, gd = 0;  // Q and dO tiles issued
     auto load_q = [&](const Item& w, int t) {
       const uint32_t st = gq % NQ;
-      if (!wait(&q_empty[st], ((gq / NQ) & 1u) ^ 1u, 400)) return false;
       const int q0 = (w.i_start() + t) * BQ;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&q_full[st], Cfg::kTile);
-        for (int kd = 0; kd < KD; ++kd)
-          tma_load_3d(sQ + st * Cfg::kTile + kd * (BQ * 128), &tm_qkv, &q_full[st], w.h * D + kd * 64, q0, w.b);
-      }
       // lse and delta share Q's stage: it is given back after dK, for which every warp has used both
-      // (dV, which frees the dO stage, does not wait for delta's readers)
+      // (dV, which frees the dO stage, does not wait for delta's readers).  They are read before
+      // the stage is free.
       float v[BQ / 32], u[BQ / 32];
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) {
@@ -279,6 +275,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const long long at = ((long long)w.b * a.H + w.h) * T + qq;
         v[i] = qq < T ? __ldg(a.lse + at) : INFINITY;
         u[i] = qq < T ? __ldg(a.delta + at) : 0.f;
+      }
+      if (!wait(&q_empty[st], ((gq / NQ) & 1u) ^ 1u, 400)) return false;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&q_full[st], Cfg::kTile);
+        for (int kd = 0; kd < KD; ++kd)
+          tma_load_3d(sQ + st * Cfg::kTile + kd * (BQ * 128), &tm_qkv, &q_full[st], w.h * D + kd * 64, q0, w.b);
       }
 #pragma unroll
       for (int i = 0; i < BQ / 32; ++i) {
@@ -480,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait_bounded(done, 0, a.status, kErrWaitTimeoutAccum, 420);
     }
   } else if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kComputeRegs));
     // ------------------------------------------------------------ compute
     const int quarter = warp & 3, half = warp >> 2;
     const int r = quarter * 32 + lane;  // key row
@@ -699,6 +701,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lb = tmem + ((uint32_t)(quarter * 32) << 16);
     const bool leader = warp == 12 && lane == 0;  // issues the TMA reductions
     uint32_t g = 0, chunk = 0;
+    // Columns held in registers at once, in 32s.  Aliased, dP^T of the next step waits until dQ has left
+    // TMEM, which then does not wait for the first half's boxes (280 -> 268 us of 2 x 4096,
+    // 16 x 128); with D = 64 nothing waits for it, and the compute warps can use the registers.
+    constexpr int kHeld = Cfg::kAlias ? 2 : 1;
     bool ok = true;  // per warp; the named barriers are met in any case
     for (uint32_t k = 0;; ++k) {
       const Item w = take_group(k, 443, warp == 12, sGroup + 8, 1, kReadout);
@@ -706,30 +712,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < w.steps; ++t, ++g) {
         if (ok && !mbar_wait_warp(dq_full, g & 1u, a.status, kErrWaitTimeoutAccum, 440)) ok = false;
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c, ++chunk) {
-          uint32_t v[32];
+        for (int c = 0; c < D / (32 * kHeld); ++c, ++chunk) {
+          uint32_t v[kHeld][32];
+#pragma unroll
+          for (int u = 0; u < kHeld; ++u)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[u][i] = 0u;
           if (ok) {
             tc_fence_after();
-            tmem_ld_32x32b_x32_async(lb + Cfg::kDQ + c * 32, v);
-            tmem_wait_ld_regs<32>(v);
-            if (c == D / 32 - 1) {
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) tmem_ld_32x32b_x32_async(lb + Cfg::kDQ + (c * kHeld + u) * 32, v[u]);
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u) tmem_wait_ld_regs<32>(v[u]);
+            if (c == D / (32 * kHeld) - 1) {
               tc_fence_before();
               warp_arrive(dq_free);
             }
           }
-          uint8_t* box = sBox + (chunk & 1) * Cfg::kBox;
-          if (leader) bulk_wait_group_read1();  // the reduction that last used this box has read it
+          uint8_t* box = sBox + (kHeld == 1 ? (chunk & 1) * Cfg::kBox : 0);
+          if (leader) {  // the reductions that last used the box(es) have read them
+            if constexpr (kHeld == 1) bulk_wait_group_read1();
+            else bulk_wait_group_read0();
+          }
           named_barrier_sync(1, kReadout);
           if (ok) {
 #pragma unroll
-            for (int ch = 0; ch < 8; ++ch)
-              *reinterpret_cast<uint4*>(box + r * 128 + ((ch ^ (r & 7)) << 4)) =
-                  make_uint4(v[ch * 4], v[ch * 4 + 1], v[ch * 4 + 2], v[ch * 4 + 3]);
+            for (int u = 0; u < kHeld; ++u)
+#pragma unroll
+              for (int ch = 0; ch < 8; ++ch)
+                *reinterpret_cast<uint4*>(box + u * Cfg::kBox + r * 128 + ((ch ^ (r & 7)) << 4)) =
+                    make_uint4(v[u][ch * 4], v[u][ch * 4 + 1], v[u][ch * 4 + 2], v[u][ch * 4 + 3]);
             fence_proxy_async_smem();
           }
           named_barrier_sync(1, kReadout);
           if (leader && ok) {
-            tma_reduce_add_3d(&tm_dq, box, w.h * D + c * 32, (w.i_start() + t) * BQ, w.b);
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u)
+              tma_reduce_add_3d(&tm_dq, box + u * Cfg::kBox, w.h * D + (c * kHeld + u) * 32, (w.i_start() + t) * BQ, w.b);
             bulk_commit_group();
           }
         }
