@@ -24,13 +24,15 @@
 // 2^-29 of itself (fp32 pairs for the exponent, a table of 64 powers, a short series;
 // tests/test_sampling.py restates the steps), so that a sum over n tokens of like
 // weight is right to about 2^-29 / sqrt(n) and the choice is that of exact arithmetic
-// but for u in a few parts in 10^8.  In 64-bit floating point the weights took 1.5 to 2
-// times as long.  For top-p's border they are rounded to 2^-31, so that a histogram holds
-// its sums as two 32-bit words of 16 bits of the weights each (32-bit adds are what
-// shared memory does fast, and they bound a flat row's pass: three words took a third more).
+// but for u in a few parts in 10^8.  (With the weights in 64-bit floating point 256 x 32000 of
+// mixed settings took 58 us where these took 46.)  For top-p's border they are rounded to
+// 2^-31, so that a histogram holds its sums as two 32-bit words of 16 bits of the weights
+// each: 32-bit adds are what shared memory does fast, and they bound a flat row's pass.
 //
-// Bound by latency for a few rows (a cluster joins its blocks three times, about 1 us
-// each), by the instructions of the weights for many.
+// Measured: 1 x 32000 bf16 with top-p 16 us (bound by the barriers of the cluster, about 2 K
+// cycles each), 256 x 32000 bf16 of mixed settings 44, 64 x 131072 fp32 with top-p 85 (0.4 TB/s:
+// bound by the instructions of the weights and the histogram's atomics, with 16 to 32 warps
+// an SM).
 #include <cfloat>
 #include <stdexcept>
 #include <string>
@@ -798,13 +800,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 
 template <typename T>
 void launch_sample(SampleArgs a, cudaStream_t s) {
-  // Blocks per row: as many as fit the GPU at once, two on each SM, when rows are few, and
-  // as many as it takes to hold the row in 64 KB of each (then two blocks fit an SM).
+  // Blocks per row: while they fit the GPU, one on each SM, when rows are few, and as many as
+  // it takes to hold the row in 64 KB of each (then two blocks fit an SM).  Eight only for
+  // up to 8 rows (clusters of eight wait for room: 16 x 32000 took 21 us, with four 18; one row 15.5
+  // and 16.6), two on each SM no more (128 x 32000: 31 us, with one block a row 29), and at least
+  // 4096 tokens to a block (1 x 4000: 14.5 us with two, 11 with one).
   const int tile = kWarps * 8;
   int splits = 1;
   while (splits < kMaxSplits &&
-         ((long long)a.rows * splits * 2 <= 2 * 148 || (long long)a.vocab * (int)sizeof(T) > splits * 65536ll) &&
-         (long long)a.vocab > (long long)splits * kThreads * 4)
+         ((long long)a.rows * splits * 2 <= (splits < 4 ? 148 : 64) ||
+          (long long)a.vocab * (int)sizeof(T) > splits * 65536ll) &&
+         (long long)a.vocab > (long long)splits * kThreads * 8)
     splits *= 2;
   a.splits = splits;
   a.warp_len = (int)(((long long)a.vocab + (long long)splits * tile - 1) / ((long long)splits * tile)) * 8;
