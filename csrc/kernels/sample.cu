@@ -306,31 +306,31 @@ struct Sampler {
       }
     }
     if (decide) {
-    u64 incl = v[0] + v[1];
+      u64 incl = v[0] + v[1];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    if (lane == 31) sh.warp_sum[warp] = incl;
-    __syncthreads();
-    u64 before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += sh.warp_sum[w];
-      total += sh.warp_sum[w];
-    }
-    const u64 goal = goal_of(total);
-    u64 excl = before + incl - v[0] - v[1];
-    if (threadIdx.x == 0) sh.goal = goal;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (excl < goal && excl + v[i] >= goal) {
-        sh.bin = threadIdx.x * 2 + i;
-        sh.excl = excl;
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
       }
-      excl += v[i];
-    }
+      if (lane == 31) sh.warp_sum[warp] = incl;
+      __syncthreads();
+      u64 before = 0, total = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sh.warp_sum[w];
+        total += sh.warp_sum[w];
+      }
+      const u64 goal = goal_of(total);
+      u64 excl = before + incl - v[0] - v[1];
+      if (threadIdx.x == 0) sh.goal = goal;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (excl < goal && excl + v[i] >= goal) {
+          sh.bin = threadIdx.x * 2 + i;
+          sh.excl = excl;
+        }
+        excl += v[i];
+      }
     }
     if (splits == 1) {
       __syncthreads();
