@@ -1,11 +1,12 @@
 // Next-token sampling: temperature, top-k, top-p, min-p and the choice by a given
-// uniform number, without a sort, with one read of the logits.
+// uniform number, without a sort, with one read of the logits from memory.
 //
 // Tokens are ordered by (logit, lowest index first); top-k, top-p and min-p each
 // keep a prefix of that order, so the kept set is "at or before one token", found
 // as follows, and the choice walks the vocabulary in index order:
 //   1. the row goes to shared memory (one block, or a cluster whose blocks each hold
-//      a slice); maximum and minimum;
+//      a slice; wide rows that would take several waves of blocks so are read again from
+//      L2 instead); maximum and minimum;
 //   2. top-k of at most kShortK: the k-th largest of the threads' own maxima bounds the
 //      k-th logit from below, so one pass lists little more than k tokens, and one block
 //      goes on over the list;
@@ -30,9 +31,8 @@
 // each: 32-bit adds are what shared memory does fast, and they bound a flat row's pass.
 //
 // Measured: 1 x 32000 bf16 with top-p 16 us (bound by the barriers of the cluster, about 2 K
-// cycles each), 256 x 32000 bf16 of mixed settings 44, 64 x 131072 fp32 with top-p 85 (0.4 TB/s:
-// bound by the instructions of the weights and the histogram's atomics, with 16 to 32 warps
-// an SM).
+// cycles each), 256 x 32000 bf16 of mixed settings 44, 64 x 131072 fp32 with top-p 70 (0.5 TB/s:
+// bound by the instructions of the weights and the histogram's atomics, with 32 warps an SM).
 #include <cfloat>
 #include <stdexcept>
 #include <string>
@@ -172,10 +172,14 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
   return v;
 }
 
-template <typename T>
+// kSlice: the block's part of the row is in shared memory; else it is read again from memory (L2)
+template <typename T, bool kSlice>
 struct Sampler {
   Shared& sh;
-  const T* slice;       // this block's part of the row in shared memory
+  const T* slice;       // this block's part of the row
+  int vocab;
+  bool vec;             // whether the row can be read in 16-byte pieces
+  bool infinite;        // some logits are infinite (only without a slice, whose values are replaced)
   int base;             // index of its first token
   int w_len;            // tokens per warp, a multiple of 8
   int splits;           // blocks that hold the tokens: 1 once they are listed
@@ -190,6 +194,32 @@ struct Sampler {
     else __syncthreads();
   }
 
+  // eight logits of the block's part, -inf for NaN and past the end
+  __device__ __forceinline__ void fetch(const T* at, float* l) const {
+    if constexpr (kSlice) {
+      load8<T>(at, l);
+    } else {
+      const int left = vocab - (base + (int)(at - slice));
+      if (vec && left >= 8) {
+        load8<T>(at, l);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l[i] = i < left ? to_float<T>(at[i]) : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) l[i] = fmaxf(l[i], -INFINITY);  // (drops NaN)
+      if (infinite) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l[i] = l[i] == INFINITY ? 0.f : -INFINITY;
+      }
+    }
+  }
+  // one of those within the vocabulary that is not NaN
+  __device__ __forceinline__ float fetch_one(const T* at) const {
+    const float l = to_float<T>(*at);
+    return !kSlice && infinite ? (l == INFINITY ? 0.f : -INFINITY) : l;
+  }
+
   // f(logit, index) for the listed tokens, or this warp's and, as -inf, the padding behind them
   template <class Fn>
   __device__ __forceinline__ void each(Fn&& f) const {
@@ -201,7 +231,7 @@ struct Sampler {
     const T* part = slice + warp * w_len;
     for (int v = lane * 8; v < w_len; v += 256) {
       float l[8];
-      load8<T>(part + v, l);
+      fetch(part + v, l);
 #pragma unroll
       for (int i = 0; i < 8; ++i) f(l[i], base + warp * w_len + v + i);
     }
@@ -214,7 +244,7 @@ struct Sampler {
     const T* part = slice + warp * w_len;
     for (int v = lane * 8; v < w_len; v += 256) {
       float l[8];
-      load8<T>(part + v, l);
+      fetch(part + v, l);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) f(l[i], l[i + 1], base + warp * w_len + v + i);
     }
@@ -388,7 +418,7 @@ struct Sampler {
     const T* part = slice + warp * w_len;
     for (int v = lane * 8; v < w_len; v += 256) {
       float l[8];
-      load8<T>(part + v, l);
+      fetch(part + v, l);
       const int idx = base + warp * w_len + v;
       uint32_t mask = 0;
 #pragma unroll
@@ -398,7 +428,7 @@ struct Sampler {
       while (mask != 0) {
         const int i = __ffs(mask) - 1;
         mask &= mask - 1;
-        append(to_float<T>(part[v + i]), idx + i);
+        append(fetch_one(part + v + i), idx + i);
       }
     }
   }
@@ -515,7 +545,7 @@ __device__ __forceinline__ u64 choice(float u, u64 total) {
   return goal < total ? goal : total - 1;
 }
 
-template <typename T>
+template <typename T, bool kSlice>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
@@ -523,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   u64* long_list = reinterpret_cast<u64*>(smem_raw + sizeof(Shared));
   u64* compare = long_list + long_cap;  // (with more than one block)
   u64* cluster_list = splits > 1 ? compare + kCap : compare;
-  T* slice = reinterpret_cast<T*>(cluster_list);
+  T* slice = reinterpret_cast<T*>(cluster_list);  // (kSlice)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits;
   const long long r = blockIdx.x / splits;
@@ -543,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         mn = fminf(mn, l[i]);
       }
     }
-    store8<T>(slice + v, l);
+    if constexpr (kSlice) store8<T>(slice + v, l);
   };
   int v = threadIdx.x * 8;
   constexpr int kStep = kThreads * 8;
@@ -601,7 +631,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
       mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     }
   }
-  Sampler<T> s{sh, slice, base, w_len, splits, compare, Row{}, 0.f, nullptr, 0};
+  Sampler<T, kSlice> s{sh,    kSlice ? slice : src + base, a.vocab, a.vec != 0, false, base, w_len, splits, compare,
+                       Row{}, 0.f, nullptr, 0};
 
   const double temp = a.temperature_rows != nullptr ? (double)a.temperature_rows[r] : a.temperature;
   const int top_k = a.top_k_rows != nullptr ? a.top_k_rows[r] : a.top_k;
@@ -633,11 +664,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   float largest = own;
   if (mx == INFINITY) {
     // infinite logits have all the weight, alike: 0 in their place, -inf in the others'
-    __syncthreads();
-    T* part = slice + warp * w_len;
-    for (int i = lane; i < w_len; i += 32)
-      part[i] = from_float<T>(to_float<T>(part[i]) == INFINITY ? 0.f : -INFINITY);
-    __syncthreads();
+    if constexpr (kSlice) {
+      __syncthreads();
+      T* part = slice + warp * w_len;
+      for (int i = lane; i < w_len; i += 32)
+        part[i] = from_float<T>(to_float<T>(part[i]) == INFINITY ? 0.f : -INFINITY);
+      __syncthreads();
+    } else {
+      s.infinite = true;
+    }
     largest = own == INFINITY ? 0.f : -INFINITY;
     mx = mn = 0.f;
   }
@@ -763,14 +798,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   __syncthreads();
   if (sh.bin >= 0) {
     // this block has the token: its warps take 256 tokens each of that warp's part
-    const T* part = slice + sh.bin * w_len;
+    const T* part = s.slice + sh.bin * w_len;
     const int v = (int)threadIdx.x * 8, idx = base + sh.bin * w_len + v;
     u64 w[8], mine = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 0;
     if (v < w_len) {
       float l[8];
-      load8<T>(part + v, l);
+      s.fetch(part + v, l);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         w[i] = kept(l[i], idx + i);
@@ -798,20 +833,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
   if (splits > 1) cluster_sync_all();  // no block leaves while its sums are read
 }
 
-template <typename T>
-void launch_sample(SampleArgs a, cudaStream_t s) {
-  // Blocks per row: while they fit the GPU, one on each SM, when rows are few, and as many as
-  // it takes to hold the row in 64 KB of each (then two blocks fit an SM).  Eight only for
-  // up to 8 rows (clusters of eight wait for room: 16 x 32000 took 21 us, with four 18; one row 15.5
-  // and 16.6), two on each SM no more (128 x 32000: 31 us, with one block a row 29), and at least
-  // 4096 tokens to a block (1 x 4000: 14.5 us with two, 11 with one).
+template <typename T, bool kSlice>
+void launch_splits(SampleArgs a, int splits, cudaStream_t s) {
   const int tile = kWarps * 8;
-  int splits = 1;
-  while (splits < kMaxSplits &&
-         ((long long)a.rows * splits * 2 <= (splits < 4 ? 148 : 64) ||
-          (long long)a.vocab * (int)sizeof(T) > splits * 65536ll) &&
-         (long long)a.vocab > (long long)splits * kThreads * 8)
-    splits *= 2;
   a.splits = splits;
   a.warp_len = (int)(((long long)a.vocab + (long long)splits * tile - 1) / ((long long)splits * tile)) * 8;
   if (a.warp_len > kThreads * 8) throw std::runtime_error("sample: the vocabulary is too large");
@@ -819,7 +843,7 @@ void launch_sample(SampleArgs a, cudaStream_t s) {
   a.long_cap = 2048;
   size_t smem;
   while (true) {  // a large vocabulary leaves less room (none is right too: the slices are used)
-    const size_t own = (size_t)a.warp_len * kWarps * sizeof(T), list = (size_t)a.long_cap * sizeof(u64);
+    const size_t own = kSlice ? (size_t)a.warp_len * kWarps * sizeof(T) : 0, list = (size_t)a.long_cap * sizeof(u64);
     smem = sizeof(Shared) + list + (splits > 1 ? kCap * sizeof(u64) + (own > list ? own : list) : own);
     if (smem <= kMaxSmem || a.long_cap == 0) break;
     a.long_cap = a.long_cap > 256 ? a.long_cap / 2 : 0;
@@ -827,7 +851,8 @@ void launch_sample(SampleArgs a, cudaStream_t s) {
   if (smem > kMaxSmem) throw std::runtime_error("sample: the vocabulary does not fit the shared memory of 8 blocks");
   static PerDeviceOnce once;
   once([] {
-    UHFS_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem));
+    UHFS_CUDA_CHECK(
+        cudaFuncSetAttribute(sample_kernel<T, kSlice>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem));
   });
   if ((long long)a.rows * splits > 0x7fffffffll) throw std::runtime_error("sample: too many rows");
   cudaLaunchConfig_t cfg{};
@@ -841,8 +866,33 @@ void launch_sample(SampleArgs a, cudaStream_t s) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = splits > 1 ? 1 : 0;
-  UHFS_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, (const SampleArgs)a));
+  UHFS_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sample_kernel<T, kSlice>, (const SampleArgs)a));
   note_launch();
+}
+
+template <typename T>
+void launch_sample(const SampleArgs& a, cudaStream_t s) {
+  // Blocks per row: while they fit the GPU, one on each SM, when rows are few, and as many as
+  // it takes to hold the row in 64 KB of each (then two blocks fit an SM).  Eight only for
+  // up to 8 rows (clusters of eight wait for room: 16 x 32000 took 21 us, with four 18; one row 15.5
+  // and 16.6), two on each SM no more (128 x 32000: 31 us, with one block a row 29), and at least
+  // 4096 tokens to a block (1 x 4000: 14.5 us with two, 11 with one).
+  const long long rows = a.rows, vocab = a.vocab;
+  int splits = 1;
+  while (splits < kMaxSplits &&
+         (rows * splits * 2 <= (splits < 4 ? 148 : 64) || vocab * (int)sizeof(T) > splits * 65536ll) &&
+         vocab > (long long)splits * kThreads * 8)
+    splits *= 2;
+  if (rows * splits > 2 * 148) {
+    // More blocks than run at once: fewer that read the row again from L2 instead of keeping it (2^16
+    // tokens to a block at most), where these are three quarters of what runs at once.  64 x 131072
+    // fp32: 64 us, 79 with slices; 256 x 50000 fp32: 80 and 122; 512 x 32000 fp32, top-k 50: 46 and
+    // 74; 100 x 131072 bf16, whose 200 blocks leave half the SMs one: 104 and 87.
+    int few = 1;
+    while (few < kMaxSplits && (rows * few * 2 <= 2 * 148 || vocab > few * 65536ll)) few *= 2;
+    if (few < splits && rows * few * 4 >= 2 * 148 * 3) return launch_splits<T, false>(a, few, s);
+  }
+  launch_splits<T, true>(a, splits, s);
 }
 
 }  // namespace

@@ -285,6 +285,33 @@ def test_gpu_same_choice_however_the_row_is_split(status_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(t=0.0), dict(k=30, p=0.9), dict(k=5000), dict(p=0.95, m=0.01), dict(t=30.0, p=0.999)])
+@pytest.mark.parametrize("n,vocab,dtype", [(230, 20001, torch.float32), (224, 17000, torch.float32),
+                                           (60, 70002, torch.float32), (64, 70000, torch.float32),
+                                           (240, 40001, torch.bfloat16)])
+def test_gpu_many_wide_rows(n, vocab, dtype, kw, status_ok):
+    """Rows that the kernel reads again instead of keeping them: the reference's choice, and that of
+    each row by itself, with infinities, NaN, long runs and rows of one kind among them."""
+    x, u = rows(n, vocab, vocab, dtype)
+    x[1] = -INF
+    x[2, 5:] = -INF
+    x[3] = 0.5
+    x[4, ::3] = float("nan")
+    x[5] = float("nan")
+    x[6, 7::1000] = INF
+    x[7] = (x[7] * 2).round() / 2
+    x[8, : vocab // 2] = torch.finfo(dtype).min
+    got = F.sample(x.cuda(), u.cuda(), temperature=kw.get("t", 1.0), top_k=kw.get("k", 0), top_p=kw.get("p", 1.0),
+                   min_p=kw.get("m", 0.0)).torch().tolist()
+    for i in [*range(9), n // 2, n - 1]:
+        row = [float(v) if v == v else -INF for v in x[i]]
+        assert got[i] == reference(row, float(u[i]), **kw), i
+    for i in range(0, n, 3):
+        assert got[i] == F.sample(x[i : i + 1].cuda(), u[i : i + 1].cuda(), temperature=kw.get("t", 1.0),
+                                  top_k=kw.get("k", 0), top_p=kw.get("p", 1.0), min_p=kw.get("m", 0.0)).torch().item(), i
+
+
+@pytest.mark.gpu
 def test_gpu_captured_and_replayed_and_other_stream(status_ok):
     x, u = rows(4, 9000, 21)
     xd, ud = x.cuda(), u.cuda()
