@@ -261,6 +261,32 @@ def test_captured_and_replayed(status_ok):
         within(out[1], grad, grad_err)
 
 
+def test_forward_mode_is_refused(monkeypatch):
+    """There is no forward-mode rule: a dual tensor is refused, not passed on without its tangent."""
+    import torch.autograd.forward_ad as fwd
+
+    from underhfs_b200.ops import functions as OF
+
+    def plain(qkv, B, T, H, D, causal, scale=None, window=None, sinks=0):
+        q, k, v = qkv.view(B, T, 3, H, D).permute(2, 0, 3, 1, 4)
+        s = (q @ k.mT * D**-0.5).masked_fill(torch.ones(T, T).triu(1).bool(), float("-inf"))
+        return (s.softmax(-1) @ v).transpose(1, 2).reshape(B * T, H * D), None
+
+    monkeypatch.setattr(OF.K, "flash_attn_qkv", plain)
+    x = torch.randn(8, 3 * 64, generator=torch.Generator().manual_seed(0))
+    call = lambda t: OF.flash_attention(t, 1, 8, 1, 64, True)  # noqa: E731
+    want = call(x)
+    assert torch.equal(call(x.clone().requires_grad_(True)).detach(), want)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError):
+            call(fwd.make_dual(x, torch.ones_like(x)))
+        assert torch.equal(call(x), want)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(call, (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(call)(x.unsqueeze(0))
+
+
 def test_refuses_cpu_tensors():
     from underhfs_b200.ops.functions import flash_attention
 

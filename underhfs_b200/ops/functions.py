@@ -10,6 +10,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from underhfs_b200.ops import kernels as K
 
@@ -288,7 +289,10 @@ def flash_attention(qkv: torch.Tensor, B: int, T: int, H: int, D: int, causal: b
         if qkv.device.index != torch._C._cuda_getDevice():
             with torch.cuda.device(qkv.device):
                 return flash_attention(qkv, B, T, H, D, causal, window, sinks)
-    if not (qkv.requires_grad and torch.is_grad_enabled()):  # no graph to build: half the host's time
+    # no graph to build: half the host's time.  (A forward-mode tangent or a functorch transform goes
+    # through apply, which refuses it: the kernel's result would come without the tangent.)
+    if (not (qkv.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0
+            and not torch._C._are_functorch_transforms_active()):
         return K.flash_attn_qkv(qkv.contiguous(), B, T, H, D, causal, window=window, sinks=sinks)[0]
     return _FlashAttention.apply(qkv.contiguous(), B, T, H, D, causal, window, sinks)
 
