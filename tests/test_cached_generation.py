@@ -47,6 +47,39 @@ def test_cpu_ragged_prompts_match_single_ones():
             assert torch.allclose(g[b], w[0], rtol=0, atol=1e-12)
 
 
+def test_cpu_lengths_written_directly_are_seen():
+    """`lengths` is the caller's to write (to go back to an earlier state, say): what is kept is attended to."""
+    m = lm()
+    ids = torch.randint(0, 64, (1, 12), generator=torch.Generator().manual_seed(3))
+    cache = m.new_cache(max_len=20)
+    first = m.decode(ids[:, :9], cache)._data
+    held = cache.lengths.clone()
+    want = m.decode(ids[:, 9:10], cache)._data
+    cache.reset()
+    assert cache.is_empty
+    cache.lengths.copy_(held)
+    assert not cache.is_empty
+    assert torch.equal(m.decode(ids[:, 9:10], cache)._data, want)
+    cache.lengths.zero_()
+    assert cache.is_empty
+    assert torch.equal(m.decode(ids[:, :9], cache)._data, first)
+    cache.lengths = held * 0
+    assert cache.is_empty
+    cache.lengths = held.clone()
+    assert torch.equal(m.decode(ids[:, 9:10], cache)._data, want)
+
+
+def test_cpu_cache_made_in_inference_mode():
+    m = lm()
+    ids = torch.randint(0, 64, (1, 6), generator=torch.Generator().manual_seed(3))
+    with torch.inference_mode():
+        cache = m.new_cache(max_len=20)
+        m.decode(ids[:, :4], cache)
+        assert not cache.is_empty
+    m.decode(ids[:, 4:], cache)
+    assert cache.lengths.tolist() == [6]
+
+
 def test_generate_samples_and_defaults_to_greedy():
     m = lm()
     prompt = tensor([1, 2, 3])
@@ -212,6 +245,45 @@ def test_generate_graph_equals_eager_steps(kw, status_ok):
     # a second run on the same cache, and the uncached path still runs
     assert m.generate(tensor(prompt), n, cache=cache, uniform=u, **kw)._storage == got
     assert m.generate(tensor(prompt), 3, uniform=u[:3], **kw)._storage[: len(prompt) + 1] == got[: len(prompt) + 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prompt", [0, 20])
+def test_captured_steps_and_eager_ones_mix(prompt, status_ok):
+    """Steps captured on an empty cache, reset, replayed (after an eager prompt or from nothing) and
+    followed by eager calls: those see what the replays cached.  (The bounds are those of
+    test_engine_steps_stay_near_the_whole_context.)"""
+    kw = dict(vocab_size=512, max_seq_len=320, features=256, hidden_features=512, layers=3, heads=4, init="normal", seed=2)
+    gpu = TransformerLM(**kw).to("cuda", dtype="bf16")
+    ids = torch.randint(0, 512, (1, 64), generator=torch.Generator().manual_seed(6)).cuda()
+    with torch.no_grad():
+        full = gpu(ids)._data[0].double()
+    cache, token = gpu.new_cache(), ids[:, :1].clone()
+    gpu.decode(token, cache)  # (warm)
+    cache.reset()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gpu.decode(token, cache)._data
+    for _ in range(2):
+        cache.reset()
+        assert cache.is_empty
+        if prompt:
+            with torch.no_grad():
+                want = gpu(ids[:, :prompt])._data[0, -1]
+            assert torch.equal(gpu.decode(ids[:, :prompt], cache)._data[0], want)  # its own exact keys and values
+        for t in range(prompt, 40):
+            token.copy_(ids[:, t : t + 1])
+            graph.replay()
+            assert t == 0 or (out[0].double() - full[t]).norm() < 0.1 * full[t].norm()
+        assert not cache.is_empty
+        for t in (40, 41):
+            got = gpu.decode(ids[:, t : t + 1], cache)._data[0].double()
+            assert (got - full[t]).norm() < 0.1 * full[t].norm()
+        assert cache.lengths.tolist() == [42]
+    cache.set_host_length(42)
+    assert not cache.is_empty
+    with pytest.raises(ValueError, match="do not fit"):
+        gpu.decode(torch.zeros(1, 279, dtype=torch.int64), cache)
 
 
 @pytest.mark.gpu

@@ -70,22 +70,23 @@ class QuantizedKVCache:
         self._cuda = self.device.type == "cuda"
         self.layers, self.batch, self.kv_heads = int(layers), int(batch), int(kv_heads)
         self.head_dim, self.max_len = int(head_dim), int(max_len)
-        if self._cuda:
-            if self.head_dim not in (64, 128):
-                raise ValueError(f"the CUDA cache takes head_dim 64 or 128, got {head_dim}")
-            pages = (self.max_len + PAGE - 1) // PAGE
-            self.pages = torch.zeros((self.layers, self.batch, self.kv_heads, pages, 40 * self.head_dim),
-                                     dtype=torch.uint8, device=self.device)
-            self.device = self.pages.device
-        else:
-            if self.head_dim < GROUP or self.head_dim % GROUP:
-                raise ValueError(f"head_dim must be a multiple of {GROUP}, got {head_dim}")
-            self._k, self._v = (torch.zeros((self.layers, self.batch, self.max_len, self.kv_heads, self.head_dim),
-                                            dtype=torch.float64) for _ in range(2))
-        #: tokens of each sequence that ``advance`` has counted (int32, on the cache's device)
-        self.lengths = torch.zeros((self.batch,), dtype=torch.int32, device=self.device)
-        # the same as one host number while every advance was a host number; None once they differ
-        self._host_length: int | None = 0
+        if self._cuda and self.head_dim not in (64, 128):
+            raise ValueError(f"the CUDA cache takes head_dim 64 or 128, got {head_dim}")
+        if not self._cuda and (self.head_dim < GROUP or self.head_dim % GROUP):
+            raise ValueError(f"head_dim must be a multiple of {GROUP}, got {head_dim}")
+        with torch.inference_mode(False):  # inference tensors could not be written later, and count no versions
+            if self._cuda:
+                pages = (self.max_len + PAGE - 1) // PAGE
+                self.pages = torch.zeros((self.layers, self.batch, self.kv_heads, pages, 40 * self.head_dim),
+                                         dtype=torch.uint8, device=self.device)
+                self.device = self.pages.device
+            else:
+                self._k, self._v = (torch.zeros((self.layers, self.batch, self.max_len, self.kv_heads, self.head_dim),
+                                                dtype=torch.float64) for _ in range(2))
+            self.lengths = torch.zeros((self.batch,), dtype=torch.int32, device=self.device)
+        # A captured step changes the lengths at every replay, which the host does not see
+        self._captured = False
+        self._note(0)
 
     @property
     def pages(self) -> torch.Tensor:
@@ -98,6 +99,33 @@ class QuantizedKVCache:
         self._layer_pages = list(value)  # making a view costs as much as a launch
 
     @property
+    def lengths(self) -> torch.Tensor:
+        """Tokens of each sequence that ``advance`` has counted: int32 [batch], on the
+        cache's device.  It may be written to."""
+        return self._lengths
+
+    @lengths.setter
+    def lengths(self, value: torch.Tensor) -> None:
+        if value.shape != (self.batch,) or value.dtype != torch.int32 or value.device != self.device:
+            raise ValueError(f"lengths must be int32 [{self.batch}] on {self.device}, got {value.dtype} "
+                             f"{list(value.shape)} on {value.device}")
+        with torch.inference_mode(False):
+            self._lengths = value.clone() if value.is_inference() else value.contiguous()
+        self._version = -1
+
+    # What the host knows of the lengths: their common value, None where they differ.  It holds for
+    # one version of the tensor, so writes from outside are noticed.
+    def _note(self, length: int | None) -> None:
+        self._host_length = length
+        self._version = self._lengths._version
+
+    def _known(self) -> bool:
+        return not self._captured and self._version == self._lengths._version
+
+    def _capturing(self) -> bool:
+        return self._cuda and torch.cuda.is_current_stream_capturing()
+
+    @property
     def nbytes(self) -> int:
         """Device bytes of the keys and values."""
         if self._cuda:
@@ -106,8 +134,14 @@ class QuantizedKVCache:
 
     @property
     def is_empty(self) -> bool:
-        """No token has been counted since the start or the last ``reset``."""
-        return self._host_length == 0
+        """No sequence has a token.  Reads the lengths back where the host cannot know them: after
+        they were written to, or once a step with ``advance`` was captured.  False while
+        a step is captured, since it may be replayed on any lengths."""
+        if self._capturing():
+            return False
+        if self._known():
+            return self._host_length == 0
+        return not bool(self._lengths.any())
 
     # ------------------------------------------------------------- checks
     def _on_device(self):
@@ -149,7 +183,7 @@ class QuantizedKVCache:
         return t
 
     def _check_room(self, tokens: int) -> None:
-        used = self._host_length or 0
+        used = (self._host_length or 0) if self._known() else 0
         if used + tokens > self.max_len:
             raise ValueError(f"{tokens} more tokens do not fit: {used} of {self.max_len} are used")
 
@@ -250,26 +284,33 @@ class QuantizedKVCache:
             if tokens < 0:
                 raise ValueError(f"tokens must not be negative, got {tokens}")
             self._check_room(tokens)
-            with self._on_device():
-                self.lengths += tokens
-            if self._host_length is not None:
-                self._host_length += tokens
-            return
-        counts = self._check_counts(tokens)
+        else:
+            tokens = self._check_counts(tokens)
+        known = self._known()
         with self._on_device():
-            self.lengths += counts
-        self._host_length = None
+            self._lengths += tokens
+        if self._capturing():
+            self._captured = True  # replays count too
+        elif known and isinstance(tokens, int) and self._host_length is not None:
+            self._note(self._host_length + tokens)
+        elif known:
+            self._note(None)
 
     def set_host_length(self, tokens: int | None) -> None:
-        """Tell the host side how many tokens every sequence holds (None: not known)
-        after a captured graph has advanced the lengths on the device."""
-        self._host_length = tokens
+        """Tell the host side how many tokens every sequence holds (None: not all the same)
+        after a captured graph has advanced the lengths on the device.  From here on the cache
+        counts along again and reads nothing back: call it after the last replay."""
+        self._captured = False
+        self._note(tokens)
 
     def reset(self) -> None:
         """Forget every token (the memory is kept and written over)."""
         with self._on_device():
-            self.lengths.zero_()
-        self._host_length = 0
+            self._lengths.zero_()
+        if self._capturing():
+            self._captured = True
+        else:
+            self._note(0)
 
 
 __all__ = ["QuantizedKVCache", "quantize_groups", "GROUP", "PAGE", "RANGE"]
