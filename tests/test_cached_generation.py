@@ -80,6 +80,25 @@ def test_cpu_cache_made_in_inference_mode():
     assert cache.lengths.tolist() == [6]
 
 
+def counts_outside_their_range(m, device):
+    """A sequence brings between none and all of the T new tokens, whatever its count says: no row of
+    another sequence, or of none, is taken for its last one, and the lengths stay true."""
+    ids = torch.randint(0, 64, (3, 6), generator=torch.Generator().manual_seed(3)).to(device)
+    held = lambda *v: torch.tensor(v, device=device)  # noqa: E731
+    a, b = m.new_cache(batch=3), m.new_cache(batch=3)
+    for part, counts, same in ((ids[:, :4], (4, -2, 7), (4, 0, 4)), (ids[:, 4:], (2**33 + 1, 2, 1), (2, 2, 1))):
+        got = m.decode(part, a, held(*counts))._data
+        want = m.decode(part, b, held(*same))._data
+        assert torch.equal(got[[0, 2]], want[[0, 2]])
+        assert a.lengths.tolist() == b.lengths.tolist()
+    assert a.lengths.tolist() == [6, 2, 5]
+    assert torch.equal(m.decode(ids[:, :1], a)._data, m.decode(ids[:, :1], b, tensor([1, 1, 1]).torch().long().to(device))._data)
+
+
+def test_cpu_counts_outside_their_range():
+    counts_outside_their_range(lm(), "cpu")
+
+
 def test_generate_samples_and_defaults_to_greedy():
     m = lm()
     prompt = tensor([1, 2, 3])
@@ -284,6 +303,11 @@ def test_captured_steps_and_eager_ones_mix(prompt, status_ok):
     assert not cache.is_empty
     with pytest.raises(ValueError, match="do not fit"):
         gpu.decode(torch.zeros(1, 279, dtype=torch.int64), cache)
+
+
+@pytest.mark.gpu
+def test_counts_outside_their_range(status_ok):
+    counts_outside_their_range(lm(features=128).to("cuda", dtype="bf16"), "cuda")
 
 
 @pytest.mark.gpu

@@ -165,7 +165,7 @@ class QuantizedKVCache:
             raise RuntimeError(f"counts are on {counts.device}, the cache on {self.device}")
         if counts.dtype == torch.int32 and counts.is_contiguous():
             return counts
-        return counts.to(torch.int32).contiguous()
+        return counts.clamp(-(2**31), 2**31 - 1).to(torch.int32).contiguous()  # (nothing wraps round)
 
     def _check_rows(self, t, name: str, heads: int | None) -> torch.Tensor:
         """t as [batch, tokens, heads (None: any), head_dim] on the cache's device."""
@@ -186,6 +186,13 @@ class QuantizedKVCache:
         used = (self._host_length or 0) if self._known() else 0
         if used + tokens > self.max_len:
             raise ValueError(f"{tokens} more tokens do not fit: {used} of {self.max_len} are used")
+
+    def admit(self, tokens: int, counts=None) -> torch.Tensor | None:
+        """For a model's step of `tokens` new tokens: ``counts`` as every call understands them (int32,
+        between 0 and `tokens`), for ``append``, ``attend`` and ``advance``."""
+        if counts is None:
+            return None
+        return self._check_counts(counts).clamp(0, tokens)
 
     # --------------------------------------------------------------- calls
     def append(self, layer: int, k, v, counts=None) -> None:

@@ -323,8 +323,9 @@ class LMEngine:
     # ------------------------------------------------------------- decode
     def decode(self, ids: torch.Tensor, cache, counts: torch.Tensor | None = None) -> torch.Tensor:
         """Logits [B, V] after the last of each sequence's new tokens ids [B, T]
-        (of which sequence b brings counts[b]); `cache` (QuantizedKVCache)
-        receives their keys and values and counts them.
+        (of which sequence b brings counts[b], held to 0..T; with none it has no
+        logits of its own); `cache` (QuantizedKVCache) receives their keys and
+        values and counts them.
 
         Into an empty cache the tokens attend to one another's own keys and
         values (flash attention); later ones attend over the cache."""
@@ -333,9 +334,10 @@ class LMEngine:
         s = self.spec
         B, T = ids.shape
         H, D = s.heads, s.head_dim
+        counts = cache.admit(T, counts)
         fresh = cache.is_empty
         pos = cache.lengths if T == 1 else cache.lengths[:, None] + torch.arange(T, device=ids.device)
-        pos = pos.reshape(-1).clamp(max=s.max_seq_len - 1)  # padding may run past the last position
+        pos = pos.reshape(-1).clamp(0, s.max_seq_len - 1)  # padding may run past the last position
         x = K.embedding(ids.reshape(-1).contiguous(), self.E, self.P.index_select(0, pos), B * T)
         for i, blk in enumerate(self.blocks):
             h, _ = K.rmsnorm(x, blk["ln1"], s.eps)

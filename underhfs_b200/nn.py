@@ -716,7 +716,8 @@ class TransformerLM(Module):
 
         ``token_ids`` [B, T] follow the tokens that ``cache`` (from ``new_cache``)
         holds, and are added to it; sequence b brings only its first counts[b]
-        tokens (int tensor on the model's device; at least 1).  No gradients."""
+        tokens (int tensor on the model's device; held to 0..T, and one with none of
+        its own gets no logits of its own).  No gradients."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
         if ids.dim() != 2 or ids.shape[0] != cache.batch or ids.shape[1] < 1:
             raise ValueError(f"decode expects token ids [{cache.batch}, tokens], got {list(ids.shape)}")
@@ -733,7 +734,8 @@ class TransformerLM(Module):
                 logits = self._engine.decode(ids, cache, counts)
                 return Tensor._wrap(logits, like=like, backend="native_cuda", op="transformer_lm", parents=(like,))
             B, T = ids.shape
-            pos = (cache.lengths[:, None].long() + torch.arange(T)).clamp(max=self.max_seq_len - 1)
+            counts = cache.admit(T, counts)
+            pos = (cache.lengths[:, None].long() + torch.arange(T)).clamp(0, self.max_seq_len - 1)
             x = self.token_embedding(Tensor._wrap(ids)) + self.position_embedding(Tensor._wrap(pos))
             for i, block in enumerate(self.blocks):
                 x = x + block.attn.decode(block.attn_norm(x), cache, i, counts)
