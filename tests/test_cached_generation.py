@@ -99,6 +99,35 @@ def test_cpu_counts_outside_their_range():
     counts_outside_their_range(lm(), "cpu")
 
 
+def past_the_end(m, device):
+    """Ragged sequences: the step that does not fit is refused and leaves the cache as it was."""
+    ids = torch.randint(0, 64, (2, 6), generator=torch.Generator().manual_seed(3)).to(device)
+    held = lambda *v: torch.tensor(v, device=device)  # noqa: E731
+    cache = m.new_cache(batch=2, max_len=10)
+    m.decode(ids, cache, held(6, 3))
+    for _ in range(4):
+        m.decode(ids[:, :1], cache)
+    for counts in (None, held(1, 0), held(2, 2)):
+        with pytest.raises(ValueError, match="do not fit"):
+            m.decode(ids[:, :1 if counts is None else 2], cache, counts)
+        assert cache.lengths.tolist() == [10, 7]
+    m.decode(ids[:, :4], cache, held(0, 2))  # (padded beyond the end, but what counts fits)
+    assert cache.lengths.tolist() == [10, 9]
+    with pytest.raises(ValueError, match="do not fit"):
+        m.decode(ids[:, :1], cache)
+    cache.lengths.copy_(torch.tensor([3, 9], dtype=torch.int32))
+    m.decode(ids[:, :1], cache)
+    with pytest.raises(ValueError, match="do not fit"):
+        m.decode(ids[:, :1], cache)
+    cache.reset()
+    m.decode(ids, cache)
+    assert cache.lengths.tolist() == [6, 6]
+
+
+def test_cpu_past_the_end_of_ragged_sequences():
+    past_the_end(lm(), "cpu")
+
+
 def test_generate_samples_and_defaults_to_greedy():
     m = lm()
     prompt = tensor([1, 2, 3])
@@ -308,6 +337,28 @@ def test_captured_steps_and_eager_ones_mix(prompt, status_ok):
 @pytest.mark.gpu
 def test_counts_outside_their_range(status_ok):
     counts_outside_their_range(lm(features=128).to("cuda", dtype="bf16"), "cuda")
+
+
+@pytest.mark.gpu
+def test_past_the_end_of_ragged_sequences(status_ok):
+    past_the_end(lm(features=128).to("cuda", dtype="bf16"), "cuda")
+
+
+@pytest.mark.gpu
+def test_ragged_steps_do_not_wait_for_the_device(status_ok):
+    """Room is counted on the host: lengths are read back only where a sequence may be at its end."""
+    m = lm(features=128).to("cuda", dtype="bf16")
+    ids = torch.randint(0, 64, (2, 6)).cuda()
+    cache, counts = m.new_cache(batch=2), torch.tensor([6, 3], device="cuda")
+    m.decode(ids, cache, counts)
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(5):
+            m.decode(ids, cache, counts)
+            m.decode(ids[:, :1], cache)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert cache.lengths.tolist() == [41, 23]
 
 
 @pytest.mark.gpu

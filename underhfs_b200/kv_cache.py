@@ -86,7 +86,7 @@ class QuantizedKVCache:
             self.lengths = torch.zeros((self.batch,), dtype=torch.int32, device=self.device)
         # A captured step changes the lengths at every replay, which the host does not see
         self._captured = False
-        self._note(0)
+        self._note(0, 0)
 
     @property
     def pages(self) -> torch.Tensor:
@@ -113,10 +113,11 @@ class QuantizedKVCache:
             self._lengths = value.clone() if value.is_inference() else value.contiguous()
         self._version = -1
 
-    # What the host knows of the lengths: their common value, None where they differ.  It holds for
-    # one version of the tensor, so writes from outside are noticed.
-    def _note(self, length: int | None) -> None:
-        self._host_length = length
+    # What the host knows of the lengths: their common value (None where they differ) and a number that
+    # none passes (None: not known).  It holds for one version of the tensor, so writes from
+    # outside are noticed.
+    def _note(self, length: int | None, bound: int | None) -> None:
+        self._host_length, self._host_bound = length, bound
         self._version = self._lengths._version
 
     def _known(self) -> bool:
@@ -189,10 +190,24 @@ class QuantizedKVCache:
 
     def admit(self, tokens: int, counts=None) -> torch.Tensor | None:
         """For a model's step of `tokens` new tokens: ``counts`` as every call understands them (int32,
-        between 0 and `tokens`), for ``append``, ``attend`` and ``advance``."""
-        if counts is None:
-            return None
-        return self._check_counts(counts).clamp(0, tokens)
+        between 0 and `tokens`), for ``append``, ``attend`` and ``advance``.
+
+        Raises where they do not fit.  The lengths are read back for that only when the host's
+        bound on them leaves it open (ragged sequences near the end, lengths written from
+        outside), and never while a step is captured: what replays put past the end is
+        left out and reported in the device status word."""
+        if counts is not None:
+            counts = self._check_counts(counts).clamp(0, tokens)
+        bound = self._host_bound if self._known() else None
+        if (bound is None or bound + tokens > self.max_len) and not self._capturing():
+            held = self._lengths.tolist()
+            new = [tokens] * self.batch if counts is None else counts.tolist()
+            for used, n in zip(held, new):
+                if used + n > self.max_len:
+                    raise ValueError(f"{n} more tokens do not fit: {used} of {self.max_len} are used")
+            if not self._captured:
+                self._note(held[0] if len(set(held)) == 1 else None, max(held))
+        return counts
 
     # --------------------------------------------------------------- calls
     def append(self, layer: int, k, v, counts=None) -> None:
@@ -285,30 +300,31 @@ class QuantizedKVCache:
                 return K.kv4_read(self._layer_pages[layer], start, count, self.head_dim, dtype)
         return tuple(x[layer, :, start : start + count].to(dtype) for x in (self._k, self._v))
 
-    def advance(self, tokens) -> None:
-        """Count the appended tokens as part of the sequences: a number for all, or an int tensor [batch]."""
+    def advance(self, tokens, *, at_most: int | None = None) -> None:
+        """Count the appended tokens as part of the sequences: a number for all, or an int tensor
+        [batch], of which the caller may know that none is above ``at_most``."""
         if isinstance(tokens, int):
             if tokens < 0:
                 raise ValueError(f"tokens must not be negative, got {tokens}")
             self._check_room(tokens)
+            length, at_most = self._host_length, tokens
         else:
-            tokens = self._check_counts(tokens)
-        known = self._known()
+            tokens, length = self._check_counts(tokens), None
+        known, bound = self._known(), self._host_bound
         with self._on_device():
             self._lengths += tokens
         if self._capturing():
             self._captured = True  # replays count too
-        elif known and isinstance(tokens, int) and self._host_length is not None:
-            self._note(self._host_length + tokens)
         elif known:
-            self._note(None)
+            self._note(None if length is None else length + tokens,
+                       None if bound is None or at_most is None else bound + at_most)
 
     def set_host_length(self, tokens: int | None) -> None:
-        """Tell the host side how many tokens every sequence holds (None: not all the same)
+        """Tell the host side how many tokens every sequence holds (None: not known)
         after a captured graph has advanced the lengths on the device.  From here on the cache
         counts along again and reads nothing back: call it after the last replay."""
         self._captured = False
-        self._note(tokens)
+        self._note(tokens, tokens)
 
     def reset(self) -> None:
         """Forget every token (the memory is kept and written over)."""
@@ -317,7 +333,7 @@ class QuantizedKVCache:
         if self._capturing():
             self._captured = True
         else:
-            self._note(0)
+            self._note(0, 0)
 
 
 __all__ = ["QuantizedKVCache", "quantize_groups", "GROUP", "PAGE", "RANGE"]

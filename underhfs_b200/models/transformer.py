@@ -355,7 +355,7 @@ class LMEngine:
         if T > 1:
             first = torch.arange(B, device=ids.device) * T
             x = x.index_select(0, first + T - 1 if counts is None else first + (counts - 1).clamp(min=0))
-        cache.advance(T if counts is None else counts)
+        cache.advance(T if counts is None else counts, at_most=T)
         h, _ = K.rmsnorm(x, self.lnf, s.eps)
         return K.linear_fwd(h, self.Wh, None)
 

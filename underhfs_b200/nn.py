@@ -717,7 +717,9 @@ class TransformerLM(Module):
         ``token_ids`` [B, T] follow the tokens that ``cache`` (from ``new_cache``)
         holds, and are added to it; sequence b brings only its first counts[b]
         tokens (int tensor on the model's device; held to 0..T, and one with none of
-        its own gets no logits of its own).  No gradients."""
+        its own gets no logits of its own).  A step that does not fit the cache is
+        refused (in a captured one, which the host does not see, the tokens past the end
+        are left out and reported in the device status word).  No gradients."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
         if ids.dim() != 2 or ids.shape[0] != cache.batch or ids.shape[1] < 1:
             raise ValueError(f"decode expects token ids [{cache.batch}, tokens], got {list(ids.shape)}")
@@ -741,7 +743,7 @@ class TransformerLM(Module):
                 x = x + block.attn.decode(block.attn_norm(x), cache, i, counts)
                 x = x + block.mlp(block.mlp_norm(x))
             last = torch.full((B,), T - 1) if counts is None else (counts.long() - 1).clamp(min=0)
-            cache.advance(T if counts is None else counts)
+            cache.advance(T if counts is None else counts, at_most=T)
             h = self.norm(Tensor._wrap(x._data[torch.arange(B), last], like=x))
             head_w = like if self.tied else self.head.weight
             return _wrap(_linear_t(h._data, head_w._data, None), h, "linear", (h, head_w))
