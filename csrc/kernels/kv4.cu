@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
 // So K is not rounded, and for V only P s and lo + 8 s are.
 // Every warp works alone: it owns a ring of pages filled by bulk copies and takes
 // every n-th page of the block's share (n warps), with its own running maximum (raised
-// only when a score exceeds it by 2^2, which keeps P s in fp16's range) and sum.  The warps of a block are joined in
+// only when a score exceeds it by 2^2) and sum.  The warps of a block are joined in
 // shared memory and the blocks of a cluster, which share one head's tokens, through
 // distributed shared memory: one launch, no workspace, no atomics, and a sum order
 // that depends on sizes only.
@@ -325,7 +325,13 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
 // 4 sequences, 32 / 8 x 128: 42 us (three query tiles read each page).
 constexpr int kMaxWarps = 8;  // per block
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescale = 2.0f;  // s <= 2 * kRange / 15 = 8192
+constexpr float kRescale = 2.0f;
+// P goes in as 2^kRaise P, so that P s, an fp16 number, stays a normal one for small P and s (V of
+// about 1e-4 over 32768 keys, scores of standard deviation 2.5: error 4e-2 of the output without, the
+// result's own rounding with).  P <= 2^kRescale, so that s < kRaiseS leaves it within fp16's range; where
+// a query sees a token of larger s (at most 2 * kRange / 15 = 8192), its power is lowered.
+constexpr int kRaise = 10;
+constexpr uint32_t kRaiseS = 18;  // exponent field of 8, the first s that is too large
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -507,7 +513,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
   for (int i = 0; i < NG; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[i][j >> 2][j & 3] = 0.f;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  // per query: maximum so far, what is subtracted from the scores (0 while there is none), log2 of P's factor
+  float m_run[2] = {-INFINITY, -INFINITY}, base[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f};
+  int raise[2] = {kRaise, kRaise};
   const int prow = (g & 1) ? (g >> 1) + 4 : (g >> 1);  // token of product row g within 8
 
   int n_done = 0;
@@ -578,13 +586,43 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
 #pragma unroll
       for (int w = 4; w <= 16; w <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], w));
     }
-    if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kRescale || mx[1] > m_run[1] + kRescale)) {
+    bool rescale = mx[0] > m_run[0] + kRescale || mx[1] > m_run[1] + kRescale;
+    // some s of the page at kRaiseS or above (adding the complement carries into the sign bits)?
+    uint32_t vs[NG / 2], large = 0;
+    load_words<NG / 2>(vs, pg + F::kVS + lane * (2 * NG));
+#pragma unroll
+    for (int n = 0; n < NG / 2; ++n) large |= vs[n] + (32u - kRaiseS) * 0x04000400u;
+    if (__any_sync(0xffffffffu, (large & 0x80008000u) != 0)) {
+      // the largest exponent of s among the tokens that each query sees
+      uint32_t top[2] = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint16_t* sv = reinterpret_cast<const uint16_t*>(pg + F::kVS);
+        uint32_t x = 0;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) x = max(x, (uint32_t)sv[vslot<D>(e * 8 + prow, gi)] >> 10);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (s[e >> 1][(e & 1) * 2 + c] > -INFINITY) top[c] = max(top[c], x);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int w = 4; w <= 16; w <<= 1) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], w));
+        const int room = kRaise + (int)kRaiseS - 1 - (int)top[c];
+        rescale |= room < raise[c];
+        raise[c] = min(raise[c], room);
+      }
+    }
+    if (__any_sync(0xffffffffu, rescale)) {
       float alpha[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const float m_new = fmaxf(m_run[c], mx[c]);
-        alpha[c] = m_new == -INFINITY ? 1.f : ex2_approx(m_run[c] - m_new);
+        const float b_new = m_new == -INFINITY ? 0.f : m_new - (float)raise[c];
+        alpha[c] = m_run[c] == -INFINITY ? 1.f : ex2_approx(base[c] - b_new);  // (no maximum: the sums are 0)
         m_run[c] = m_new;
+        base[c] = b_new;
         l_run[c] *= alpha[c];
       }
 #pragma unroll
@@ -594,7 +632,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
 #pragma unroll
       for (int j = 0; j < 4; ++j) o_lo[j] *= alpha[j & 1];
     }
-    const float base[2] = {m_run[0] == -INFINITY ? 0.f : m_run[0], m_run[1] == -INFINITY ? 0.f : m_run[1]};
     // O^T += (s V)^T P^T: lane's tokens t, t + 4, t + 8, t + 12 of 16, channels 4 g .. + 3 of each group
     constexpr int NW = D / 64;  // words per lane and token
 #pragma unroll
@@ -686,7 +723,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
           make_float4(fmaf(o[gi][0][c], kCodeUnit, lo_sum[gi][c]), fmaf(o[gi][0][2 + c], kCodeUnit / 16, lo_sum[gi][c]),
                       fmaf(o[gi][1][c], kCodeUnit, lo_sum[gi][c]), fmaf(o[gi][1][2 + c], kCodeUnit / 16, lo_sum[gi][c]));
     if (g == 0) {
-      wm[warp * 8 + col] = m_run[c];
+      wm[warp * 8 + col] = m_run[c] == -INFINITY ? -INFINITY : base[c];
       wl[warp * 8 + col] = l_run[c];
     }
   }

@@ -288,6 +288,65 @@ def test_attention_strides_scale_and_large_queries(status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,size", [(4096, 1.0), (4096, 1e-2), (4096, 1e-4), (32768, 1e-3), (32768, 1e-4), (32768, 30.0)])
+def test_attention_keeps_small_and_large_values(n, size, D, status):
+    """Long contexts whose probabilities span many powers of two (scores of standard deviation 2.5), with
+    values of any size: the error is that of the roundings, not of fp16's range.
+
+    In the 2-norm over thousands of outputs, independent roundings add by their squares: of each token
+    P s (8 steps at most) and lo + 8 s, H16 of themselves or 2^-25 where they are below fp16's normal range;
+    P s enters as at least 2^10 times itself, P at least its ratio to the largest: its 2^-25 is
+    2^-35 of the largest probability.  Twice that, and the result's own rounding.  (40 sequences: a
+    warp has an eighth of the keys, and one maximum for them.)"""
+    B, Hkv, G = 40, 4, 2
+    cache = QuantizedKVCache(1, B, Hkv, D, n)
+    k, v = randn(1, n, Hkv, D, seed=1), (size * randn(1, n, Hkv, D, seed=2).float()).bfloat16()
+    cache.append(0, k.expand(B, -1, -1, -1), v.expand(B, -1, -1, -1))
+    cache.advance(n - 1)
+    q = (2.5 * randn(B, 1, Hkv * G, D, seed=3).float()).bfloat16()
+    got = cache.attend(0, q)[:, 0].double().view(B, Hkv, G, D)
+    kk, vv = (t[0].double() for t in cache.read(0, dtype=torch.float32))
+    p = torch.softmax(torch.einsum("bhgd,nhd->bhgn", q.double().view(B, Hkv, G, D), kk) * D**-0.5, -1)
+    o = torch.einsum("bhgn,nhd->bhgd", p, vv)
+    g = vv.unflatten(-1, (-1, 32))
+    lo, step = g.amin(-1, keepdim=True), (g.amax(-1, keepdim=True) - g.amin(-1, keepdim=True)) / 15
+    mid = (lo + 8 * step).abs()
+    part = ((H16 * 8 * step) ** 2 + torch.maximum(H16 * mid, torch.full_like(mid, 2.0**-25)) ** 2).expand(g.shape).flatten(-2)
+    small = (8 * 2.0**-35 * n**0.5 * p.amax(-1)).norm() * D**0.5
+    spread = torch.einsum("bhgn,nhd->bhgd", p**2, part).sqrt().norm() + small
+    assert (got - o).norm() <= torch.finfo(torch.bfloat16).eps / 2 * o.norm() + 2 * spread
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_over_values_of_all_sizes_at_once(D, dtype, status):
+    """Tokens of ordinary values, then some thousands of times larger (to the format's range), then ordinary
+    ones: nothing overflows, and a query that does not see the large ones has the bits it has without them."""
+    lens, tq = [900, 700], [6, 6]
+    q = randn(2, 6, 4, D, seed=60, dtype=dtype)
+    outs = []
+    for large in (1.0, 100.0, 3000.0, RANGE / 5):
+        cache = QuantizedKVCache(1, 2, 2, D, 900)
+        k, v = randn(2, 900, 2, D, seed=61, dtype=dtype), randn(2, 900, 2, D, seed=62, dtype=dtype)
+        for at in (5, 211, 450, 691, 897):  # (the last two are seen by some of the new tokens only)
+            v[:, at] = (large * v[:, at].float()).to(dtype)
+        n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        cache.append(0, k, v, counts=n)
+        cache.advance(n - 6)
+        for window in (None, 400):
+            got = cache.attend(0, q, window=window)
+            assert got.isfinite().all()
+            check_attend(cache, q, got, lens, tq, window, 0)
+        outs.append(cache.attend(0, q, window=60))
+    # window 60 of sequence 1: positions 694 .. 699 see 635 .. 699 at most; token 691 is in all of them;
+    # of sequence 0: 894 .. 899 see 835 .. 899, token 897 from the fourth query on
+    for o in outs[1:]:
+        assert torch.equal(o[0, :3], outs[0][0, :3]) and not torch.equal(o[0, 3:], outs[0][0, 3:])
+
+
+@pytest.mark.gpu
 def test_masked_tokens_may_hold_anything(status):
     """NaN and infinities behind the window, behind the sequence and in another sequence change nothing."""
     lens, tq = [200, 90], [1, 1]
