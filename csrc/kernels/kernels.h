@@ -139,6 +139,7 @@ struct Kv4Append {
   unsigned char* pages;
   const int *lengths, *counts;
   int B, T, H, pages_per_head;
+  int t_begin;           // set by the launcher: first token of this launch
   int capacity;          // tokens; rows that would go past it are reported and left out
   DeviceStatus* status;  // set by the launcher
 };
@@ -146,6 +147,7 @@ struct Kv4Read {
   const unsigned char* pages;
   void *k, *v;  // [B, n, H, D], contiguous
   int B, n, H, pages_per_head, start;
+  int t_begin;  // set by the launcher
 };
 struct Kv4Attend {
   const void* q;  // [B, Tq, Hq, D] with element strides, D contiguous

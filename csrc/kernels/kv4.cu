@@ -73,7 +73,7 @@ struct Place {
   bool on;
 };
 template <int D, int kRows>
-__device__ __forceinline__ Place<D> place(int H) {
+__device__ __forceinline__ Place<D> place(int H, int t_begin) {
   constexpr int LPR = D / 8;
   const int span = H * LPR, per_block = span < 256 ? 256 / span : 1;  // runs of tokens per block
   int u = blockIdx.x * 256 + threadIdx.x, run = 0;
@@ -81,7 +81,7 @@ __device__ __forceinline__ Place<D> place(int H) {
     run = (int)threadIdx.x / span;
     u = (int)threadIdx.x - run * span;
   }
-  return Place<D>{u / LPR, u % LPR, ((int)blockIdx.y * per_block + run) * kRows, u < span && run < per_block};
+  return Place<D>{u / LPR, u % LPR, t_begin + ((int)blockIdx.y * per_block + run) * kRows, u < span && run < per_block};
 }
 
 // y + kMagic has round(y) in its low bits, for |y| < 2^22
@@ -196,7 +196,7 @@ template <int D, typename T, int kRows>
 __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4Append a) {
   using F = Kv4<D>;
   constexpr int LPR = D / 8;  // threads per row
-  const Place<D> pl = place<D, kRows>(a.H);
+  const Place<D> pl = place<D, kRows>(a.H, a.t_begin);
   const int lw = pl.lw, gi = lw / 4, b = blockIdx.z;  // channels [8 lw, 8 lw + 8)
   const int count = a.counts != nullptr ? min(a.counts[b], a.T) : a.T;
   const long long start = a.lengths[b];
@@ -261,7 +261,7 @@ template <int D, typename T, int kRows>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
   using F = Kv4<D>;
   constexpr int LPR = D / 8;
-  const Place<D> pl = place<D, kRows>(a.H);
+  const Place<D> pl = place<D, kRows>(a.H, a.t_begin);
   if (!pl.on) return;
   const int lw = pl.lw, gi = lw / 4, b = blockIdx.z;
   const unsigned char* head = a.pages + ((long long)b * a.H + pl.h) * a.pages_per_head * F::kBytes;
@@ -815,12 +815,22 @@ void check_rows(const void* p, int elem, long long sb, long long st, long long s
     throw std::runtime_error(std::string(what) + ": rows must be 16-byte aligned");
 }
 
-// The grid of place<D, rows>: x over heads, y over runs of tokens, z over sequences
-dim3 row_grid(int B, int tokens, int H, int D, int rows, const char* what) {
-  const int span = H * (D / 8), per_block = span < 256 ? 256 / span : 1;
-  const long long y = ((long long)tokens + per_block * rows - 1) / (per_block * rows);
-  if (H > (1 << 24) || y > 65535 || B > 65535) throw std::runtime_error(std::string(what) + ": too many rows");
-  return dim3((unsigned)((span + 255) / 256), (unsigned)y, (unsigned)B);
+// Calls launch(grid of place<D, rows>, first sequence, its number, first token) for all tokens of
+// all sequences: x over heads, y over runs of tokens, z over sequences.  One launch, unless there are more runs or
+// sequences than the 65535 of y and z (262140 tokens of 16-bit type).
+template <class Launch>
+void for_row_grids(int B, int tokens, int H, int D, int rows, const char* what, Launch&& launch) {
+  constexpr int kMaxGrid = 65535;
+  if (H > (1 << 24)) throw std::runtime_error(std::string(what) + ": too many heads");
+  const int span = H * (D / 8), per_run = (span < 256 ? 256 / span : 1) * rows;  // tokens
+  const int step = kMaxGrid * per_run;
+  for (int b = 0; b < B; b += kMaxGrid) {
+    const int nb = B - b < kMaxGrid ? B - b : kMaxGrid;
+    for (long long t = 0; t < tokens; t += step) {
+      const int n = tokens - t < step ? (int)(tokens - t) : step;
+      launch(dim3((unsigned)((span + 255) / 256), (unsigned)((n + per_run - 1) / per_run), (unsigned)nb), b, nb, (int)t);
+    }
+  }
 }
 
 }  // namespace
@@ -845,27 +855,44 @@ void kv4_append(const Kv4Append& p, int dtype, int D, cudaStream_t s) {
     if (x < 0 || x > 0x7fffffffll) throw std::runtime_error("kv4 append: strides of tokens and heads must fit 32 bits");
   UHFS_KV4_TYPES(dtype, {
     constexpr int kRows = sizeof(T) == 2 ? 4 : 2;
-    const dim3 grid = row_grid(p.B, p.T, p.H, D, kRows, "kv4 append");
-    if (D == 64) kv4_append_kernel<64, T, kRows><<<grid, 256, 0, s>>>(a);
-    else kv4_append_kernel<128, T, kRows><<<grid, 256, 0, s>>>(a);
+    for_row_grids(p.B, p.T, p.H, D, kRows, "kv4 append", [&](dim3 grid, int b, int nb, int t) {
+      a.B = nb;
+      a.t_begin = t;
+      a.k = static_cast<const T*>(p.k) + b * p.k_stride_b;
+      a.v = static_cast<const T*>(p.v) + b * p.v_stride_b;
+      a.pages = p.pages + (long long)b * p.H * p.pages_per_head * (40 * D);
+      a.lengths = p.lengths + b;
+      if (p.counts != nullptr) a.counts = p.counts + b;
+      if (D == 64) kv4_append_kernel<64, T, kRows><<<grid, 256, 0, s>>>(a);
+      else kv4_append_kernel<128, T, kRows><<<grid, 256, 0, s>>>(a);
+      note_launch();
+      UHFS_CUDA_CHECK(cudaGetLastError());
+    });
   });
-  note_launch();
-  UHFS_CUDA_CHECK(cudaGetLastError());
 }
 
-void kv4_read(const Kv4Read& a, int dtype, int D, cudaStream_t s) {
-  if (a.B <= 0 || a.n <= 0 || a.H <= 0) return;
-  check_shape(D, a.pages, "kv4 read");
-  if (a.start < 0 || (long long)a.start + a.n > (long long)a.pages_per_head * kPage)
+void kv4_read(const Kv4Read& p, int dtype, int D, cudaStream_t s) {
+  if (p.B <= 0 || p.n <= 0 || p.H <= 0) return;
+  check_shape(D, p.pages, "kv4 read");
+  if (p.start < 0 || (long long)p.start + p.n > (long long)p.pages_per_head * kPage)
     throw std::runtime_error("kv4 read: tokens outside the cache");
-  check_rows(a.k, 4, 0, 0, 0, "kv4 read");
-  check_rows(a.v, 4, 0, 0, 0, "kv4 read");
+  check_rows(p.k, 4, 0, 0, 0, "kv4 read");
+  check_rows(p.v, 4, 0, 0, 0, "kv4 read");
   constexpr int kRows = 4;
-  const dim3 grid = row_grid(a.B, a.n, a.H, D, kRows, "kv4 read");
-  UHFS_KV4_TYPES(dtype, if (D == 64) kv4_read_kernel<64, T, kRows><<<grid, 256, 0, s>>>(a);
-                 else kv4_read_kernel<128, T, kRows><<<grid, 256, 0, s>>>(a));
-  note_launch();
-  UHFS_CUDA_CHECK(cudaGetLastError());
+  Kv4Read a = p;
+  UHFS_KV4_TYPES(dtype, {
+    for_row_grids(p.B, p.n, p.H, D, kRows, "kv4 read", [&](dim3 grid, int b, int nb, int t) {
+      a.B = nb;
+      a.t_begin = t;
+      a.pages = p.pages + (long long)b * p.H * p.pages_per_head * (40 * D);
+      a.k = static_cast<T*>(p.k) + (long long)b * p.n * p.H * D;
+      a.v = static_cast<T*>(p.v) + (long long)b * p.n * p.H * D;
+      if (D == 64) kv4_read_kernel<64, T, kRows><<<grid, 256, 0, s>>>(a);
+      else kv4_read_kernel<128, T, kRows><<<grid, 256, 0, s>>>(a);
+      note_launch();
+      UHFS_CUDA_CHECK(cudaGetLastError());
+    });
+  });
 }
 
 void kv4_attend(const Kv4Attend& p, int dtype, int D, cudaStream_t s) {

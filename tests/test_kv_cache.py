@@ -399,6 +399,44 @@ def test_offsets_beyond_32_bits(status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 131_070 + 3), (torch.bfloat16, 262_140 + 5)])
+def test_more_tokens_than_one_grid(dtype, n, status):
+    """Appends and reads of more runs of tokens than a grid has in one dimension."""
+    cache = QuantizedKVCache(1, 1, 16, 128, n + 1)
+    x = randn(1, 1009, 16, 128, seed=1, dtype=dtype)
+    k = torch.cat([x] * (n // 1009 + 1), 1)[:, :n]
+    cache.append(0, k, -k, counts=torch.tensor([n - 1], dtype=torch.int32, device="cuda"))
+    want = quantize_groups(x), quantize_groups(-x)
+    for got, w in zip(cache.read(0, dtype=torch.float16), want):
+        assert got.shape[1] == n + 1
+        for at in (0, 130 * 1009, n // 1009 * 1009):
+            part = got[:, at : min(at + 1009, n - 1)]
+            assert torch.equal(part, w[:, : part.shape[1]].half())
+        assert (got[:, n - 1 :] == 0).all()
+    cache.advance(n - 1)
+    cache.append(0, x[:, :2], x[:, 1:3])
+    for got, w in zip(cache.read(0, n - 1, 2, dtype=torch.float32), (x[:, :2], x[:, 1:3])):
+        assert torch.equal(got, quantize_groups(w).float())
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_one_grid(status):
+    B = 65_535 + 9
+    cache = QuantizedKVCache(1, B, 1, 64, 3)
+    k, v = randn(B, 2, 1, 64, seed=1), randn(B, 2, 1, 64, seed=2)
+    cache.append(0, k, v, counts=2 - torch.arange(B, device="cuda") % 2)
+    for got, x in zip(cache.read(0, 0, 2, dtype=torch.bfloat16), (k, v)):
+        want = quantize_groups(x).bfloat16()
+        want[1::2, 1] = 0
+        assert torch.equal(got, want)
+    # one visible token: its own value, but for the roundings of s (code - 8) and lo + 8 s and the result's
+    got, want = cache.attend(0, k[:, :1]).double(), cache.read(0, 0, 1, dtype=torch.float32)[1].double()
+    top = want.unflatten(-1, (-1, 32)).abs().amax(-1, keepdim=True)  # 8 s + |lo + 8 s| <= 3 of the largest
+    err = (3 * H16 * top).expand(B, 1, 1, 2, 32).flatten(-2) + 2.0**-8 * want.abs() + 1e-6
+    assert ((got - want).abs() <= 1.01 * err).all()
+
+
+@pytest.mark.gpu
 def test_captured_decoding_and_two_streams(status):
     """A captured step (append, attend, advance) replays with the lengths it finds on the device;
     two caches on two streams do not disturb each other."""
