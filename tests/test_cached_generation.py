@@ -362,6 +362,54 @@ def test_ragged_steps_do_not_wait_for_the_device(status_ok):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("other", ["allocates", "waits", "generates", "waits for the device"])
+def test_generate_beside_another_thread(other, status_ok):
+    """The captured steps of one thread and what another does meanwhile leave each other alone; a wait for the
+    whole device, which CUDA refuses during any capture, costs the capture but no token."""
+    import threading
+
+    _, m = gpu_pair()
+    x = torch.randn(64, 64, device="cuda")
+    kw = dict(cache="int4", temperature=0.9, top_p=0.95)
+    want = [m.generate(tensor([3, 1, 4]), 40, seed=s, **kw)._storage for s in range(6)]
+    torch.cuda.synchronize()
+    done, failed = threading.Event(), []
+
+    def beside():
+        n = 0
+        try:
+            while not done.is_set():
+                n += 1
+                if other == "allocates":
+                    torch.empty(n % 61 + 1, 1 << 20, device="cuda")
+                    if n % 50 == 0:
+                        torch.cuda.empty_cache()
+                elif other == "waits":
+                    assert x.sum().item() is not None
+                elif other == "generates":
+                    assert m.generate(tensor([3, 1, 4]), 40, seed=n % 6, **kw)._storage == want[n % 6]
+                else:
+                    try:
+                        torch.cuda.synchronize()
+                    except RuntimeError:
+                        pass
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    t = threading.Thread(target=beside)
+    t.start()
+    try:
+        for _ in range(3):
+            for s in range(6):
+                assert m.generate(tensor([3, 1, 4]), 40, seed=s, **kw)._storage == want[s]
+    finally:
+        done.set()
+        t.join()
+    assert not failed, failed
+    assert torch.cuda.current_stream() == torch.cuda.default_stream()
+
+
+@pytest.mark.gpu
 def test_cache_needs_the_engine_on_cuda():
     m = lm(features=64, heads=1).to("cuda")
     with pytest.raises(ValueError, match="bf16 engine"):

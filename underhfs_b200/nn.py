@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+import threading
 from collections import OrderedDict
 from dataclasses import dataclass
 from typing import Any, Iterable, Iterator
@@ -761,7 +762,9 @@ class TransformerLM(Module):
         ``cache="int4"`` (or a batch-1 cache of ``new_cache``, which is reset) keeps
         their keys and values in 4 bits and runs new tokens only; prompt and new
         tokens then have to fit the cache.  On CUDA the steps of such a run are
-        one captured graph."""
+        one captured graph.  Threads may generate side by side; during a capture (some
+        milliseconds) CUDA refuses another thread's wait for the whole device, and torch
+        its CUDA random numbers."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
         if ids.dim() != 1:
             raise ValueError("TransformerLM.generate expects 1D token ids")
@@ -828,13 +831,30 @@ class TransformerLM(Module):
                     graph.replay()
                 else:
                     choose(self.decode(token, cache))
-                    if dev.type == "cuda" and n - i > 4:  # the capture costs a few eager steps
-                        graph = torch.cuda.CUDAGraph()
-                        with torch.cuda.graph(graph):
-                            choose(self.decode(token, cache))
+                    if dev.type == "cuda" and i == 1 and n > 5:  # the capture costs a few eager steps
+                        graph = _captured(lambda: choose(self.decode(token, cache)))
                 out[i : i + 1].copy_(token[0])
             cache.set_host_length(len(prompt) + n - 1)  # replays advanced the device's lengths only
             return [int(v) for v in out.tolist()]
+
+
+_CAPTURE = threading.Lock()  # one capture at a time: each begins with a wait for the whole device
+
+
+def _captured(step) -> "torch.cuda.CUDAGraph | None":
+    """`step` as a graph, or None where another thread broke the capture.  Nothing of it has run.
+
+    Other threads may launch, allocate and wait for their streams meanwhile (the global error mode would
+    refuse that, and end the capture).  A wait for the whole device is refused in any mode and
+    ends the capture."""
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with _CAPTURE, torch.cuda.stream(torch.cuda.current_stream()):  # (a failed capture leaves its stream set)
+            with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+                step()
+    except RuntimeError:
+        return None
+    return graph
 
 
 def _require_cuda(device: Device) -> None:
