@@ -156,6 +156,18 @@ def test_generate_over_the_cache_on_the_cpu():
     assert m.generate(prompt, 0, cache="int4")._storage == [5, 6, 7, 8]
 
 
+@pytest.mark.parametrize("cache", [None, "int4"])
+@pytest.mark.parametrize("kw,match", [
+    (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(top_p=7.0), "top_p"), (dict(top_p=-0.5), "top_p"), (dict(top_k=-3), "top_k"), (dict(min_p=2.0), "min_p"),
+    (dict(temperature=0.5, min_p=float("nan")), "min_p")])
+@pytest.mark.parametrize("n", [0, 3])
+def test_generate_refuses_settings_with_and_without_a_cache(kw, match, cache, n):
+    """Greedy decoding uses none of them, but a wrong one is refused all the same."""
+    with pytest.raises(ValueError, match=match):
+        lm().generate(tensor([1, 2]), n, cache=cache, **kw)
+
+
 def test_refusals():
     m = lm()
     with pytest.raises(ValueError, match="do not fit"):

@@ -84,7 +84,18 @@ def softmax(input: Tensor) -> Tensor:
     return input.softmax()
 
 
-def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dtype, low: float, high: float):
+_SETTINGS = {"temperature": (0.0, 1e30), "top_k": (0, 2**31 - 1), "top_p": (0.0, 1.0), "min_p": (0.0, 1.0)}
+
+
+def check_sampling(**settings) -> None:
+    """Raise ValueError for a sampling setting, given as a number, that ``sample`` would refuse."""
+    for name, value in settings.items():
+        low, high = _SETTINGS[name]
+        if not isinstance(value, (torch.Tensor, Tensor)) and not low <= value <= high:  # False for NaN
+            raise ValueError(f"{name} must lie in [{low:g}, {high:g}], got {value}")
+
+
+def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dtype):
     """A sampling setting: a checked number, or a tensor with one value per row."""
     if not isinstance(value, (int, float)):
         value = value._data if isinstance(value, Tensor) else value
@@ -99,8 +110,9 @@ def _setting(value, name: str, rows: int, device: torch.device, dtype: torch.dty
         if dtype == torch.int32 and value.dtype == torch.int64:
             value = value.clamp(0, 2**31 - 1)  # <= 0 is off
         return value.to(dtype).contiguous()
-    if not low <= value <= high:  # False for NaN
-        raise ValueError(f"{name} must lie in [{low:g}, {high:g}], got {value}")
+    low, high = _SETTINGS[name]
+    if not low <= value <= high:
+        check_sampling(**{name: value})
     return int(value) if dtype == torch.int32 else float(value)
 
 
@@ -140,10 +152,10 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -
     real = torch.float32 if x.is_cuda else torch.float64
     if u.dim() != 1 or u.dtype != real or not u.is_contiguous():
         u = u.detach().reshape(-1).to(real).contiguous()
-    temperature = _setting(temperature, "temperature", rows, x.device, real, 0.0, 1e30)
-    top_k = _setting(top_k, "top_k", rows, x.device, torch.int32, 0, 2**31 - 1)
-    top_p = _setting(top_p, "top_p", rows, x.device, real, 0.0, 1.0)
-    min_p = _setting(min_p, "min_p", rows, x.device, real, 0.0, 1.0)
+    temperature = _setting(temperature, "temperature", rows, x.device, real)
+    top_k = _setting(top_k, "top_k", rows, x.device, torch.int32)
+    top_p = _setting(top_p, "top_p", rows, x.device, real)
+    min_p = _setting(min_p, "min_p", rows, x.device, real)
     if x.is_cuda:
         from underhfs_b200.ops import kernels as K
 

@@ -769,6 +769,8 @@ class TransformerLM(Module):
         if ids.dim() != 1:
             raise ValueError("TransformerLM.generate expects 1D token ids")
         generated = [int(v) for v in ids.tolist()]
+        kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        F.check_sampling(**kw)
         if uniform is not None:
             uniform = (uniform._data if isinstance(uniform, Tensor) else uniform).reshape(-1)
             if uniform.numel() != max_new_tokens:
@@ -784,7 +786,6 @@ class TransformerLM(Module):
             uniform = torch.zeros(max(0, max_new_tokens))
         dev = (self._engine_device() if self._engine is not None else self.token_embedding.weight._data.device)
         uniform = uniform.to(dev)
-        kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         if cache is not None:
             return tensor(generated + self._generate_cached(generated, max_new_tokens, uniform, kw, cache))
         with torch.no_grad():
