@@ -168,6 +168,23 @@ def test_generate_refuses_settings_with_and_without_a_cache(kw, match, cache, n)
         lm().generate(tensor([1, 2]), n, cache=cache, **kw)
 
 
+def test_a_refused_generate_leaves_the_cache_as_it_was():
+    m = lm()
+    ids = torch.randint(0, 64, (1, 9), generator=torch.Generator().manual_seed(3))
+    cache, other = m.new_cache(max_len=20), lm(layers=1).new_cache(max_len=30)
+    pair = m.new_cache(batch=2, max_len=20)
+    m.decode(ids, cache)
+    want = cache.read(0, 0, 9, dtype=torch.float64)[0].clone()
+    lm(layers=1).decode(ids, other)
+    pair.advance(4)
+    for c, prompt, n, match in ((cache, [1] * 15, 6, "do not fit"), (cache, [], 2, "prompt"), (other, [1, 2], 3, "another model"),
+                                (pair, [1, 2], 3, "token ids")):
+        with pytest.raises(ValueError, match=match):
+            m.generate(torch.tensor(prompt, dtype=torch.int64), n, cache=c)
+    assert cache.lengths.tolist() == [9] and other.lengths.tolist() == [9] and pair.lengths.tolist() == [4, 4]
+    assert torch.equal(cache.read(0, 0, 9, dtype=torch.float64)[0], want)
+
+
 def test_refusals():
     m = lm()
     with pytest.raises(ValueError, match="do not fit"):
@@ -419,6 +436,17 @@ def test_generate_beside_another_thread(other, status_ok):
         t.join()
     assert not failed, failed
     assert torch.cuda.current_stream() == torch.cuda.default_stream()
+
+
+@pytest.mark.gpu
+def test_a_cache_on_another_device_is_refused_and_kept():
+    m = lm(features=128).to("cuda", dtype="bf16")
+    cache = lm(features=128).new_cache()
+    cache.advance(5)
+    for call in (lambda: m.decode(torch.zeros(1, 2, dtype=torch.int64), cache), lambda: m.generate(tensor([1]), 2, cache=cache)):
+        with pytest.raises(RuntimeError, match="the cache is on cpu"):
+            call()
+    assert cache.lengths.tolist() == [5]
 
 
 @pytest.mark.gpu

@@ -712,6 +712,18 @@ class TransformerLM(Module):
         return QuantizedKVCache(len(self.blocks), batch, self.heads, self.features // self.heads,
                                 self.max_seq_len if max_len is None else max_len, device=w.device)
 
+    def _check_decode(self, ids: torch.Tensor, cache) -> None:
+        if ids.dim() != 2 or ids.shape[0] != cache.batch or ids.shape[1] < 1:
+            raise ValueError(f"decode expects token ids [{cache.batch}, tokens], got {list(ids.shape)}")
+        if (cache.layers, cache.kv_heads, cache.head_dim) != (len(self.blocks), self.heads, self.features // self.heads):
+            raise ValueError("the cache was made for another model")
+        if cache.max_len > self.max_seq_len:
+            raise ValueError(f"the cache holds {cache.max_len} tokens, the model has {self.max_seq_len} positions")
+        if cache.device != self.token_embedding.weight._data.device:
+            raise RuntimeError(f"the cache is on {cache.device}, the model on {self.token_embedding.weight._data.device}")
+        if self._zero3 is not None:
+            raise RuntimeError("a ZeRO-3 sharded model does not decode over a cache")
+
     def decode(self, token_ids: Tensor | torch.Tensor, cache, counts: torch.Tensor | None = None) -> Tensor:
         """Logits [B, V] after the last new token of each of B sequences.
 
@@ -722,14 +734,7 @@ class TransformerLM(Module):
         refused (in a captured one, which the host does not see, the tokens past the end
         are left out and reported in the device status word).  No gradients."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
-        if ids.dim() != 2 or ids.shape[0] != cache.batch or ids.shape[1] < 1:
-            raise ValueError(f"decode expects token ids [{cache.batch}, tokens], got {list(ids.shape)}")
-        if (cache.layers, cache.kv_heads, cache.head_dim) != (len(self.blocks), self.heads, self.features // self.heads):
-            raise ValueError("the cache was made for another model")
-        if cache.max_len > self.max_seq_len:
-            raise ValueError(f"the cache holds {cache.max_len} tokens, the model has {self.max_seq_len} positions")
-        if self._zero3 is not None:
-            raise RuntimeError("a ZeRO-3 sharded model does not decode over a cache")
+        self._check_decode(ids, cache)
         like = self.token_embedding.weight
         ids = ids.to(cache.device, torch.int64)
         with torch.no_grad():
@@ -805,10 +810,11 @@ class TransformerLM(Module):
             if cache != "int4":
                 raise ValueError(f"unknown cache {cache!r} (int4)")
             cache = self.new_cache(max_len=min(self.max_seq_len, max(len(prompt) + n, 1)))
-        else:
-            cache.reset()
         if len(prompt) + n > cache.max_len:
             raise ValueError(f"{len(prompt)} + {n} tokens do not fit the cache of {cache.max_len}")
+        ids = torch.tensor([prompt], dtype=torch.int64, device=cache.device)
+        self._check_decode(ids, cache)
+        cache.reset()  # (not before: a refused call leaves it as it was)
         if n < 1:
             return []
         dev = cache.device
@@ -823,7 +829,7 @@ class TransformerLM(Module):
         guard = torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext()
         with torch.no_grad(), guard:
             u.copy_(uniform[:1])
-            choose(self.decode(torch.tensor([prompt], dtype=torch.int64, device=dev), cache))
+            choose(self.decode(ids, cache))
             out[:1].copy_(token[0])
             graph = None
             for i in range(1, n):
