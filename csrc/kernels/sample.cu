@@ -22,12 +22,12 @@
 // Weights 2^((l - max) log2(e) / T) are 64-bit integers in units of 2^-44: sums do
 // not depend on the order of atomics, blocks or warps, and a token on the border of
 // top-p or of u is decided alike however the row was split.  A weight is right to
-// 2^-29 of itself (fp32 pairs for the exponent, a table of 64 powers, a short series;
+// 2^-29 of itself and one unit (fp32 pairs for the exponent, a table of 64 powers, a short series;
 // tests/test_sampling.py restates the steps), so that a sum over n tokens of like
 // weight is right to about 2^-29 / sqrt(n) and the choice is that of exact arithmetic
-// but for u in a few parts in 10^8.  (With the weights in 64-bit floating point 256 x 32000 of
+// but for u or top-p in a few parts in 10^8.  (With the weights in 64-bit floating point 256 x 32000 of
 // mixed settings took 58 us where these took 46.)  For top-p's border they are rounded to
-// 2^-31, so that a histogram holds its sums as two 32-bit words of 16 bits of the weights
+// 2^-31 (see coarse()), so that a histogram holds its sums as two 32-bit words of 16 bits of the weights
 // each: 32-bit adds are what shared memory does fast, and they bound a flat row's pass.
 //
 // Measured: 1 x 32000 bf16 with top-p 16 us (bound by the barriers of the cluster, about 2 K
@@ -123,8 +123,12 @@ struct Row {
 struct Weights {
   u64 a, b;
 };
-// in units of 2^-31
-__device__ __forceinline__ uint32_t coarse(u64 w) { return (uint32_t)((w + (1u << 12)) >> 13); }
+// In units of 2^-31, rounded up or down by the token's place: the multiples of the golden ratio spread the
+// thresholds so evenly that a run of equal weights sums to within some units of the truth, however small they are.
+// (Rounded to the nearest, 131071 weights of 0.44 units were nothing, and of 1.6 two units each.)
+__device__ __forceinline__ uint32_t coarse(u64 w, int idx) {
+  return (uint32_t)((w + ((uint32_t)idx * 0x9E3779B1u >> 19)) >> 13);
+}
 template <bool kExact>
 __device__ __forceinline__ Weights weights(const Row& row, const uint32_t* powers, float la, float lb) {
   auto both = [](float x) { return make_float2(x, x); };
@@ -462,17 +466,17 @@ struct Sampler {
   template <bool kWeights, class Goal>
   __device__ __forceinline__ u64 select(u64 border, Goal&& goal_of) {
     constexpr int kWords = kWeights ? 2 : 1;
-    auto val = [&](float l) -> uint32_t { return kWeights ? coarse(weigh(l)) : 1; };
+    auto val = [&](float l, int idx) -> uint32_t { return kWeights ? coarse(weigh(l), idx) : 1; };
     clear(kWords, kBins);
     if (listed != nullptr || !kWeights || border != 0) {
       each([&](float l, int idx) {
-        if (l > -INFINITY && order_key(l, idx) >= border) add<kWeights>(bin_of(l), val(l));
+        if (l > -INFINITY && order_key(l, idx) >= border) add<kWeights>(bin_of(l), val(l, idx));
       });
     } else {
-      each_pair([&](float la, float lb, int) {
+      each_pair([&](float la, float lb, int idx) {
         const Weights w = weigh(la, lb);
-        add<kWeights>(bin_of(la), coarse(w.a));
-        add<kWeights>(bin_of(lb), coarse(w.b));
+        add<kWeights>(bin_of(la), coarse(w.a, idx));
+        add<kWeights>(bin_of(lb), coarse(w.b, idx + 1));
       });
     }
     const u64 goal = find_bin(kWords, kBins, goal_of);
@@ -492,7 +496,7 @@ struct Sampler {
           list);
       if (n <= kCap) {
         u64* w = sh.hist;  // (every block has passed the gather's barrier: the histogram has been read)
-        for (int i = threadIdx.x; i < n; i += kThreads) w[i] = val(key_logit(list[i]));
+        for (int i = threadIdx.x; i < n; i += kThreads) w[i] = val(key_logit(list[i]), key_index(list[i]));
         if (threadIdx.x == 0) sh.border = 0;
         __syncthreads();
         // the blocks share the tokens out; eight lanes compare one with all others
@@ -527,7 +531,7 @@ struct Sampler {
       each([&](float l, int idx) {
         const u64 key = order_key(l, idx);
         if (l > -INFINITY && key >= border && bin_of(l) == bin && (shift == 56 || (key >> (shift + 8)) == prefix))
-          add<kWeights>(255 - (int)((key >> shift) & 255), val(l));
+          add<kWeights>(255 - (int)((key >> shift) & 255), val(l, idx));
       });
       const u64 left = sum;
       find_bin(kWords, 256, [&](u64) { return goal - left; });

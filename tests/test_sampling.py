@@ -165,6 +165,22 @@ def test_kernel_weights_hold_their_error(temperature, kind):
         assert kernel_weight(far, mx, temperature, exact).tolist() == [0, 0, 0]
 
 
+def test_rounded_weights_of_a_run_sum_to_its_sum():
+    """The kernel's rounding of weights to 2^-31 for top-p's border (coarse() in csrc/kernels/sample.cu): over any run of
+    tokens the sum is off by some units, whatever the weight.  (The thresholds are multiples of the golden ratio
+    modulo 1: of n of them, n x lie below x but for a few times log n.)"""
+    import numpy as np
+
+    idx = np.arange(327680, dtype=np.int64)
+    t = ((idx * 0x9E3779B1) & 0xFFFFFFFF) >> 19
+    assert t.max() == 2**13 - 1 and ((2**44 + t) >> 13).max() == 2**31  # the largest stays the largest
+    g = np.random.default_rng(0)
+    for w in [1, 2, 3629, 4095, 4096, 4097, 8191, 8192, 12345, *g.integers(1, 1 << 16, 20)]:
+        run = np.concatenate(([0], np.cumsum((int(w) + t) >> 13)))
+        off = run - np.arange(len(run)) * (w / 8192)
+        assert off.max() - off.min() <= 32  # of any run: off at its end minus off at its start
+
+
 @pytest.mark.parametrize("kw,match", [
     (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
     (dict(top_k=-1), "top_k"), (dict(top_p=1.5), "top_p"), (dict(top_p=-0.1), "top_p"),
@@ -333,6 +349,24 @@ def test_gpu_captured_and_replayed_and_other_stream(status_ok):
         got = F.sample(xd, ud, top_p=0.9).torch()
     side.synchronize()
     assert got.tolist() == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,vocab", [(1, 131072), (70, 131072), (3, 40001), (300, 50000)])
+@pytest.mark.parametrize("tail,p", [(-22.3, 0.99999), (-21.0, 0.9999), (-21.0, 0.99995), (-20.6, 0.99992), (-23.75, 0.999999)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gpu_top_p_over_a_long_flat_tail(n, vocab, tail, p, dtype, status_ok):
+    """One likely token and a long tail whose weights are near the unit of top-p's histogram: the tokens kept are
+    those of exact arithmetic but for 64 units of 2^-31 of the largest weight (a run's rounding, at
+    the two ends of what is summed), 2^-29 of the tail and 2^-44 a token."""
+    x = torch.full((n, vocab), tail).to(dtype)
+    x[:, 0] = 0
+    w = math.exp(float(x[0, 1]))
+    last = F.sample(x.cuda(), torch.ones(n, device="cuda"), top_p=p).torch()  # u = 1: the last token kept
+    goal, off = p * (1 + (vocab - 1) * w), 64 * 2.0**-31 + (vocab - 1) * (w * 2.0**-29 + 2.0**-44)
+    fewest, most = (max(0, math.ceil((g - 1) / w)) for g in (goal - off, goal + off))
+    assert fewest <= last.min().item() and last.max().item() <= most, (fewest, last, most)
+    assert (last == last[0]).all()
 
 
 @pytest.mark.gpu
