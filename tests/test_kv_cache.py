@@ -1,6 +1,7 @@
 """The 4-bit key / value cache: write, read back, attention over it; CPU and CUDA."""
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -52,6 +53,42 @@ def test_quantised_special_values():
     assert (y[0] == 0).all() and (y[1] == 3).all() and (y[4] == 0).all()
     assert y[2, 0] == y[2, 2] == RANGE and y[2, 1] == -RANGE
     assert y[3, 0] == 0 and abs(y[3, 1] - 7) < 15 * 7 * H16
+
+
+def format_by_fractions(x):
+    """The documented format in exact arithmetic, group by group: lo = fp16(min), s = fp16(fp32(fp32(max - lo) *
+    fp32(1 / 15))), code = (x - lo) / s rounded half to even, held to 0..15."""
+    import numpy as np
+
+    def near(v):  # half to even
+        k = v.numerator // v.denominator
+        rest = v - k
+        return k + (rest > Fraction(1, 2) or (rest == Fraction(1, 2) and k % 2))
+
+    out = []
+    for row in x.reshape(-1, 32).float().numpy():
+        lo = np.float16(row.min())
+        s = np.float16(np.float32(row.max() - np.float32(lo)) * np.float32(1 / 15))
+        lo, s = Fraction(float(lo)), Fraction(float(s))
+        out.append([float(lo + s * max(0, min(15, near((Fraction(float(v)) - lo) / s) if s else 0))) for v in row])
+    return torch.tensor(out, dtype=torch.float64).view(x.shape)
+
+
+def format_inputs(dtype):
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(6, 40, 64, generator=g)
+    x[1] = x[1] * 1e-3 + 0.7
+    x[2] *= torch.logspace(-4, 4, 40).unsqueeze(1)
+    x[3] = (x[3] * 8).round() / 4
+    x[4] = torch.randint(0, 31, (40, 64), generator=g) * 0.5  # quotients on halves
+    x[5] = torch.randint(-3, 4, (40, 64), generator=g).float() * 1000
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantised_values_are_those_of_the_format(dtype):
+    x = format_inputs(dtype)
+    assert torch.equal(quantize_groups(x), format_by_fractions(x))
 
 
 def test_cpu_cache_holds_and_attends():
@@ -191,6 +228,16 @@ def test_special_values_are_stored_finite(status):
         cache.append(0, x.to(dtype), x.to(dtype))
         for got in cache.read(0, dtype=torch.float32):
             assert torch.equal(got, quantize_groups(x.to(dtype)).float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_stored_values_are_those_of_the_format(dtype, status):
+    x = format_inputs(dtype)
+    cache = QuantizedKVCache(1, 6, 1, 64, 40)
+    cache.append(0, x.unsqueeze(2).cuda(), -x.unsqueeze(2).cuda())
+    for got, want in zip(cache.read(0, dtype=torch.float32), (x, -x)):
+        assert torch.equal(got[:, :, 0].double().cpu(), format_by_fractions(want).float().double())
 
 
 def fill(B, keys, Hkv, D, lens, tq, dtype, seed=0):
