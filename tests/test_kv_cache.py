@@ -314,6 +314,18 @@ def test_attention(B, tq, lens, Hq, Hkv, D, window, sinks, dtype, status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(None, 0), (200, 5)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 2, 64), (6, 2, 128)])
+def test_attention_of_prompts_onto_a_filled_cache(Hq, Hkv, D, window, sinks, status):
+    """Hundreds of new tokens (many tiles of queries to a head) behind cached ones, ragged."""
+    lens, tq = [1500, 700], [601, 300]
+    cache = fill(2, 1600, Hkv, D, lens, tq, torch.bfloat16)
+    q = randn(2, 601, Hq, D, seed=57)
+    counts = torch.tensor(tq, dtype=torch.int32, device="cuda")
+    check_attend(cache, q, cache.attend(0, q, window=window, sinks=sinks, counts=counts), lens, tq, window, sinks)
+
+
+@pytest.mark.gpu
 def test_attention_strides_scale_and_large_queries(status):
     lens, tq = [300, 41], [2, 2]
     cache = fill(2, 320, 2, 64, lens, tq, torch.bfloat16)
