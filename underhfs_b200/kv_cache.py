@@ -38,6 +38,10 @@ def _raw(t) -> torch.Tensor:
 _HERE = contextlib.nullcontext()
 
 
+def _no_inference_mode():
+    return torch.inference_mode(False) if torch.is_inference_mode_enabled() else _HERE
+
+
 def quantize_groups(x: torch.Tensor) -> torch.Tensor:
     """The values (float64) that the 4-bit codes of x [..., D] stand for.
 
@@ -74,7 +78,7 @@ class QuantizedKVCache:
             raise ValueError(f"the CUDA cache takes head_dim 64 or 128, got {head_dim}")
         if not self._cuda and (self.head_dim < GROUP or self.head_dim % GROUP):
             raise ValueError(f"head_dim must be a multiple of {GROUP}, got {head_dim}")
-        with torch.inference_mode(False):  # inference tensors could not be written later, and count no versions
+        with _no_inference_mode():  # inference tensors could not be written later, and count no versions
             if self._cuda:
                 pages = (self.max_len + PAGE - 1) // PAGE
                 self.pages = torch.zeros((self.layers, self.batch, self.kv_heads, pages, 40 * self.head_dim),
@@ -109,7 +113,7 @@ class QuantizedKVCache:
         if value.shape != (self.batch,) or value.dtype != torch.int32 or value.device != self.device:
             raise ValueError(f"lengths must be int32 [{self.batch}] on {self.device}, got {value.dtype} "
                              f"{list(value.shape)} on {value.device}")
-        with torch.inference_mode(False):
+        with _no_inference_mode():
             self._lengths = value.clone() if value.is_inference() else value.contiguous()
         self._version = -1
 
@@ -124,7 +128,7 @@ class QuantizedKVCache:
         return not self._captured and self._version == self._lengths._version
 
     def _capturing(self) -> bool:
-        return self._cuda and torch.cuda.is_current_stream_capturing()
+        return self._cuda and torch._C._cuda_isCurrentStreamCapturing()
 
     @property
     def nbytes(self) -> int:
@@ -138,11 +142,9 @@ class QuantizedKVCache:
         """No sequence has a token.  Reads the lengths back where the host cannot know them: after
         they were written to, or once a step with ``advance`` was captured.  False while
         a step is captured, since it may be replayed on any lengths."""
-        if self._capturing():
-            return False
         if self._known():
-            return self._host_length == 0
-        return not bool(self._lengths.any())
+            return self._host_length == 0 and not self._capturing()
+        return not self._capturing() and not bool(self._lengths.any())
 
     # ------------------------------------------------------------- checks
     def _on_device(self):

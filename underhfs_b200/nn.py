@@ -806,7 +806,8 @@ class TransformerLM(Module):
     def _generate_cached(self, prompt: list[int], n: int, uniform: torch.Tensor, kw: dict, cache) -> list[int]:
         if not prompt:
             raise ValueError("generation over a cache needs a prompt")
-        if isinstance(cache, str):
+        given = not isinstance(cache, str)
+        if not given:
             if cache != "int4":
                 raise ValueError(f"unknown cache {cache!r} (int4)")
             cache = self.new_cache(max_len=min(self.max_seq_len, max(len(prompt) + n, 1)))
@@ -814,7 +815,8 @@ class TransformerLM(Module):
             raise ValueError(f"{len(prompt)} + {n} tokens do not fit the cache of {cache.max_len}")
         ids = torch.tensor([prompt], dtype=torch.int64, device=cache.device)
         self._check_decode(ids, cache)
-        cache.reset()  # (not before: a refused call leaves it as it was)
+        if given:
+            cache.reset()  # (not before: a refused call leaves it as it was)
         if n < 1:
             return []
         dev = cache.device
