@@ -63,9 +63,9 @@ __device__ __forceinline__ int vhalf(int c) {
 // cost some 12 instructions before they bound them: the threads of a block span the heads
 // (and, where those are few, several runs of tokens), so that a place costs no division by
 // the number of heads and is worked out once for kRows tokens, whose loads overlap (four for
-// 16-bit types: prompt write and read back of 8 x 2048, 16 x 128 took 92 us, 102 with one; two
-// of 32-bit ones, which need the registers of four).  Measured at that size: write 63 us, 2.8
-// TB/s, bound by its instructions (184 for 8 values, min and max, quotients and places
+// 16-bit types: prompt write and read back of 8 x 2048, 16 x 128 take 62 and 38 us, 73 and 41 with one; two
+// of 32-bit ones, which need the registers of four).  Measured at that size: write 62 us, 2.8
+// TB/s (fp32 52 in a graph, bf16 59), bound by its instructions (184 for 8 values, min and max, quotients and places
 // included), read back 38 us, 4.7 TB/s.
 template <int D>
 struct Place {
@@ -319,10 +319,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Read a) {
 // distributed shared memory: one launch, no workspace, no atomics, and a sum order
 // that depends on sizes only.
 //
-// Measured: 32 sequences of 2 to 4 K keys, 32 x 128: 121 us, 4.2 TB/s (the loads alone 96, the
+// Measured: 32 sequences of 2 to 4 K keys, 32 x 128: 122 us, 4.2 TB/s (the loads alone 96, the
 // arithmetic alone 113: 630 instructions a page at 16 warps an SM, waiting on one another
 // and on the integer pipe); 1 x 1000 keys, 12 x 64: 10 us; 5 new tokens over windows of 8192 of
-// 4 sequences, 32 / 8 x 128: 42 us (three query tiles read each page).
+// 4 sequences, 32 / 8 x 128: 41 us (three query tiles read each page).
 constexpr int kMaxWarps = 8;  // per block
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 2.0f;

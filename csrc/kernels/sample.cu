@@ -30,8 +30,8 @@
 // 2^-31 (see coarse()), so that a histogram holds its sums as two 32-bit words of 16 bits of the weights
 // each: 32-bit adds are what shared memory does fast, and they bound a flat row's pass.
 //
-// Measured: 1 x 32000 bf16 with top-p 16 us (bound by the barriers of the cluster, about 2 K
-// cycles each), 256 x 32000 bf16 of mixed settings 44, 64 x 131072 fp32 with top-p 70 (0.5 TB/s:
+// Measured: 1 x 32000 bf16 with top-p 17 us (bound by the barriers of the cluster, about 2 K
+// cycles each), 256 x 32000 bf16 of mixed settings 45, 64 x 131072 fp32 with top-p 69 (0.5 TB/s:
 // bound by the instructions of the weights and the histogram's atomics, with 32 warps an SM).
 #include <cfloat>
 #include <stdexcept>
@@ -889,9 +889,10 @@ void launch_sample(const SampleArgs& a, cudaStream_t s) {
     splits *= 2;
   if (rows * splits > 2 * 148) {
     // More blocks than run at once: fewer that read the row again from L2 instead of keeping it (2^16
-    // tokens to a block at most), where these are three quarters of what runs at once.  64 x 131072
-    // fp32: 64 us, 79 with slices; 256 x 50000 fp32: 80 and 122; 512 x 32000 fp32, top-k 50: 46 and
-    // 74; 100 x 131072 bf16, whose 200 blocks leave half the SMs one: 104 and 87.
+    // tokens to a block at most), where these are three quarters of what runs at once.  Rows that are in
+    // L2: 64 x 131072 fp32 69 us, 85 with slices; 256 x 50000 fp32 85 and 129; 512 x 32000 fp32, top-k 50,
+    // 37 and 60 (rows from memory: 90 and 91, 90 and 131, 42 and 67).  100 x 131072 bf16, whose 200
+    // blocks leave half the SMs one: 104 and 87.
     int few = 1;
     while (few < kMaxSplits && (rows * few * 2 <= 2 * 148 || vocab > few * 65536ll)) few *= 2;
     if (few < splits && rows * few * 4 >= 2 * 148 * 3) return launch_splits<T, false>(a, few, s);
