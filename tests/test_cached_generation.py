@@ -391,10 +391,9 @@ def test_ragged_steps_do_not_wait_for_the_device(status_ok):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("other", ["allocates", "waits", "generates", "waits for the device"])
+@pytest.mark.parametrize("other", ["allocates", "waits", "generates"])
 def test_generate_beside_another_thread(other, status_ok):
-    """The captured steps of one thread and what another does meanwhile leave each other alone; a wait for the
-    whole device, which CUDA refuses during any capture, costs the capture but no token."""
+    """The captured steps of one thread and what another does meanwhile leave each other alone."""
     import threading
 
     _, m = gpu_pair()
@@ -415,13 +414,8 @@ def test_generate_beside_another_thread(other, status_ok):
                         torch.cuda.empty_cache()
                 elif other == "waits":
                     assert x.sum().item() is not None
-                elif other == "generates":
-                    assert m.generate(tensor([3, 1, 4]), 40, seed=n % 6, **kw)._storage == want[n % 6]
                 else:
-                    try:
-                        torch.cuda.synchronize()
-                    except RuntimeError:
-                        pass
+                    assert m.generate(tensor([3, 1, 4]), 40, seed=n % 6, **kw)._storage == want[n % 6]
         except BaseException as e:  # noqa: BLE001
             failed.append(e)
 
@@ -435,6 +429,7 @@ def test_generate_beside_another_thread(other, status_ok):
         done.set()
         t.join()
     assert not failed, failed
+    assert torch.randn(3, device="cuda").isfinite().all()
     assert torch.cuda.current_stream() == torch.cuda.default_stream()
 
 

@@ -767,9 +767,11 @@ class TransformerLM(Module):
         ``cache="int4"`` (or a batch-1 cache of ``new_cache``, which is reset) keeps
         their keys and values in 4 bits and runs new tokens only; prompt and new
         tokens then have to fit the cache.  On CUDA the steps of such a run are
-        one captured graph.  Threads may generate side by side; during a capture (some
-        milliseconds) CUDA refuses another thread's wait for the whole device, and torch
-        its CUDA random numbers."""
+        one captured graph.  Threads may generate, launch, allocate and wait for their
+        streams side by side.  During a capture (some milliseconds a call) CUDA
+        refuses another thread's wait for the whole device, which ends the capture with an error, and
+        torch its CUDA random numbers: beside such threads take ``decode`` and
+        functional.sample step by step."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
         if ids.dim() != 1:
             raise ValueError("TransformerLM.generate expects 1D token ids")
@@ -841,29 +843,17 @@ class TransformerLM(Module):
                 else:
                     choose(self.decode(token, cache))
                     if dev.type == "cuda" and i == 1 and n > 5:  # the capture costs a few eager steps
-                        graph = _captured(lambda: choose(self.decode(token, cache)))
+                        graph = torch.cuda.CUDAGraph()
+                        # thread-local: in the global error mode, the default, what other threads
+                        # allocate or wait for meanwhile fails and ends the capture
+                        with _CAPTURE, torch.cuda.graph(graph, capture_error_mode="thread_local"):
+                            choose(self.decode(token, cache))
                 out[i : i + 1].copy_(token[0])
             cache.set_host_length(len(prompt) + n - 1)  # replays advanced the device's lengths only
             return [int(v) for v in out.tolist()]
 
 
 _CAPTURE = threading.Lock()  # one capture at a time: each begins with a wait for the whole device
-
-
-def _captured(step) -> "torch.cuda.CUDAGraph | None":
-    """`step` as a graph, or None where another thread broke the capture.  Nothing of it has run.
-
-    Other threads may launch, allocate and wait for their streams meanwhile (the global error mode would
-    refuse that, and end the capture).  A wait for the whole device is refused in any mode and
-    ends the capture."""
-    graph = torch.cuda.CUDAGraph()
-    try:
-        with _CAPTURE, torch.cuda.stream(torch.cuda.current_stream()):  # (a failed capture leaves its stream set)
-            with torch.cuda.graph(graph, capture_error_mode="thread_local"):
-                step()
-    except RuntimeError:
-        return None
-    return graph
 
 
 def _require_cuda(device: Device) -> None:
