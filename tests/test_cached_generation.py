@@ -185,6 +185,21 @@ def test_a_refused_generate_leaves_the_cache_as_it_was():
     assert torch.equal(cache.read(0, 0, 9, dtype=torch.float64)[0], want)
 
 
+def no_token_to_choose(m, kw):
+    with torch.no_grad():
+        m.norm.weight._data.fill_(float("nan"))  # logits of NaN
+    for cache in (None, "int4"):
+        with pytest.raises(ValueError, match="no token"):
+            m.generate(tensor([1, 2]), 9, cache=cache, temperature=0.7, **kw)
+    with pytest.raises(ValueError, match="no token"):
+        m.generate(tensor([1, 2]), 1, cache="int4")
+
+
+def test_cpu_generate_without_a_token_to_choose():
+    no_token_to_choose(lm(), {})
+    no_token_to_choose(lm(), dict(top_k=3, top_p=0.9))
+
+
 def test_refusals():
     m = lm()
     with pytest.raises(ValueError, match="do not fit"):
@@ -431,6 +446,14 @@ def test_generate_beside_another_thread(other, status_ok):
     assert not failed, failed
     assert torch.randn(3, device="cuda").isfinite().all()
     assert torch.cuda.current_stream() == torch.cuda.default_stream()
+
+
+@pytest.mark.gpu
+def test_generate_without_a_token_to_choose():
+    from underhfs_b200.ops._lib import core
+
+    no_token_to_choose(lm(features=128).to("cuda", dtype="bf16"), {})
+    core().device_status(True)  # the steps after it reported a token outside the vocabulary
 
 
 @pytest.mark.gpu

@@ -771,7 +771,9 @@ class TransformerLM(Module):
         streams side by side.  During a capture (some milliseconds a call) CUDA
         refuses another thread's wait for the whole device, which ends the capture with an error, and
         torch its CUDA random numbers: beside such threads take ``decode`` and
-        functional.sample step by step."""
+        functional.sample step by step.
+
+        Logits that leave no token to choose (all NaN or -inf) raise ValueError."""
         ids = token_ids._data if isinstance(token_ids, Tensor) else token_ids
         if ids.dim() != 1:
             raise ValueError("TransformerLM.generate expects 1D token ids")
@@ -800,7 +802,7 @@ class TransformerLM(Module):
                 context = generated[-self.max_seq_len:]
                 logits = self(torch.tensor(context, dtype=torch.int64, device=dev))
                 if temperature > 0:
-                    generated.append(int(F.sample(logits._data[-1], uniform[i], **kw).torch().item()))
+                    generated.append(_chosen(F.sample(logits._data[-1], uniform[i], **kw).torch().item()))
                 else:
                     generated.append(int(torch.argmax(logits._data[-1].float()).item()))
         return tensor(generated)
@@ -829,6 +831,8 @@ class TransformerLM(Module):
 
         def choose(logits: Tensor) -> None:
             token.copy_(F.sample(logits._data, u, **kw).torch().view(1, 1))
+            if dev.type != "cuda":
+                _chosen(token.item())
 
         guard = torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext()
         with torch.no_grad(), guard:
@@ -850,7 +854,13 @@ class TransformerLM(Module):
                             choose(self.decode(token, cache))
                 out[i : i + 1].copy_(token[0])
             cache.set_host_length(len(prompt) + n - 1)  # replays advanced the device's lengths only
-            return [int(v) for v in out.tolist()]
+            return [_chosen(v) for v in out.tolist()]
+
+
+def _chosen(token) -> int:
+    if token < 0:
+        raise ValueError("no token can be chosen: every logit is NaN or -inf")
+    return int(token)
 
 
 _CAPTURE = threading.Lock()  # one capture at a time: each begins with a wait for the whole device
