@@ -200,6 +200,16 @@ def test_cpu_generate_without_a_token_to_choose():
     no_token_to_choose(lm(), dict(top_k=3, top_p=0.9))
 
 
+def test_only_causal_attention_decodes():
+    from underhfs.kv_cache import QuantizedKVCache
+    from underhfs.nn import SelfAttention
+
+    cache = QuantizedKVCache(1, 1, 1, 32, 8, device="cpu")
+    with pytest.raises(ValueError, match="causal"):
+        SelfAttention(32).decode(tensor(torch.zeros(1, 2, 32)), cache, 0)
+    assert (cache.read(0)[0] == 0).all()
+
+
 def test_refusals():
     m = lm()
     with pytest.raises(ValueError, match="do not fit"):

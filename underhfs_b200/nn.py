@@ -367,6 +367,8 @@ class SelfAttention(Module):
     def decode(self, x: Tensor, cache, layer: int, counts: torch.Tensor | None = None) -> Tensor:
         """forward for new tokens x [batch, tokens, features] of sequences whose
         earlier keys and values are in ``cache`` (QuantizedKVCache); theirs are added."""
+        if not self.causal:
+            raise ValueError("decoding over a cache needs causal attention")
         t = x._data
         B, T, Fd = t.shape
         fresh = cache.is_empty
