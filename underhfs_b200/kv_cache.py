@@ -105,7 +105,7 @@ class QuantizedKVCache:
     @property
     def lengths(self) -> torch.Tensor:
         """Tokens of each sequence that ``advance`` has counted: int32 [batch], on the
-        cache's device.  It may be written to."""
+        cache's device.  It may be written to, but not by a captured step (which takes ``advance``)."""
         return self._lengths
 
     @lengths.setter
@@ -253,7 +253,8 @@ class QuantizedKVCache:
         heads a multiple of kv_heads, which consecutive query heads share) ->
         the same shape.  Token t of sequence b is at position lengths[b] + t and
         sees the keys up to its own; with ``window``, of those the last
-        ``window`` and the first ``sinks``.  Rows t >= counts[b] are zeros."""
+        ``window`` and the first ``sinks``.  Rows t >= counts[b] are zeros.  Tokens past
+        ``max_len`` see the keys that are there and are reported in the device status word.  No gradients."""
         self._check_layer(layer)
         q = self._check_rows(q, "q", None)
         heads, tokens = q.shape[2], q.shape[1]
