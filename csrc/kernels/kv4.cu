@@ -331,7 +331,7 @@ constexpr float kRescale = 2.0f;
 // result's own rounding with).  P <= 2^kRescale, so that s < kRaiseS leaves it within fp16's range; where
 // a query sees a token of larger s (at most 2 * kRange / 15 = 8192), its power is lowered.
 constexpr int kRaise = 10;
-constexpr uint32_t kRaiseS = 18;  // exponent field of 8, the first s that is too large
+constexpr int kRaiseS = 18;  // exponent field of 8, the first s that is too large
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -516,6 +516,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
   // per query: maximum so far, what is subtracted from the scores (0 while there is none), log2 of P's factor
   float m_run[2] = {-INFINITY, -INFINITY}, base[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f};
   int raise[2] = {kRaise, kRaise};
+  uint32_t headroom = (32 - kRaiseS) * 0x04000400u;  // brings the first s that some query has to lower its power for to 2^16
   const int prow = (g & 1) ? (g >> 1) + 4 : (g >> 1);  // token of product row g within 8
 
   int n_done = 0;
@@ -587,11 +588,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
       for (int w = 4; w <= 16; w <<= 1) mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xffffffffu, mx[c], w));
     }
     bool rescale = mx[0] > m_run[0] + kRescale || mx[1] > m_run[1] + kRescale;
-    // some s of the page at kRaiseS or above (adding the complement carries into the sign bits)?
+    // some s of the page too large for a query (the sum's sign bits)?
     uint32_t vs[NG / 2], large = 0;
     load_words<NG / 2>(vs, pg + F::kVS + lane * (2 * NG));
 #pragma unroll
-    for (int n = 0; n < NG / 2; ++n) large |= vs[n] + (32u - kRaiseS) * 0x04000400u;
+    for (int n = 0; n < NG / 2; ++n) large |= vs[n] + headroom;
     if (__any_sync(0xffffffffu, (large & 0x80008000u) != 0)) {
       // the largest exponent of s among the tokens that each query sees
       uint32_t top[2] = {0, 0};
@@ -609,10 +610,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) kv4_attend_kernel(const Kv4
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int w = 4; w <= 16; w <<= 1) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], w));
-        const int room = kRaise + (int)kRaiseS - 1 - (int)top[c];
+        const int room = kRaise + kRaiseS - 1 - (int)top[c];
         rescale |= room < raise[c];
         raise[c] = min(raise[c], room);
       }
+      // (pages of like scales do not come here again)
+      headroom = (32 - kRaiseS - kRaise + __reduce_max_sync(0xffffffffu, max(raise[0], raise[1]))) * 0x04000400u;
     }
     if (__any_sync(0xffffffffu, rescale)) {
       float alpha[2];
