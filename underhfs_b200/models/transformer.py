@@ -328,7 +328,8 @@ class LMEngine:
         values and counts them.
 
         Into an empty cache the tokens attend to one another's own keys and
-        values (flash attention); later ones attend over the cache."""
+        values (flash attention); later ones, and those of a captured step, whose
+        replays may find any lengths, attend over the cache."""
         if self.context_attention is not None:
             raise RuntimeError("context parallelism does not decode over a cache")
         s = self.spec
